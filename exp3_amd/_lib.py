@@ -18,7 +18,7 @@ SPX_OK = 0
 SPX_EINVAL = -1
 SPX_EUNSUPPORTED = -2
 SPX_ELAUNCH = -3
-ABI_VERSION = 9
+ABI_VERSION = 10
 # int32 counters behind the attention entry points' work_queue (SPX_WORK_QUEUE_INTS)
 WORK_QUEUE_INTS = 16
 
@@ -28,6 +28,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S = ctypes.POINTER(ctypes.c_int64)
+_L = ctypes.c_int64
 
 # name -> argument types (restype is int for all compute entry points)
 _PROTOTYPES = {
@@ -60,11 +61,17 @@ _PROTOTYPES = {
     "spx_sparse_attention_rescue": [_P, _S, _P, _P, _P, _S, _P, _S, _P, _P, _S, _P, _P, _I, _I,
                                     _I, _I, _I, _I, _I, _F, _P, _S, _P, _S, _P, _P],
     "spx_decode_attention": [_P, _S, _P, _S, _P, _S, _I, _I, _I, _I, _I, _F, _P, _P, _P],
+    "spx_paged_append": [_P, _S, _P, _S, _P, _S, _P, _P, _I, _I, _I, _P, _L, _I, _P, _P, _P, _P,
+                         _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
+    "spx_paged_gather": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P],
+    "spx_paged_attention": [_P, _S, _P, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
+                            _I, _I, _F, _P, _P, _P, _P],
 }
 
 # helpers without a status: sizes (int64)
 _SIZE_FUNCTIONS = {"spx_selector_workspace_bytes": [_I, _I, _I, _I],
                    "spx_decode_workspace_bytes": [_I, _I, _I, _I, _I],
+                   "spx_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
                    "spx_attention_queue_ints": [_I, _I, _I, _I, _I]}
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES) + tuple(_SIZE_FUNCTIONS) + ("spx_last_error",

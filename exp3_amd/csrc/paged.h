@@ -1,0 +1,51 @@
+// Paged KV cache shared by the append, gather and attention kernels.
+//
+// Pages: [pages, Hkv, page_size, D] bf16, or in 4 bits [pages, Hkv, page_size, D / 2] bytes
+// (E2M1, even dim in the low half) with scales [pages, Hkv, page_size, D / 32] (E8M0). A
+// (page, head) pair is one contiguous run of rows, so 16 consecutive tokens of a head are one
+// run of 4 KB (bf16, D = 128) or 1 KB + 64 bytes (4 bits).
+#pragma once
+
+#include "common.h"
+
+namespace spx {
+
+constexpr int kPagedGroup = 32;          // dims per scale of a 4-bit page
+constexpr int kPagedMinPage = 16, kPagedMaxPage = 1024;
+
+// Which tokens a call is about and where they are: token i of sequence b has position
+// starts[b] + i and is live if starts[b] >= 0, i < counts[b] (counts may be null) and the
+// position is within the table.
+struct PagedMap {
+  const int32_t* table;                  // [B, width], rows table_stride apart
+  int64_t table_stride;
+  const int32_t* starts;
+  const int32_t* counts;
+  int width, pages, page_shift, kv_heads;
+
+  __device__ __forceinline__ int64_t capacity() const { return (int64_t)width << page_shift; }
+  // Position of token i of sequence b, or -1.
+  __device__ __forceinline__ int position(int b, int i) const {
+    const int start = starts[b];
+    if (start < 0 || (counts != nullptr && i >= counts[b])) return -1;
+    const int64_t p = (int64_t)start + i;
+    return p < capacity() ? (int)p : -1;
+  }
+  // Page of a position, or -1 where the table names none.
+  __device__ __forceinline__ int page(int b, int p) const {
+    const int id = table[b * table_stride + (p >> page_shift)];
+    return (unsigned)id < (unsigned)pages ? id : -1;
+  }
+  // Row (of D elements) of a position of a KV head in the page arrays.
+  __device__ __forceinline__ int64_t row(int page_id, int head, int p) const {
+    return (((int64_t)page_id * kv_heads + head) << page_shift) + (p & ((1 << page_shift) - 1));
+  }
+};
+
+// Checks of the arguments that all entry points share; fills the map.
+int paged_map(PagedMap& m, const int32_t* page_table, int64_t table_stride, int table_width,
+              const int32_t* starts, const int32_t* counts, const void* key_pages,
+              const void* value_pages, const void* key_scales, const void* value_scales, int pages,
+              int page_size, int batch, int tokens, int kv_heads, int head_dim);
+
+}  // namespace spx

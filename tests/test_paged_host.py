@@ -1,0 +1,149 @@
+"""The paged cache on the host: what the functions and the C entry points refuse, before any
+launch, and the 64-bit reference's 4-bit grid against its definition."""
+
+import ctypes
+
+import pytest
+import torch
+
+from exp3_amd import _lib, paged
+import paged_reference as ref
+
+FAKE, OFF = 1 << 20, (1 << 20) + 8
+S4 = (ctypes.c_int64 * 4)(4096, 512, 128, 1)
+ODD = (ctypes.c_int64 * 4)(4096, 512, 132, 1)
+
+
+def _append(q=FAKE, k=FAKE, ks=S4, cos=FAKE, sin=FAKE, rope=(4096, 128, 0), table=(FAKE, 32, 32),
+            starts=FAKE, pages=(FAKE, FAKE, None, None), sizes=(64, 128), shape=(2, 1, 28, 4, 128),
+            q_out=FAKE, k_out=None):
+    return _lib.load().spx_paged_append(q, S4, k, ks, FAKE, S4, cos, sin, *rope, *table, starts,
+                                        None, *pages, *sizes, *shape, q_out, k_out, None)
+
+
+def _gather(table=(FAKE, 32, 32), pages=(FAKE, FAKE, None, None), sizes=(64, 128),
+            shape=(2, 1, 4, 128), out=FAKE):
+    return _lib.load().spx_paged_gather(*table, FAKE, None, *pages, *sizes, *shape, out, FAKE, None)
+
+
+def _attention(q=FAKE, qs=S4, table=(FAKE, 32, 32), pages=(FAKE, FAKE, None, None), sizes=(64, 128),
+               max_keys=0, shape=(2, 1, 28, 4, 128), workspace=FAKE, out=FAKE):
+    return _lib.load().spx_paged_attention(q, qs, *table, FAKE, None, *pages, *sizes, max_keys,
+                                           *shape, 0.1, workspace, out, None, None)
+
+
+@pytest.mark.parametrize("call,heads", ((_append, (28, 4)), (_gather, (4,)), (_attention, (28, 4))))
+def test_shared_arguments(call, heads):
+    unsupported, invalid = _lib.SPX_EUNSUPPORTED, _lib.SPX_EINVAL
+    for size in (8, 24, 100, 2048):
+        assert call(sizes=(64, size)) == unsupported and b"page_size" in _lib.load().spx_last_error()
+    assert call(shape=(2, 1, *heads, 64)) == unsupported
+    for shape in ((0, 1, *heads, 128), (2, 0, *heads, 128), (2, 1, *heads[:-1], 0, 128)):
+        assert call(shape=shape) == invalid
+    assert call(sizes=(0, 128)) == invalid
+    assert call(table=(None, 32, 32)) == call(table=(FAKE, 32, 0)) == invalid
+    assert call(table=(FAKE, 32, (1 << 23) + 1)) == invalid       # 2^30 + 128 positions
+    for pages in ((None, FAKE, None, None), (FAKE, OFF, None, None), (FAKE, FAKE, FAKE, None),
+                  (FAKE, FAKE, FAKE, FAKE + 4)):
+        assert call(pages=pages) == invalid
+
+
+def test_append_arguments():
+    unsupported, invalid = _lib.SPX_EUNSUPPORTED, _lib.SPX_EINVAL
+    assert _append(k=None) == _append(k=OFF) == _append(ks=ODD) == _append(starts=None) == invalid
+    assert _append(q_out=None) == _append(k_out=OFF) == _append(q=OFF) == invalid
+    assert _append(sin=None) == _append(cos=OFF) == invalid
+    assert _append(rope=(4095, 128, 0)) == invalid                # the table reaches 4096
+    for rotary in (0, 8, 120, 144):
+        assert _append(rope=(4096, rotary, 0)) == unsupported
+    assert _append(shape=(1 << 20, 1 << 10, 28, 4, 128)) == invalid
+
+
+def test_gather_and_attention_arguments():
+    invalid = _lib.SPX_EINVAL
+    assert _gather(out=None) == _gather(out=OFF) == invalid
+    assert _attention(q=None) == _attention(q=OFF) == _attention(qs=ODD) == invalid
+    assert _attention(out=None) == _attention(max_keys=-1) == invalid
+    assert _attention(shape=(2, 1, 27, 4, 128)) == _attention(shape=(1 << 16, 1 << 10, 32, 4, 128)) \
+        == invalid
+    size = _lib.load().spx_paged_attention_workspace_bytes
+    assert size(32, 128, 0, 2, 1, 28, 4, 128) >= 0
+    for bad in ((32, 128, 0, 2, 1, 27, 4, 128), (32, 128, 0, 0, 1, 28, 4, 128),
+                (32, 128, 0, 2, 1, 28, 4, 64), (32, 128, -1, 2, 1, 28, 4, 128)):
+        assert size(*bad) == -1
+
+
+def test_wrappers_refuse():
+    cache = paged.empty_pages(4, 16, 2, 128, "cpu")
+    x = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
+    table, starts = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for call in (lambda: paged.append_tokens(cache, table, starts, x, x),
+                 lambda: paged.gather_tokens(cache, table, starts, 1),
+                 lambda: paged.paged_attention(x, cache, table, starts, 0.1)):
+        with pytest.raises(ValueError, match="ROCm GPU"):
+            call()
+    for bad in ((4, 8, 2, 128), (4, 24, 2, 128), (4, 2048, 2, 128), (4, 16, 2, 64)):
+        with pytest.raises(ValueError, match="unsupported"):
+            paged.empty_pages(*bad, "cpu")
+
+
+def test_wrapper_checks_of_shapes():
+    """The checks that need no GPU tensors of their own, on the CPU."""
+    cpu = torch.device("cpu")
+    good = paged.empty_pages(4, 16, 2, 128, "cpu", four_bit=True)
+    assert paged._check_cache(good, cpu)[1:] == (2, 128)
+    assert (good.page_size, good.kv_heads, good.head_dim, good.four_bit) == (16, 2, 128, True)
+    half = paged.empty_pages(4, 16, 2, 256, "cpu")
+    assert paged._check_cache(half, cpu)[1:] == (2, 256) and half.head_dim == 256
+    bad = (paged.PagedCache(good.key_pages, good.value_pages, good.key_scales),
+           paged.PagedCache(good.key_pages, good.value_pages),
+           paged.PagedCache(half.key_pages, half.value_pages[:3]),
+           paged.PagedCache(half.key_pages.transpose(1, 2), half.value_pages.transpose(1, 2)),
+           paged.PagedCache(half.key_pages.half(), half.value_pages.half()),
+           paged.PagedCache(good.key_pages, good.value_pages, good.key_scales[..., :2],
+                            good.value_scales[..., :2]))
+    for cache in bad:
+        with pytest.raises(ValueError):
+            paged._check_cache(cache, cpu)
+    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    paged._check_map(table, starts, starts, 2, cpu)
+    paged._check_map(torch.zeros(2, 9, dtype=torch.int32)[:, 2:6], starts, None, 2, cpu)
+    for wrong in ((table.long(), starts, None), (table, starts.long(), None), (table[:1], starts, None),
+                  (table, starts[:1], None), (table, starts, starts.long()),
+                  (table.repeat(1, 2)[:, ::2], starts, None),
+                  (table, torch.zeros(4, dtype=torch.int32)[::2], None)):
+        with pytest.raises(ValueError):
+            paged._check_map(*wrong, 2, cpu)
+
+
+def test_rope_table_far_positions():
+    cos, sin = paged.rope_table(131072, 128)
+    angle = torch.tensor(131071.0, dtype=torch.float64) * \
+        1.0e6 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128)
+    # one rounding to fp32 of a value that fp64 has to 131072 x 2^-52
+    assert (cos[-1].double() - angle.cos()).abs().max() <= 2.0 ** -25 + 2.0 ** -34
+    assert (sin[-1].double() - angle.sin()).abs().max() <= 2.0 ** -25 + 2.0 ** -34
+    assert cos.shape == sin.shape == (131072, 64) and cos.dtype == torch.float32
+
+
+def test_reference_grid():
+    """Each value against all representable ones: none is nearer, ties have an even code."""
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(40, 32, generator=gen, dtype=torch.float64)
+    x[0, :17] = torch.tensor([0, .25, .75, 1.25, 1.75, 2.5, 3.5, 5, 6, 6.9, -.25, -.75, -2.5, -5,
+                              0.2500001, 2.4999, -0.0])
+    x[0, 17:] = 0.1
+    got = ref.four_bit(x)
+    assert got[0, :17].tolist() == [0, 0, 1, 1, 2, 2, 4, 4, 6, 6, 0, -1, -2, -4, 0.5, 2, 0]
+    top = x.abs().amax(-1)
+    step = 2.0 ** torch.ceil(torch.log2(top / 7))
+    step = torch.where(top / step >= 7, step * 2, step)
+    near = ((x.abs() / step[:, None])[..., None] - ref.GRID).abs().amin(-1)
+    assert torch.equal((x - got).abs() / step[:, None], near)
+    assert torch.equal(ref.four_bit(torch.zeros(1, 32)), torch.zeros(1, 32, dtype=torch.float64))
+    wild = torch.zeros(2, 64)
+    wild[0, 3], wild[1, 40] = float("inf"), float("nan")
+    out = ref.four_bit(wild)
+    assert torch.isnan(out[0, :32]).all() and torch.isnan(out[1, 32:]).all()
+    assert (out[0, 32:] == 0).all() and (out[1, :32] == 0).all()
+    assert ref.four_bit(torch.full((1, 32), 3.3e38, dtype=torch.float64)).max() == 6 * 2.0 ** 125
