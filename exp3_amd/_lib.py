@@ -71,7 +71,7 @@ _PROTOTYPES = {
 # helpers without a status: sizes (int64)
 _SIZE_FUNCTIONS = {"spx_selector_workspace_bytes": [_I, _I, _I, _I],
                    "spx_decode_workspace_bytes": [_I, _I, _I, _I, _I],
-                   "spx_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
+                   "spx_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I, _I],
                    "spx_attention_queue_ints": [_I, _I, _I, _I, _I]}
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES) + tuple(_SIZE_FUNCTIONS) + ("spx_last_error",

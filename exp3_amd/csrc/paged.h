@@ -42,6 +42,14 @@ struct PagedMap {
   }
 };
 
+// Eight 4-bit values as bf16: exact, a value has two bits.
+__device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+
 // Checks of the arguments that all entry points share; fills the map.
 int paged_map(PagedMap& m, const int32_t* page_table, int64_t table_stride, int table_width,
               const int32_t* starts, const int32_t* counts, const void* key_pages,

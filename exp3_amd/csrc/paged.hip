@@ -227,14 +227,6 @@ struct GatherArgs {
   uint16_t* v_out;
 };
 
-// Eight 4-bit values as bf16: exact, a value has two bits.
-__device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
-  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
-               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
-}
-
 template <int D, bool kFour>
 __global__ __launch_bounds__(kPagedThreads) void paged_gather_kernel(GatherArgs a) {
   constexpr int kPieces = D / 8, kRows = kPagedThreads / kPieces;

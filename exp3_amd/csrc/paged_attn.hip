@@ -1,10 +1,51 @@
-// Attention of new tokens over a paged KV cache (bf16 or 4-bit pages, fp32 softmax and
-// accumulation): one workgroup per (sequence, token, query head), one key per wave and step.
+// Attention of new tokens over a paged KV cache: decode steps and a few drafted tokens
+// (bf16 or 4-bit pages; bf16 queries and outputs, fp32 scores, softmax and accumulation).
+//
+// Columns n = i group + h of a KV head (token i of T, query head h of the group) share its K
+// and V; 16 of them are one tile. A stream is a (sequence, KV head, column tile), its work
+// ceil(keys / unit) units.
+//
+// Bound: HBM (each visible row of K and V once per column tile); with 4-bit pages the unpacking
+// is close behind.
+//   * The streams' units, in order, are dealt in equal runs to the workgroups of one grid that
+//     fills the chip. The lengths are device data, so every workgroup finds its run itself:
+//     a prefix sum over the batch in one wave (a load and some shuffles), no host
+//     synchronisation, and a captured launch can be replayed with other lengths. A stream
+//     that falls to one workgroup is written out directly; of the others each workgroup
+//     leaves at most two partial results (its run's first and last stream), joined by a
+//     second kernel in a fixed order.
+//   * A unit is a few 16-key tiles per wave, four waves. Page ids come from a register that holds
+//     those of the wave's next 64 tiles, so no load waits for a page table entry of its own.
+//   * Scores: S^T = K Q^T, v_mfma_f32_16x16x32_bf16, K rows as A operand straight from memory.
+//     The order of the dims in the sum is free: with 4-bit pages a lane takes 32 consecutive
+//     dims of a row, which are 16 bytes and one scale, widened exactly to bf16 by
+//     v_cvt_scalef32_pk_bf16_fp4 (two values and their scale an instruction).
+//   * P V, 4-bit pages: v_mfma_f32_16x16x32_bf16 over the keys of two tiles. Their scores lie
+//     in the lane as the A operand wants them; a lane holds its dims of the eight rows it needs,
+//     and byte permutes pair the keys. P is split into two bf16 parts (2^-16 left over, below
+//     the output's rounding; one part alone would add as much error as that rounding). bf16
+//     pages: v_mfma_f32_16x16x4_f32 as in decode.hip, P as it is and V widened; an infinite
+//     value then stays infinite (a part of P that is 0 would make it NaN; 4-bit values are
+//     never infinite), and the lower rate is enough for four times the bytes.
+//   * The running maximum is raised, and O scaled, only in steps where it grows.
+#include <algorithm>
+#include <cmath>
+
 #include "paged.h"
 
 namespace spx {
 
 constexpr int kPaThreads = 256, kPaWaves = kPaThreads / 64;
+constexpr int kPaCols = 16;
+constexpr int kPaMaxGrid = 1024;         // workgroups that share the units (weights in the merge)
+constexpr int kPaCus = 256;
+
+template <int D, bool kFour>
+struct PagedShape {
+  static constexpr int kTiles = kFour ? 4 : 2;                 // 16-key tiles per wave and unit
+  static constexpr int kUnit = 16 * kTiles * kPaWaves;         // keys of a unit
+  static constexpr int kPerCu = D == 128 ? 3 : 2;              // resident workgroups
+};
 
 struct PagedAttnArgs {
   PagedMap map;
@@ -14,95 +55,668 @@ struct PagedAttnArgs {
   const void* value_pages;
   const uint8_t* key_scales;
   const uint8_t* value_scales;
-  int tokens, q_heads, kv_heads, group;
-  float scale_log2;
+  int batch, tokens, q_heads, kv_heads, group;
+  int cols, col_tiles;                   // tokens x group, tiles of 16 of them
+  int grid;                              // workgroups sharing the units; 0: one per stream
+  float scale_log2;                      // >= 0: a negative scale is applied to q's sign
+  uint32_t q_sign;                       // 0 or 0x80008000
   uint16_t* out;
   float* lse;
+  float* part_o;                         // [2 grid][16][D]
+  float* part_ml;                        // [2 grid][16][2]
 };
 
-// dims (D / 64) lane .. of a row, as fp32
-template <int D, bool kFour>
-__device__ __forceinline__ void load_row(const void* pages, const uint8_t* scales, int64_t row,
-                                         int lane, float (&x)[D / 64]) {
-  constexpr int N = D / 64;
-#pragma unroll
-  for (int e = 0; e < N; e += 2) {
-    const int64_t at = row * (D / 2) + (lane * N + e) / 2;       // pairs of dims
-    uint32_t w;
-    if (kFour) {
-      const uint32_t byte = scales[row * (D / kPagedGroup) + lane * N / kPagedGroup];
-      w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(
-                                           (uint32_t) static_cast<const uint8_t*>(pages)[at],
-                                           __uint_as_float(byte << 23), 0));
-    } else {
-      w = static_cast<const uint32_t*>(pages)[at];
-    }
-    x[e] = bf16_lo(w);
-    x[e + 1] = bf16_hi(w);
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int first_lane(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Weight of a partial with maximum m in a merge with maximum top: an empty partial
+// (m = -inf) counts nothing, also where every partial is empty.
+__device__ __forceinline__ float part_weight(float m, float top) {
+  return m == -INFINITY ? 0.0f : exp2_fast(m - top);
+}
+
+// ---------------------------------------------------------------- division of the work
+
+// Live tokens of a sequence: 0 .. live - 1.
+__device__ __forceinline__ int live_tokens(const PagedAttnArgs& a, int b, int& start) {
+  start = a.map.starts[b];
+  int live = a.map.counts ? min(a.map.counts[b], a.tokens) : a.tokens;
+  if (start < 0) live = 0;
+  const int64_t room = a.map.capacity() - start;
+  return room < live ? (int)max(room, (int64_t)0) : max(live, 0);
+}
+
+// Keys that a column tile of a sequence sees at most.
+__device__ __forceinline__ int tile_keys(const PagedAttnArgs& a, int start, int live, int tile) {
+  const int first = tile * kPaCols / a.group;
+  const int last = min((min((tile + 1) * kPaCols, a.cols) - 1) / a.group, live - 1);
+  return last < first ? 0 : start + last + 1;
+}
+
+template <int kUnit>
+__device__ __forceinline__ int64_t head_units(const PagedAttnArgs& a, int b) {
+  int start;
+  const int live = live_tokens(a, b, start);
+  int64_t units = 0;
+  for (int tile = 0; tile < a.col_tiles; ++tile)
+    units += (tile_keys(a, start, live, tile) + kUnit - 1) / kUnit;
+  return units;
+}
+
+struct Run {                             // units begin .. end of the workgroup w
+  int64_t per;
+  int rest;
+  __device__ __forceinline__ Run(int64_t total, int grid)
+      : per(total / grid), rest((int)(total % grid)) {}
+  __device__ __forceinline__ int64_t begin(int w) const { return w * per + min(w, rest); }
+  __device__ __forceinline__ int owner(int64_t u) const {
+    const int64_t wide = rest * (per + 1);
+    return (int)(u < wide ? u / (per + 1) : rest + (u - wide) / per);
   }
+};
+
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const int lo = __builtin_amdgcn_readlane((int)x, lane);
+  const int hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+  return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
+__device__ __forceinline__ int64_t wave_prefix(int64_t x, int lane) {     // inclusive
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// All units, and those of the sequences before b.
+template <int kUnit>
+__device__ __forceinline__ int64_t count_units(const PagedAttnArgs& a, int lane, int b,
+                                               int64_t& before) {
+  int64_t total = 0;
+  before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+    const int64_t units = b0 + lane < a.batch ? head_units<kUnit>(a, b0 + lane) * a.kv_heads : 0;
+    const int64_t sum = wave_prefix(units, lane);
+    if (b >= b0 && b < b0 + kWave) before = total + lane_value(sum - units, b - b0);
+    total += lane_value(sum, kWave - 1);
+  }
+  return total;
+}
+
+struct Stream {
+  int b, kvh, tile, start, live, keys, units;
+  int64_t first;                         // of its units
+
+  template <int kUnit>
+  __device__ __forceinline__ void measure(const PagedAttnArgs& a) {
+    live = live_tokens(a, b, start);
+    start = first_lane(start);
+    live = first_lane(live);
+    keys = tile_keys(a, start, live, tile);
+    units = (keys + kUnit - 1) / kUnit;
+  }
+  // The stream of unit u. false: there is none (lengths that change under the launch must not
+  // make it loop).
+  template <int kUnit>
+  __device__ __forceinline__ bool find(const PagedAttnArgs& a, int lane, int64_t u) {
+    int64_t total = 0;
+    b = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kWave) {
+      const int64_t units = b0 + lane < a.batch ? head_units<kUnit>(a, b0 + lane) * a.kv_heads : 0;
+      const int64_t sum = wave_prefix(units, lane);
+      const uint64_t past = __ballot(total + sum > u);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = b0 + l;
+        total += lane_value(sum - units, l);
+        break;
+      }
+      total += lane_value(sum, kWave - 1);
+    }
+    b = first_lane(b);
+    const int64_t each = max(head_units<kUnit>(a, b), (int64_t)1);
+    kvh = min(first_lane((int)((u - total) / each)), a.kv_heads - 1);
+    first = total + kvh * each;
+    for (tile = 0; tile < a.col_tiles; ++tile) {
+      measure<kUnit>(a);
+      if (u < first + units) return true;
+      first += units;
+    }
+    return false;
+  }
+  // The next one that has units.
+  template <int kUnit>
+  __device__ __forceinline__ bool next(const PagedAttnArgs& a) {
+    first += units;
+    do {
+      if (++tile == a.col_tiles) {
+        tile = 0;
+        if (++kvh == a.kv_heads) {
+          kvh = 0;
+          if (++b == a.batch) return false;
+        }
+      }
+      measure<kUnit>(a);
+    } while (units == 0);
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------------- one stream
+
+// Dims of the lane c in a V row and an O register.
+template <int D, bool kFour>
+__device__ __forceinline__ int value_dim(int c, int i) {
+  return kFour ? D / 16 * c + i : 128 * (i / 8) + 8 * c + i % 8;
 }
 
 template <int D, bool kFour>
-__global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a) {
-  constexpr int N = D / 64;
-  __shared__ float part_m[kPaWaves], part_l[kPaWaves], part_o[kPaWaves][D];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t out_row = blockIdx.x;
-  const int h = (int)(out_row % a.q_heads), i = (int)(out_row / a.q_heads % a.tokens);
-  const int b = (int)(out_row / a.q_heads / a.tokens), kvh = h / a.group;
-  const int last = a.map.position(b, i);
-  const uint16_t* qr = a.q + b * a.qs_b + i * a.qs_t + h * a.qs_h + lane * N;
-  float q[N], o[N], m = -INFINITY, l = 0.0f;
+struct KeyTile {                         // a lane's part of 16 rows of K: row c
+  u32x4 raw[D / (kFour ? 128 : 32)];
+  uint32_t scale[kFour ? D / 128 : 1];
+
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, int64_t row, int c, int g) {
+    if constexpr (kFour) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.key_pages) + row * (D / 2);
+      const uint8_t* s = a.key_scales + row * (D / kPagedGroup);
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    q[e] = __uint_as_float((uint32_t)qr[e] << 16);
-    o[e] = 0.0f;
+      for (int x = 0; x < D / 128; ++x) {
+        raw[x] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * (D / 2) + 64 * x + 16 * g));
+        scale[x] = s[(uint32_t)(c * (D / kPagedGroup) + 4 * x + g)];
+      }
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(a.key_pages) + row * D;
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk)
+        raw[kk] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * D + 32 * kk + 8 * g));
+    }
   }
-  for (int p = w; p <= last; p += kPaWaves) {
-    const int page = a.map.page(b, p);
-    if (page < 0) continue;
-    const int64_t row = a.map.row(page, kvh, p);
-    float k[N], v[N];
-    load_row<D, kFour>(a.key_pages, a.key_scales, row, lane, k);
-    load_row<D, kFour>(a.value_pages, a.value_scales, row, lane, v);
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < N; ++e) s += q[e] * k[e];
-    s = wave_sum(s) * a.scale_log2;
-    const float m_new = max_nan(m, s);
-    const float shift = m_new == -INFINITY ? 0.0f : m_new;
-    const float corr = exp2_fast(m - shift), prob = exp2_fast(s - shift);
-    l = l * corr + prob;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = o[e] * corr + prob * v[e];
-    m = m_new;
+  // Eight dims of the row as A operand of product kk.
+  __device__ __forceinline__ u32x4 operand(int kk) const {
+    if constexpr (!kFour) return raw[kk];
+    else return widen8(raw[kk / 4][kk % 4], __uint_as_float(scale[kk / 4] << 23));
   }
-  if (lane == 0) {
-    part_m[w] = m;
-    part_l[w] = l;
+  // Dim of the operand's first element.
+  static __device__ __forceinline__ int dim(int kk, int g) {
+    return kFour ? 128 * (kk / 4) + 32 * g + 8 * (kk % 4) : 32 * kk + 8 * g;
   }
+};
+
+template <int D, bool kFour>
+struct ValueRow {                        // a lane's dims of one row of V
+  uint32_t raw[kFour ? D / 128 : D / 32];
+  uint32_t scale;
+
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, int64_t row, int at, int c) {
+    if constexpr (kFour) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.value_pages) + row * (D / 2);
+      if constexpr (D == 128) {
+        raw[0] = *reinterpret_cast<const uint32_t*>(p + (uint32_t)(at * 64 + 4 * c));
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(p + (uint32_t)(at * 128 + 8 * c));
+        raw[0] = w[0];
+        raw[1] = w[1];
+      }
+      scale = a.value_scales[row * (D / kPagedGroup) +
+                             (uint32_t)(at * (D / kPagedGroup) + c * (D / 16) / kPagedGroup)];
+    } else {
+      const uint16_t* p = static_cast<const uint16_t*>(a.value_pages) + row * D;
 #pragma unroll
-  for (int e = 0; e < N; ++e) part_o[w][lane * N + e] = o[e];
+      for (int x = 0; x < D / 128; ++x) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(p + (uint32_t)(at * D + 128 * x + 8 * c));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) raw[4 * x + e] = w[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (auto& x : raw) x = 0;
+    scale = 127;
+  }
+  __device__ __forceinline__ bool finite() const {
+    if constexpr (kFour) return scale != 255;
+    bool ok = true;
+#pragma unroll
+    for (uint32_t x : raw)
+      ok = ok && (x & 0x7f80u) != 0x7f80u && (x & 0x7f800000u) != 0x7f800000u;
+    return ok;
+  }
+  // Dims 8 x .. 8 x + 7 of the lane's as four bf16 pairs.
+  __device__ __forceinline__ u32x4 wide(int x) const {
+    if constexpr (kFour) return widen8(raw[x], __uint_as_float(scale << 23));
+    else return u32x4{raw[4 * x], raw[4 * x + 1], raw[4 * x + 2], raw[4 * x + 3]};
+  }
+};
+
+template <int D, bool kFour>
+struct Accumulator {
+  using Shape = PagedShape<D, kFour>;
+  static constexpr int T = Shape::kTiles, KK = D / 32, N = D / 16;
+  f32x4 o[N];                            // [query row 4 g + r][value_dim(c, i)]
+  float m, l;                            // of column c, m unscaled; l over this lane's keys
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (auto& x : o) x = f32x4{};
+    m = -INFINITY;
+    l = 0.0f;
+  }
+
+  // One wave's tiles from key0 on. limit: the last key that column c sees, first_limit: that of
+  // the tile's first column.
+  __device__ __forceinline__ void step(const PagedAttnArgs& a, const Stream& s, const u32x4 (&q)[KK],
+                                       int ids, int id0, int key0, int limit, int first_limit,
+                                       int c, int g) {
+    KeyTile<D, kFour> key[T];
+    ValueRow<D, kFour> value[T][4];
+    bool placed = true;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int id = __builtin_amdgcn_readlane(ids, id0 + t);
+      const int64_t row = a.map.row(max(id, 0), s.kvh, key0 + 16 * t);
+      bad |= (id < 0 ? 1u : 0u) << t;
+      key[t].load(a, row, c, g);
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int64_t row = a.map.row(max(__builtin_amdgcn_readlane(ids, id0 + t), 0), s.kvh,
+                                    key0 + 16 * t);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) value[t][r].load(a, row, 4 * g + r, c);
+    }
+    placed = bad == 0;
+    __builtin_amdgcn_sched_barrier(0);   // every load of the step is issued by now
+    f32x4 x[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      x[t] = f32x4{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) x[t] = mfma16(key[t].operand(kk), q[kk], x[t]);
+    }
+    const bool masked = !placed || key0 + 16 * T - 1 > first_limit;
+    bool split = false;                  // V rows of some columns only, not finite: left out
+    if (masked) {
+      // scores of keys that a column does not see are -inf; rows that no column sees are 0, so
+      // that what lies behind the last token does not meet a probability of 0
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int p = key0 + 16 * t + 4 * g + r;
+          const bool here = !(bad >> t & 1);
+          if (!here || p > limit) x[t][r] = -INFINITY;
+          if (!here || p >= s.keys) {
+            value[t][r].clear();
+          } else if (p > first_limit && !value[t][r].finite()) {
+            split = true;
+            value[t][r].clear();
+          }
+        }
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m)) {
+      const float m_new = fmaxf(m, mx);
+      const float corr = m == -INFINITY ? 0.0f : exp2_fast((m - m_new) * a.scale_log2);
+      l *= corr;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float cr = __shfl(corr, 4 * g + r);
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i][r] *= cr;
+      }
+      m = m_new;
+    }
+    const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float p = exp2_fast(__builtin_fmaf(x[t][r], a.scale_log2, -shift));
+        if (masked && x[t][r] == -INFINITY) p = 0.0f;      // also with a scale of 0
+        x[t][r] = p;
+        l += p;
+      }
+    if constexpr (kFour) {
+#pragma unroll
+      for (int t = 0; t < T; t += 2) {
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[t + e / 2][2 * (e % 2)], w = x[t + e / 2][2 * (e % 2) + 1];
+          hi[e] = pack_bf16x2(u, w);
+          lo[e] = pack_bf16x2(u - bf16_lo(hi[e]), w - bf16_hi(hi[e]));
+        }
+#pragma unroll
+        for (int y = 0; y < N / 8; ++y) {
+          u32x4 row[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) row[j] = value[t + j / 4][j % 4].wide(y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            u32x4 b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              b[e] = __builtin_amdgcn_perm(row[2 * e + 1][i / 2], row[2 * e][i / 2],
+                                           i % 2 ? 0x07060302u : 0x05040100u);
+            o[8 * y + i] = mfma16(hi, b, o[8 * y + i]);
+            o[8 * y + i] = mfma16(lo, b, o[8 * y + i]);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const uint32_t v2 = value[t][r].raw[i / 2];
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_lo(v2), o[i], 0, 0, 0);
+            o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_hi(v2), o[i + 1], 0, 0, 0);
+          }
+    }
+    if (__any(split)) add_split_rows(a, s, x, key0, limit, first_limit, c, g);
+  }
+
+  // The V rows that step() left out, one after the other: only into the columns that see them.
+  __device__ __forceinline__ void add_split_rows(const PagedAttnArgs& a, const Stream& s,
+                                                 const f32x4 (&p)[T], int key0, int limit,
+                                                 int first_limit, int c, int g) {
+    const int last = min(key0 + 16 * T, s.keys);
+#pragma unroll 1
+    for (int at = max(key0, first_limit + 1); at < last; ++at) {
+      const int id = a.map.page(s.b, at);
+      if (id < 0) continue;
+      ValueRow<D, kFour> v;
+      v.load(a, a.map.row(id, s.kvh, at), 0, c);
+      const bool left_out = !v.finite();
+      float mine = 0.0f;                 // the probability of key `at`, where this lane has it
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mine = key0 + 16 * t + 4 * g + r == at ? p[t][r] : mine;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float prob = __shfl(mine, 16 * (at / 4 % 4) + 4 * g + r);
+        const int seen = __shfl(limit, 4 * g + r);
+        const bool sees = left_out && at <= seen;
+#pragma unroll
+        for (int y = 0; y < N / 8; ++y) {
+          const u32x4 w = v.wide(y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[8 * y + 2 * e][r] += sees ? prob * bf16_lo(w[e]) : 0.0f;
+            o[8 * y + 2 * e + 1][r] += sees ? prob * bf16_hi(w[e]) : 0.0f;
+          }
+        }
+      }
+    }
+  }
+};
+
+// grid > 0: workgroup w takes its run of all units; grid == 0: workgroup w is stream w.
+template <int D, bool kFour>
+__global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void paged_attn_kernel(
+    PagedAttnArgs a) {
+  using Shape = PagedShape<D, kFour>;
+  constexpr int T = Shape::kTiles, KK = D / 32, kIdUnits = kWave / T;
+  __shared__ float part_m[kPaWaves][kPaCols], part_l[kPaWaves][kPaCols];
+  __shared__ __align__(16) float part_o[kPaWaves][kPaCols][D];
+  const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+
+  Stream s;
+  int64_t u, end, begin;
+  if (a.grid > 0) {
+    int64_t unused;
+    const Run run(count_units<Shape::kUnit>(a, lane, 0, unused), a.grid);
+    begin = u = run.begin(blockIdx.x);
+    end = run.begin(blockIdx.x + 1);
+    if (u >= end) return;
+    if (!s.find<Shape::kUnit>(a, lane, u)) return;
+  } else {
+    const int stream = blockIdx.x;
+    s.tile = stream % a.col_tiles;
+    s.kvh = stream / a.col_tiles % a.kv_heads;
+    s.b = stream / a.col_tiles / a.kv_heads;
+    s.first = begin = u = 0;
+    s.measure<Shape::kUnit>(a);
+    end = s.units;
+  }
+
+  for (;;) {
+    const int cols = min(kPaCols, a.cols - s.tile * kPaCols);
+    const int n = s.tile * kPaCols + min(c, cols - 1);    // columns past the last repeat it
+    const int token = n / a.group, head = s.kvh * a.group + n % a.group;
+    const int limit = s.start + token;
+    const int first_limit = s.start + s.tile * kPaCols / a.group;
+    u32x4 q[KK];
+    const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      q[kk] = *reinterpret_cast<const u32x4*>(qr + KeyTile<D, kFour>::dim(kk, g));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[kk][e] ^= a.q_sign;
+    }
+    Accumulator<D, kFour> acc;
+    acc.clear();
+    const int j0 = (int)(u - s.first), j1 = (int)(min(end, s.first + s.units) - s.first);
+    for (int jb = j0; jb < j1; jb += kIdUnits) {
+      // page ids of the wave's tiles in units jb .. jb + kIdUnits - 1
+      const int p = (jb + lane / T) * Shape::kUnit + (w * T + lane % T) * 16;
+      const int ids = a.map.page(s.b, min(p, s.keys - 1));
+      const int je = min(j1, jb + kIdUnits);
+      for (int j = jb; j < je; ++j) {
+        const int key0 = j * Shape::kUnit + w * T * 16;
+        if (key0 >= s.keys) break;
+        acc.step(a, s, q, ids, (j - jb) * T, key0, limit, first_limit, c, g);
+      }
+    }
+    float l = acc.l;
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+      part_m[w][c] = acc.m == -INFINITY ? -INFINITY : acc.m * a.scale_log2;
+      part_l[w][c] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < Accumulator<D, kFour>::N; i += 4)
+        *reinterpret_cast<f32x4*>(&part_o[w][4 * g + r][value_dim<D, kFour>(c, i)]) =
+            f32x4{acc.o[i][r], acc.o[i + 1][r], acc.o[i + 2][r], acc.o[i + 3][r]};
+    block_sync();
+    const bool whole = j0 == 0 && j1 == s.units;
+    const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
+    for (int e = threadIdx.x; e < cols * (D / 4); e += kPaThreads) {
+      const int col = e / (D / 4), d = (e % (D / 4)) * 4;
+      float top = part_m[0][col];
+#pragma unroll
+      for (int x = 1; x < kPaWaves; ++x) top = fmaxf(top, part_m[x][col]);
+      float sum = 0.0f;
+      f32x4 v{};
+#pragma unroll
+      for (int x = 0; x < kPaWaves; ++x) {
+        const float wt = part_weight(part_m[x][col], top);
+        const f32x4 po = *reinterpret_cast<const f32x4*>(&part_o[x][col][d]);
+        sum += wt * part_l[x][col];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] += wt * po[y];
+      }
+      const int cn = s.tile * kPaCols + col;
+      if (cn / a.group >= s.live) {      // not live: sees nothing, whatever step() added
+        v = f32x4{};
+        sum = 0.0f;
+        top = -INFINITY;
+      }
+      if (whole) {
+        const int64_t row = ((int64_t)s.b * a.tokens + cn / a.group) * a.q_heads +
+                            s.kvh * a.group + cn % a.group;
+        const float inv = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
+        u32x2 packed;
+        packed[0] = pack_bf16x2(v[0] * inv, v[1] * inv);
+        packed[1] = pack_bf16x2(v[2] * inv, v[3] * inv);
+        *reinterpret_cast<u32x2*>(a.out + row * D + d) = packed;
+        if (d == 0 && a.lse) a.lse[row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)slot * kPaCols + col) * D + d) = v;
+        if (d == 0) {
+          a.part_ml[(slot * kPaCols + col) * 2] = top;
+          a.part_ml[(slot * kPaCols + col) * 2 + 1] = sum;
+        }
+      }
+    }
+    u = s.first + j1;
+    if (u >= end || !s.next<Shape::kUnit>(a)) return;
+    block_sync();                        // the partials are read before they are overwritten
+  }
+}
+
+// Join of the partial results of a row: one workgroup per (row, 64 dims), the partials in turn
+// over 16 groups of threads. Rows of one workgroup are written already; rows of streams
+// without keys are written here.
+constexpr int kPaMergeDims = 64;
+
+template <int D, bool kFour>
+__global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a) {
+  using Shape = PagedShape<D, kFour>;
+  constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaThreads / kLanes;
+  __shared__ float weight[kPaMaxGrid];
+  __shared__ float red[2][kPaWaves];
+  __shared__ __align__(16) float acc_s[kGroups][kPaMergeDims];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int h = (int)(row % a.q_heads), i = (int)(row / a.q_heads % a.tokens);
+  Stream s;
+  s.b = (int)(row / a.q_heads / a.tokens);
+  s.kvh = h / a.group;
+  const int n = i * a.group + h % a.group;
+  int64_t before;
+  const Run run(count_units<Shape::kUnit>(a, lane, s.b, before), a.grid);
+  const int64_t each = head_units<Shape::kUnit>(a, s.b);
+  s.first = before + s.kvh * each;
+  for (s.tile = 0;; ++s.tile) {
+    s.measure<Shape::kUnit>(a);
+    if (s.tile == n / kPaCols) break;
+    s.first += s.units;
+  }
+  const int col = n % kPaCols, d0 = blockIdx.y * kPaMergeDims;
+  const int dim = d0 + tid % kLanes * 4, gr = tid / kLanes;
+  if (s.units == 0) {
+    if (gr == 0) *reinterpret_cast<u32x2*>(a.out + row * D + dim) = u32x2{};
+    if (tid == 0 && d0 == 0 && a.lse) a.lse[row] = -INFINITY;
+    return;
+  }
+  const int w0 = run.owner(s.first), w1 = run.owner(s.first + s.units - 1);
+  if (w0 == w1) return;
+  const int parts = w1 - w0 + 1;
+  // the stream is the first one of every workgroup but perhaps w0
+  const int slot0 = 2 * w0 + (run.begin(w0) == s.first ? 0 : 1);
+  auto slot = [&](int x) { return x == 0 ? slot0 : 2 * (w0 + x); };
+  float top = -INFINITY;
+  for (int x = tid; x < parts; x += kPaThreads)
+    top = fmaxf(top, a.part_ml[(slot(x) * kPaCols + col) * 2]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) red[0][w] = top;
   block_sync();
-  float top = part_m[0], sum = 0.0f;
-#pragma unroll
-  for (int x = 1; x < kPaWaves; ++x) top = max_nan(top, part_m[x]);
-  const float shift = top == -INFINITY ? 0.0f : top;
-  float wt[kPaWaves];
-#pragma unroll
-  for (int x = 0; x < kPaWaves; ++x) {
-    wt[x] = exp2_fast(part_m[x] - shift);
-    sum += wt[x] * part_l[x];
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float sum = 0.0f;
+  for (int x = tid; x < parts; x += kPaThreads) {
+    const float* ml = a.part_ml + (slot(x) * kPaCols + col) * 2;
+    const float wt = part_weight(ml[0], top);
+    weight[x] = wt;
+    sum += wt * ml[1];
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int d = threadIdx.x; d < D; d += kPaThreads) {
-    float acc = 0.0f;
+  sum = wave_sum(sum);
+  if (lane == 0) red[1][w] = sum;
+  block_sync();
+  f32x4 acc{};
+#pragma unroll 4
+  for (int x = gr; x < parts; x += kGroups) {
+    const f32x4 po =
+        *reinterpret_cast<const f32x4*>(a.part_o + ((int64_t)slot(x) * kPaCols + col) * D + dim);
 #pragma unroll
-    for (int x = 0; x < kPaWaves; ++x) acc += wt[x] * part_o[x][d];
-    a.out[out_row * D + d] = to_bf16_bits(acc * inv);
+    for (int y = 0; y < 4; ++y) acc[y] += weight[x] * po[y];
   }
-  if (threadIdx.x == 0 && a.lse)
-    a.lse[out_row] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  *reinterpret_cast<f32x4*>(&acc_s[gr][dim - d0]) = acc;
+  block_sync();
+  sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  if (tid < kPaMergeDims / 2) {
+    const float inv = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
+    float x = 0.0f, y = 0.0f;
+#pragma unroll
+    for (int r = 0; r < kGroups; ++r) {
+      x += acc_s[r][2 * tid];
+      y += acc_s[r][2 * tid + 1];
+    }
+    *reinterpret_cast<uint32_t*>(a.out + row * D + d0 + 2 * tid) = pack_bf16x2(x * inv, y * inv);
+  }
+  if (tid == 0 && d0 == 0 && a.lse) a.lse[row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------- host
+
+// Workgroups that share the units, or 0: one per stream and no second launch, where a stream
+// has at most two units (the second launch costs more than it saves).
+template <int D, bool kFour>
+static int paged_grid(int64_t keys, int64_t streams) {
+  using Shape = PagedShape<D, kFour>;
+  const int64_t units = (keys + Shape::kUnit - 1) / Shape::kUnit;
+  if (units <= 2) return 0;
+  return (int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units);
+}
+
+struct PagedSizes {
+  int64_t keys, streams, rows;
+};
+
+static int paged_sizes(int table_width, int page_size, int max_keys, int batch, int tokens,
+                       int q_heads, int kv_heads, PagedSizes& z) {
+  if (table_width <= 0 || page_size <= 0 || max_keys < 0 || batch <= 0 || tokens <= 0 ||
+      q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0)
+    return SPX_EINVAL;
+  z.keys = (int64_t)table_width * page_size;
+  if (max_keys > 0) z.keys = std::min<int64_t>(z.keys, max_keys);
+  const int64_t cols = (int64_t)tokens * (q_heads / kv_heads);
+  z.streams = (int64_t)batch * kv_heads * ((cols + kPaCols - 1) / kPaCols);
+  z.rows = (int64_t)batch * tokens * q_heads;
+  return z.rows <= 0x7fffffff && z.streams <= 0x7fffffff ? SPX_OK : SPX_EINVAL;
+}
+
+static int paged_grid_of(const PagedSizes& z, int head_dim, bool four) {
+  if (head_dim == 128)
+    return four ? paged_grid<128, true>(z.keys, z.streams) : paged_grid<128, false>(z.keys, z.streams);
+  return four ? paged_grid<256, true>(z.keys, z.streams) : paged_grid<256, false>(z.keys, z.streams);
+}
+
+template <int D, bool kFour>
+static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, hipStream_t st) {
+  if (a.grid > 0) {
+    SPX_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+                SPX_EINVAL, "paged_attention: workspace null or not 16-byte aligned");
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
+  }
+  paged_attn_kernel<D, kFour>
+      <<<(unsigned)(a.grid > 0 ? a.grid : z.streams), kPaThreads, 0, st>>>(a);
+  if (a.grid > 0)
+    paged_merge_kernel<D, kFour>
+        <<<dim3((unsigned)z.rows, D / kPaMergeDims), kPaThreads, 0, st>>>(a);
+  return launch_status("paged_attention");
 }
 
 }  // namespace spx
@@ -110,12 +724,13 @@ __global__ __launch_bounds__(kPaThreads) void paged_attn_kernel(PagedAttnArgs a)
 using namespace spx;
 
 extern "C" int64_t spx_paged_attention_workspace_bytes(int table_width, int page_size, int max_keys,
-                                                       int batch, int tokens, int q_heads,
-                                                       int kv_heads, int head_dim) {
-  if (table_width <= 0 || page_size <= 0 || max_keys < 0 || batch <= 0 || tokens <= 0 ||
-      q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || (head_dim != 128 && head_dim != 256))
+                                                       int four_bit, int batch, int tokens,
+                                                       int q_heads, int kv_heads, int head_dim) {
+  PagedSizes z;
+  if (paged_sizes(table_width, page_size, max_keys, batch, tokens, q_heads, kv_heads, z) != SPX_OK ||
+      (head_dim != 128 && head_dim != 256))
     return -1;
-  return 0;
+  return (int64_t)2 * paged_grid_of(z, head_dim, four_bit != 0) * kPaCols * (head_dim + 2) * 4;
 }
 
 extern "C" int spx_paged_attention(const void* q, const int64_t* q_strides,
@@ -131,31 +746,34 @@ extern "C" int spx_paged_attention(const void* q, const int64_t* q_strides,
                                key_pages, value_pages, key_scales, value_scales, pages, page_size,
                                batch, tokens, kv_heads, head_dim);
   if (status != SPX_OK) return status;
-  SPX_REQUIRE(q_heads > 0 && q_heads % kv_heads == 0 && max_keys >= 0, SPX_EINVAL,
-              "bad shape: q_heads %d kv_heads %d max_keys %d", q_heads, kv_heads, max_keys);
+  PagedSizes z;
+  SPX_REQUIRE(paged_sizes(table_width, page_size, max_keys, batch, tokens, q_heads, kv_heads, z) ==
+                  SPX_OK,
+              SPX_EINVAL, "bad shape: batch %d tokens %d q_heads %d kv_heads %d max_keys %d", batch,
+              tokens, q_heads, kv_heads, max_keys);
   SPX_REQUIRE(q && q_strides && out, SPX_EINVAL, "null pointer");
   SPX_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                   q_strides[3] == 1 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 7) == 0,
               SPX_EINVAL,
               "q, out: bases must be 16-byte aligned, q's dim stride 1, the others multiples of 8");
-  const int64_t rows = (int64_t)batch * tokens * q_heads;
-  SPX_REQUIRE(rows <= 0x7fffffff, SPX_EINVAL, "more than 2^31 - 1 query rows");
   a.q = static_cast<const uint16_t*>(q);
   a.qs_b = q_strides[0]; a.qs_t = q_strides[1]; a.qs_h = q_strides[2];
   a.key_pages = key_pages; a.value_pages = value_pages;
   a.key_scales = static_cast<const uint8_t*>(key_scales);
   a.value_scales = static_cast<const uint8_t*>(value_scales);
-  a.tokens = tokens; a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads;
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.batch = batch; a.tokens = tokens; a.q_heads = q_heads; a.kv_heads = kv_heads;
+  a.group = q_heads / kv_heads;
+  a.cols = tokens * a.group;
+  a.col_tiles = (a.cols + kPaCols - 1) / kPaCols;
+  a.grid = paged_grid_of(z, head_dim, key_scales != nullptr);
+  a.scale_log2 = (float)(std::abs((double)scale) * 1.4426950408889634);
+  a.q_sign = scale < 0 ? 0x80008000u : 0;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (head_dim == 128) {
-    if (key_scales) paged_attn_kernel<128, true><<<(unsigned)rows, kPaThreads, 0, st>>>(a);
-    else paged_attn_kernel<128, false><<<(unsigned)rows, kPaThreads, 0, st>>>(a);
-  } else {
-    if (key_scales) paged_attn_kernel<256, true><<<(unsigned)rows, kPaThreads, 0, st>>>(a);
-    else paged_attn_kernel<256, false><<<(unsigned)rows, kPaThreads, 0, st>>>(a);
-  }
-  return launch_status("paged_attention");
+  if (head_dim == 128)
+    return key_scales ? launch_paged<128, true>(a, z, workspace, st)
+                      : launch_paged<128, false>(a, z, workspace, st);
+  return key_scales ? launch_paged<256, true>(a, z, workspace, st)
+                    : launch_paged<256, false>(a, z, workspace, st);
 }

@@ -262,7 +262,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if return_lse else None
     if batch and tokens:
         shape = (batch, tokens, q_heads, kv_heads, head_dim)
-        nbytes = _lib.load().spx_paged_attention_workspace_bytes(place[2], pages[5], bound, *shape)
+        nbytes = _lib.load().spx_paged_attention_workspace_bytes(
+            place[2], pages[5], bound, cache.four_bit, *shape)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
         _call(device, "spx_paged_attention", q.data_ptr(), _lib.strides(q), *place, *pages, bound,
               *shape, float(scale), _lib.ptr(workspace), out.data_ptr(), _lib.ptr(lse))

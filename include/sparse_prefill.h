@@ -379,7 +379,7 @@ int spx_paged_gather(const int32_t* page_table, int64_t table_stride, int table_
  * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after.
  * Results do not depend on the launch's timing. */
 int64_t spx_paged_attention_workspace_bytes(int table_width, int page_size, int max_keys,
-                                            int batch, int tokens, int q_heads, int kv_heads,
+                                            int four_bit, int batch, int tokens, int q_heads, int kv_heads,
                                             int head_dim);
 int spx_paged_attention(const void* q, const int64_t* q_strides, const int32_t* page_table,
                         int64_t table_stride, int table_width, const int32_t* starts,

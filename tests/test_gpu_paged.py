@@ -304,6 +304,35 @@ def test_attention_special_values(gpu, bits):
     assert torch.equal(out[~bad], want[~bad])
 
 
+@pytest.mark.parametrize("bits", (16, 4))
+@pytest.mark.parametrize("layout", ((12, 2, 128), (6, 1, 256)))
+def test_attention_special_values_of_later_tokens(gpu, layout, bits):
+    """Values that are not finite at tokens that only some of the rows see: the others are as
+    they were, bit for bit, and those that see them are NaN or infinite."""
+    s = ref.make(23, 2, 5, *layout, 16, 20, (200, 61), bits=bits)
+    want, _ = _check_attention(s, 0.1)
+    cache, table, starts, _ = ref.on_gpu(s)
+    for b, p, dim, x in ((0, 202, 40, "nan"), (0, 204, 100, "inf"), (1, 65, 7, "-inf")):
+        page, slot = int(s.table[b, p // 16]), p % 16
+        if bits == 4:
+            cache.value_scales[page, 0, slot, dim // 32] = 255
+        else:
+            cache.value_pages[page, 0, slot, dim] = float(x)
+    out = paged.paged_attention(s.q.cuda(), cache, table, starts, 0.1).double().cpu()
+    off = torch.zeros_like(out, dtype=torch.bool)
+    heads = layout[0] // layout[1]
+    for b, first, dim in ((0, 2, 40), (0, 4, 100), (1, 4, 7)):
+        dims = slice(dim // 32 * 32, dim // 32 * 32 + 32) if bits == 4 else slice(dim, dim + 1)
+        off[b, first:, :heads, dims] = True
+    assert torch.equal(~torch.isfinite(out), off)
+    # rounding of the rows that see them goes another way in their finite dims
+    torch.testing.assert_close(out[~off], want[~off], rtol=2.0 ** -7, atol=1e-4)
+    assert torch.equal(out[0, :2], want[0, :2]) and torch.equal(out[1, :4], want[1, :4])
+    if bits == 16:
+        assert (out[0, 4, :heads, 100] == float("inf")).all()
+        assert (out[1, 4, :heads, 7] == -float("inf")).all()
+
+
 def test_attention_one_sided_scores(gpu):
     """Scores far from 0 on either side: the maximum is subtracted."""
     s = ref.make(19, 1, 1, 4, 2, 128, 64, 12, (700,))

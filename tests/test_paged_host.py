@@ -67,9 +67,9 @@ def test_gather_and_attention_arguments():
     assert _attention(shape=(2, 1, 27, 4, 128)) == _attention(shape=(1 << 16, 1 << 10, 32, 4, 128)) \
         == invalid
     size = _lib.load().spx_paged_attention_workspace_bytes
-    assert size(32, 128, 0, 2, 1, 28, 4, 128) >= 0
-    for bad in ((32, 128, 0, 2, 1, 27, 4, 128), (32, 128, 0, 0, 1, 28, 4, 128),
-                (32, 128, 0, 2, 1, 28, 4, 64), (32, 128, -1, 2, 1, 28, 4, 128)):
+    assert size(32, 128, 0, 0, 2, 1, 28, 4, 128) >= 0
+    for bad in ((32, 128, 0, 0, 2, 1, 27, 4, 128), (32, 128, 0, 1, 0, 1, 28, 4, 128),
+                (32, 128, 0, 0, 2, 1, 28, 4, 64), (32, 128, -1, 1, 2, 1, 28, 4, 128)):
         assert size(*bad) == -1
 
 
