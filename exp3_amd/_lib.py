@@ -28,7 +28,6 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S = ctypes.POINTER(ctypes.c_int64)
-_L = ctypes.c_int64
 
 # name -> argument types (restype is int for all compute entry points)
 _PROTOTYPES = {
@@ -61,17 +60,16 @@ _PROTOTYPES = {
     "spx_sparse_attention_rescue": [_P, _S, _P, _P, _P, _S, _P, _S, _P, _P, _S, _P, _P, _I, _I,
                                     _I, _I, _I, _I, _I, _F, _P, _S, _P, _S, _P, _P],
     "spx_decode_attention": [_P, _S, _P, _S, _P, _S, _I, _I, _I, _I, _I, _F, _P, _P, _P],
-    "spx_paged_append": [_P, _S, _P, _S, _P, _S, _P, _P, _I, _I, _I, _P, _L, _I, _P, _P, _P, _P,
-                         _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P],
-    "spx_paged_gather": [_P, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P],
-    "spx_paged_attention": [_P, _S, _P, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I,
-                            _I, _I, _F, _P, _P, _P, _P],
+    # the first argument and the strides as packed bytes
+    "spx_paged_append": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P],
+    "spx_paged_gather": [_P, _P, _P, _P],
+    "spx_paged_attention": [_P, _P, _P, _I, _I, _F, _P, _P, _P, _P],
 }
 
 # helpers without a status: sizes (int64)
 _SIZE_FUNCTIONS = {"spx_selector_workspace_bytes": [_I, _I, _I, _I],
                    "spx_decode_workspace_bytes": [_I, _I, _I, _I, _I],
-                   "spx_paged_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I, _I],
+                   "spx_paged_attention_workspace_bytes": [_P, _I, _I],
                    "spx_attention_queue_ints": [_I, _I, _I, _I, _I]}
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES) + tuple(_SIZE_FUNCTIONS) + ("spx_last_error",
@@ -147,6 +145,11 @@ def stream(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = torch.cuda.current_device() if device.index is None else device.index
     return _raw_stream(index)
+
+
+def stream_of(index: int) -> int:
+    """The current stream of the device with this index."""
+    return stream(torch.device("cuda", index)) if _raw_stream is None else _raw_stream(index)
 
 
 def work_queue(batch, sequence, q_heads, kv_heads, head_dim, device):

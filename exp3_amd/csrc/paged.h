@@ -50,10 +50,7 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w, float scale) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
 }
 
-// Checks of the arguments that all entry points share; fills the map.
-int paged_map(PagedMap& m, const int32_t* page_table, int64_t table_stride, int table_width,
-              const int32_t* starts, const int32_t* counts, const void* key_pages,
-              const void* value_pages, const void* key_scales, const void* value_scales, int pages,
-              int page_size, int batch, int tokens, int kv_heads, int head_dim);
+// Checks of a cache description; fills the map.
+int paged_map(PagedMap& m, const spx_paged_cache* cache);
 
 }  // namespace spx

@@ -19,37 +19,40 @@ namespace spx {
 
 constexpr int kPagedThreads = 256;
 
-int paged_map(PagedMap& m, const int32_t* page_table, int64_t table_stride, int table_width,
-              const int32_t* starts, const int32_t* counts, const void* key_pages,
-              const void* value_pages, const void* key_scales, const void* value_scales, int pages,
-              int page_size, int batch, int tokens, int kv_heads, int head_dim) {
-  SPX_REQUIRE(head_dim == 128 || head_dim == 256, SPX_EUNSUPPORTED,
-              "head_dim %d unsupported (128 or 256)", head_dim);
-  SPX_REQUIRE(page_size >= kPagedMinPage && page_size <= kPagedMaxPage &&
-                  (page_size & (page_size - 1)) == 0,
+int paged_map(PagedMap& m, const spx_paged_cache* cache) {
+  SPX_REQUIRE(cache != nullptr, SPX_EINVAL, "null cache");
+  const spx_paged_cache& z = *cache;
+  SPX_REQUIRE(z.head_dim == 128 || z.head_dim == 256, SPX_EUNSUPPORTED,
+              "head_dim %d unsupported (128 or 256)", z.head_dim);
+  SPX_REQUIRE(z.page_size >= kPagedMinPage && z.page_size <= kPagedMaxPage &&
+                  (z.page_size & (z.page_size - 1)) == 0,
               SPX_EUNSUPPORTED, "page_size %d unsupported (a power of two from %d to %d)",
-              page_size, kPagedMinPage, kPagedMaxPage);
-  SPX_REQUIRE(batch > 0 && tokens > 0 && kv_heads > 0 && pages > 0 && table_width > 0, SPX_EINVAL,
-              "bad shape: batch %d tokens %d kv_heads %d pages %d table width %d", batch, tokens,
-              kv_heads, pages, table_width);
-  SPX_REQUIRE((int64_t)table_width * page_size <= (1 << 30), SPX_EINVAL,
-              "a table of %d pages of %d tokens exceeds 2^30 positions", table_width, page_size);
-  SPX_REQUIRE(page_table && starts && key_pages && value_pages, SPX_EINVAL, "null pointer");
-  SPX_REQUIRE((key_scales == nullptr) == (value_scales == nullptr), SPX_EINVAL,
+              z.page_size, kPagedMinPage, kPagedMaxPage);
+  SPX_REQUIRE(z.batch > 0 && z.tokens > 0 && z.kv_heads > 0 && z.pages > 0 && z.table_width > 0,
+              SPX_EINVAL, "bad shape: batch %d tokens %d kv_heads %d pages %d table width %d",
+              z.batch, z.tokens, z.kv_heads, z.pages, z.table_width);
+  SPX_REQUIRE((int64_t)z.table_width * z.page_size <= (1 << 30), SPX_EINVAL,
+              "a table of %d pages of %d tokens exceeds 2^30 positions", z.table_width,
+              z.page_size);
+  SPX_REQUIRE(z.page_table && z.starts && z.key_pages && z.value_pages, SPX_EINVAL, "null pointer");
+  SPX_REQUIRE((z.key_scales == nullptr) == (z.value_scales == nullptr), SPX_EINVAL,
               "key_scales and value_scales go together");
-  SPX_REQUIRE(((reinterpret_cast<uintptr_t>(key_pages) | reinterpret_cast<uintptr_t>(value_pages)) &
-               15) == 0 &&
-                  ((reinterpret_cast<uintptr_t>(key_scales) |
-                    reinterpret_cast<uintptr_t>(value_scales)) & 7) == 0,
-              SPX_EINVAL, "pages must be 16-byte, scales 8-byte aligned");
-  m.table = page_table;
-  m.table_stride = table_stride;
-  m.starts = starts;
-  m.counts = counts;
-  m.width = table_width;
-  m.pages = pages;
-  m.page_shift = __builtin_ctz(page_size);
-  m.kv_heads = kv_heads;
+  auto misaligned = [](const void* x, const void* y, uintptr_t to) {
+    return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & (to - 1)) != 0;
+  };
+  SPX_REQUIRE(!misaligned(z.key_pages, z.value_pages, 16) &&
+                  !misaligned(z.key_scales, z.value_scales, 8) &&
+                  !misaligned(z.page_table, z.starts, 4) && !misaligned(z.counts, nullptr, 4),
+              SPX_EINVAL,
+              "pages must be 16-byte, scales 8-byte, page_table, starts and counts 4-byte aligned");
+  m.table = z.page_table;
+  m.table_stride = z.table_stride;
+  m.starts = z.starts;
+  m.counts = z.counts;
+  m.width = z.table_width;
+  m.pages = z.pages;
+  m.page_shift = __builtin_ctz(z.page_size);
+  m.kv_heads = z.kv_heads;
   return SPX_OK;
 }
 
@@ -280,19 +283,14 @@ static unsigned row_blocks(int64_t rows) {
 
 using namespace spx;
 
-extern "C" int spx_paged_append(const void* q, const int64_t* q_strides, const void* k,
-                                const int64_t* k_strides, const void* v, const int64_t* v_strides,
+extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
+                                const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, int q_heads,
                                 const float* rope_cos, const float* rope_sin, int rope_positions,
-                                int rotary_dim, int interleaved, const int32_t* page_table,
-                                int64_t table_stride, int table_width, const int32_t* starts,
-                                const int32_t* counts, void* key_pages, void* value_pages,
-                                void* key_scales, void* value_scales, int pages, int page_size,
-                                int batch, int tokens, int q_heads, int kv_heads, int head_dim,
-                                void* q_out, void* k_out, void* stream) {
+                                int rotary_dim, int interleaved, void* q_out, void* k_out,
+                                void* stream) {
   AppendArgs a{};
-  int status = paged_map(a.map, page_table, table_stride, table_width, starts, counts, key_pages,
-                         value_pages, key_scales, value_scales, pages, page_size, batch, tokens,
-                         kv_heads, head_dim);
+  int status = paged_map(a.map, cache);
   if (status != SPX_OK) return status;
   SPX_REQUIRE(q == nullptr || (q_heads > 0 && q_out), SPX_EINVAL, "q needs q_heads and q_out");
   if (q != nullptr && (status = row_source(a.q, q, q_strides, "q")) != SPX_OK) return status;
@@ -301,12 +299,12 @@ extern "C" int spx_paged_append(const void* q, const int64_t* q_strides, const v
   SPX_REQUIRE((rope_cos == nullptr) == (rope_sin == nullptr), SPX_EINVAL,
               "rope_cos and rope_sin go together");
   if (rope_cos != nullptr) {
-    SPX_REQUIRE(rotary_dim > 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0, SPX_EUNSUPPORTED,
-                "rotary_dim %d unsupported (a multiple of 16 up to head_dim %d)", rotary_dim,
-                head_dim);
-    SPX_REQUIRE(rope_positions >= (int64_t)table_width * page_size, SPX_EINVAL,
+    SPX_REQUIRE(rotary_dim > 0 && rotary_dim <= cache->head_dim && rotary_dim % 16 == 0,
+                SPX_EUNSUPPORTED, "rotary_dim %d unsupported (a multiple of 16 up to head_dim %d)",
+                rotary_dim, cache->head_dim);
+    SPX_REQUIRE(rope_positions >= (int64_t)cache->table_width * cache->page_size, SPX_EINVAL,
                 "the rope table has %d positions, the page table reaches %lld", rope_positions,
-                (long long)table_width * page_size);
+                (long long)cache->table_width * cache->page_size);
     SPX_REQUIRE(((reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin)) &
                  15) == 0, SPX_EINVAL, "rope tables must be 16-byte aligned");
   }
@@ -315,59 +313,61 @@ extern "C" int spx_paged_append(const void* q, const int64_t* q_strides, const v
   a.cos = rope_cos; a.sin = rope_sin;
   a.rotary = rope_cos ? rotary_dim : 0;
   a.interleaved = interleaved;
-  a.tokens = tokens;
-  a.kv_heads = kv_heads;
-  a.rows = (q ? q_heads : 0) + 2 * kv_heads;
-  a.total = (int64_t)batch * tokens * a.rows;
-  SPX_REQUIRE(a.total <= (int64_t)1 << 33, SPX_EINVAL, "more than 2^33 rows in a call");
-  a.key_pages = key_pages; a.value_pages = value_pages;
-  a.key_scales = static_cast<uint8_t*>(key_scales);
-  a.value_scales = static_cast<uint8_t*>(value_scales);
+  a.tokens = cache->tokens;
+  a.kv_heads = cache->kv_heads;
+  const int64_t rows = (q ? q_heads : 0) + 2 * (int64_t)a.kv_heads;
+  SPX_REQUIRE(rows <= 0x7fffffff && (double)cache->batch * cache->tokens * rows <= 0x1p33,
+              SPX_EINVAL, "more than 2^33 rows in a call");
+  a.rows = (int)rows;
+  a.total = (int64_t)cache->batch * cache->tokens * rows;
+  a.key_pages = cache->key_pages; a.value_pages = cache->value_pages;
+  a.key_scales = static_cast<uint8_t*>(cache->key_scales);
+  a.value_scales = static_cast<uint8_t*>(cache->value_scales);
   a.q_out = static_cast<uint16_t*>(q_out);
   a.k_out = static_cast<uint16_t*>(k_out);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned blocks = head_dim == 128 ? row_blocks<128>(a.total) : row_blocks<256>(a.total);
-  if (head_dim == 128) {
-    if (key_scales) paged_append_kernel<128, true><<<blocks, kPagedThreads, 0, st>>>(a);
+  const bool four = cache->key_scales != nullptr;
+  if (cache->head_dim == 128) {
+    const unsigned blocks = row_blocks<128>(a.total);
+    if (four) paged_append_kernel<128, true><<<blocks, kPagedThreads, 0, st>>>(a);
     else paged_append_kernel<128, false><<<blocks, kPagedThreads, 0, st>>>(a);
   } else {
-    if (key_scales) paged_append_kernel<256, true><<<blocks, kPagedThreads, 0, st>>>(a);
+    const unsigned blocks = row_blocks<256>(a.total);
+    if (four) paged_append_kernel<256, true><<<blocks, kPagedThreads, 0, st>>>(a);
     else paged_append_kernel<256, false><<<blocks, kPagedThreads, 0, st>>>(a);
   }
   return launch_status("paged_append");
 }
 
-extern "C" int spx_paged_gather(const int32_t* page_table, int64_t table_stride, int table_width,
-                                const int32_t* starts, const int32_t* counts, const void* key_pages,
-                                const void* value_pages, const void* key_scales,
-                                const void* value_scales, int pages, int page_size, int batch,
-                                int tokens, int kv_heads, int head_dim, void* k_out, void* v_out,
+extern "C" int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out,
                                 void* stream) {
   GatherArgs a{};
-  const int status = paged_map(a.map, page_table, table_stride, table_width, starts, counts,
-                               key_pages, value_pages, key_scales, value_scales, pages, page_size,
-                               batch, tokens, kv_heads, head_dim);
+  const int status = paged_map(a.map, cache);
   if (status != SPX_OK) return status;
   SPX_REQUIRE(k_out && v_out &&
                   ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) ==
                       0,
               SPX_EINVAL, "outputs null or not 16-byte aligned");
-  a.key_pages = key_pages; a.value_pages = value_pages;
-  a.key_scales = static_cast<const uint8_t*>(key_scales);
-  a.value_scales = static_cast<const uint8_t*>(value_scales);
-  a.tokens = tokens;
-  a.kv_heads = kv_heads;
-  a.total = (int64_t)batch * tokens * 2 * kv_heads;
-  SPX_REQUIRE(a.total <= (int64_t)1 << 33, SPX_EINVAL, "more than 2^33 rows in a call");
+  a.key_pages = cache->key_pages; a.value_pages = cache->value_pages;
+  a.key_scales = static_cast<const uint8_t*>(cache->key_scales);
+  a.value_scales = static_cast<const uint8_t*>(cache->value_scales);
+  a.tokens = cache->tokens;
+  a.kv_heads = cache->kv_heads;
+  SPX_REQUIRE(2.0 * cache->batch * cache->tokens * cache->kv_heads <= 0x1p33 &&
+                  cache->kv_heads <= 1 << 29,
+              SPX_EINVAL, "more than 2^33 rows in a call");
+  a.total = (int64_t)cache->batch * cache->tokens * 2 * cache->kv_heads;
   a.k_out = static_cast<uint16_t*>(k_out);
   a.v_out = static_cast<uint16_t*>(v_out);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned blocks = head_dim == 128 ? row_blocks<128>(a.total) : row_blocks<256>(a.total);
-  if (head_dim == 128) {
-    if (key_scales) paged_gather_kernel<128, true><<<blocks, kPagedThreads, 0, st>>>(a);
+  const bool four = cache->key_scales != nullptr;
+  if (cache->head_dim == 128) {
+    const unsigned blocks = row_blocks<128>(a.total);
+    if (four) paged_gather_kernel<128, true><<<blocks, kPagedThreads, 0, st>>>(a);
     else paged_gather_kernel<128, false><<<blocks, kPagedThreads, 0, st>>>(a);
   } else {
-    if (key_scales) paged_gather_kernel<256, true><<<blocks, kPagedThreads, 0, st>>>(a);
+    const unsigned blocks = row_blocks<256>(a.total);
+    if (four) paged_gather_kernel<256, true><<<blocks, kPagedThreads, 0, st>>>(a);
     else paged_gather_kernel<256, false><<<blocks, kPagedThreads, 0, st>>>(a);
   }
   return launch_status("paged_gather");

@@ -684,17 +684,17 @@ struct PagedSizes {
   int64_t keys, streams, rows;
 };
 
-static int paged_sizes(int table_width, int page_size, int max_keys, int batch, int tokens,
-                       int q_heads, int kv_heads, PagedSizes& z) {
-  if (table_width <= 0 || page_size <= 0 || max_keys < 0 || batch <= 0 || tokens <= 0 ||
-      q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0)
-    return SPX_EINVAL;
-  z.keys = (int64_t)table_width * page_size;
-  if (max_keys > 0) z.keys = std::min<int64_t>(z.keys, max_keys);
-  const int64_t cols = (int64_t)tokens * (q_heads / kv_heads);
-  z.streams = (int64_t)batch * kv_heads * ((cols + kPaCols - 1) / kPaCols);
-  z.rows = (int64_t)batch * tokens * q_heads;
-  return z.rows <= 0x7fffffff && z.streams <= 0x7fffffff ? SPX_OK : SPX_EINVAL;
+static bool paged_sizes(const spx_paged_cache& z, int q_heads, int max_keys, PagedSizes& s) {
+  if (z.table_width <= 0 || z.page_size <= 0 || max_keys < 0 || z.batch <= 0 || z.tokens <= 0 ||
+      q_heads <= 0 || z.kv_heads <= 0 || q_heads % z.kv_heads != 0)
+    return false;
+  if ((double)z.batch * z.tokens * q_heads > 0x7fffffff) return false;
+  s.rows = (int64_t)z.batch * z.tokens * q_heads;
+  s.keys = (int64_t)z.table_width * z.page_size;
+  if (max_keys > 0) s.keys = std::min<int64_t>(s.keys, max_keys);
+  const int64_t cols = (int64_t)z.tokens * (q_heads / z.kv_heads);
+  s.streams = (int64_t)z.batch * z.kv_heads * ((cols + kPaCols - 1) / kPaCols);
+  return true;
 }
 
 static int paged_grid_of(const PagedSizes& z, int head_dim, bool four) {
@@ -723,57 +723,50 @@ static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, h
 
 using namespace spx;
 
-extern "C" int64_t spx_paged_attention_workspace_bytes(int table_width, int page_size, int max_keys,
-                                                       int four_bit, int batch, int tokens,
-                                                       int q_heads, int kv_heads, int head_dim) {
+extern "C" int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* cache, int q_heads,
+                                                       int max_keys) {
   PagedSizes z;
-  if (paged_sizes(table_width, page_size, max_keys, batch, tokens, q_heads, kv_heads, z) != SPX_OK ||
-      (head_dim != 128 && head_dim != 256))
+  if (cache == nullptr || !paged_sizes(*cache, q_heads, max_keys, z) ||
+      (cache->head_dim != 128 && cache->head_dim != 256))
     return -1;
-  return (int64_t)2 * paged_grid_of(z, head_dim, four_bit != 0) * kPaCols * (head_dim + 2) * 4;
+  return (int64_t)2 * paged_grid_of(z, cache->head_dim, cache->key_scales != nullptr) * kPaCols *
+         (cache->head_dim + 2) * 4;
 }
 
-extern "C" int spx_paged_attention(const void* q, const int64_t* q_strides,
-                                   const int32_t* page_table, int64_t table_stride, int table_width,
-                                   const int32_t* starts, const int32_t* counts,
-                                   const void* key_pages, const void* value_pages,
-                                   const void* key_scales, const void* value_scales, int pages,
-                                   int page_size, int max_keys, int batch, int tokens, int q_heads,
-                                   int kv_heads, int head_dim, float scale, void* workspace,
-                                   void* out, float* lse, void* stream) {
+extern "C" int spx_paged_attention(const spx_paged_cache* cache, const void* q,
+                                   const int64_t* q_strides, int q_heads, int max_keys, float scale,
+                                   void* workspace, void* out, float* lse, void* stream) {
   PagedAttnArgs a{};
-  const int status = paged_map(a.map, page_table, table_stride, table_width, starts, counts,
-                               key_pages, value_pages, key_scales, value_scales, pages, page_size,
-                               batch, tokens, kv_heads, head_dim);
+  const int status = paged_map(a.map, cache);
   if (status != SPX_OK) return status;
   PagedSizes z;
-  SPX_REQUIRE(paged_sizes(table_width, page_size, max_keys, batch, tokens, q_heads, kv_heads, z) ==
-                  SPX_OK,
-              SPX_EINVAL, "bad shape: batch %d tokens %d q_heads %d kv_heads %d max_keys %d", batch,
-              tokens, q_heads, kv_heads, max_keys);
+  SPX_REQUIRE(paged_sizes(*cache, q_heads, max_keys, z), SPX_EINVAL,
+              "bad shape: batch %d tokens %d q_heads %d kv_heads %d max_keys %d", cache->batch,
+              cache->tokens, q_heads, cache->kv_heads, max_keys);
   SPX_REQUIRE(q && q_strides && out, SPX_EINVAL, "null pointer");
   SPX_REQUIRE(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0 &&
                   q_strides[3] == 1 && ((q_strides[0] | q_strides[1] | q_strides[2]) & 7) == 0,
               SPX_EINVAL,
               "q, out: bases must be 16-byte aligned, q's dim stride 1, the others multiples of 8");
+  const bool four = cache->key_scales != nullptr;
   a.q = static_cast<const uint16_t*>(q);
   a.qs_b = q_strides[0]; a.qs_t = q_strides[1]; a.qs_h = q_strides[2];
-  a.key_pages = key_pages; a.value_pages = value_pages;
-  a.key_scales = static_cast<const uint8_t*>(key_scales);
-  a.value_scales = static_cast<const uint8_t*>(value_scales);
-  a.batch = batch; a.tokens = tokens; a.q_heads = q_heads; a.kv_heads = kv_heads;
-  a.group = q_heads / kv_heads;
-  a.cols = tokens * a.group;
+  a.key_pages = cache->key_pages; a.value_pages = cache->value_pages;
+  a.key_scales = static_cast<const uint8_t*>(cache->key_scales);
+  a.value_scales = static_cast<const uint8_t*>(cache->value_scales);
+  a.batch = cache->batch; a.tokens = cache->tokens;
+  a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.group = q_heads / cache->kv_heads;
+  a.cols = cache->tokens * a.group;
   a.col_tiles = (a.cols + kPaCols - 1) / kPaCols;
-  a.grid = paged_grid_of(z, head_dim, key_scales != nullptr);
+  a.grid = paged_grid_of(z, cache->head_dim, four);
   a.scale_log2 = (float)(std::abs((double)scale) * 1.4426950408889634);
   a.q_sign = scale < 0 ? 0x80008000u : 0;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (head_dim == 128)
-    return key_scales ? launch_paged<128, true>(a, z, workspace, st)
-                      : launch_paged<128, false>(a, z, workspace, st);
-  return key_scales ? launch_paged<256, true>(a, z, workspace, st)
-                    : launch_paged<256, false>(a, z, workspace, st);
+  if (cache->head_dim == 128)
+    return four ? launch_paged<128, true>(a, z, workspace, st)
+                : launch_paged<128, false>(a, z, workspace, st);
+  return four ? launch_paged<256, true>(a, z, workspace, st)
+              : launch_paged<256, false>(a, z, workspace, st);
 }

@@ -27,6 +27,8 @@ pass.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
+import struct
 
 import torch
 
@@ -92,58 +94,70 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 1.0e6, device=Non
     return angle.cos().float(), angle.sin().float()
 
 
-def _check_cache(cache: PagedCache, device: torch.device) -> tuple:
-    """The cache's part of a call's arguments, checked: (four pointers, pages, page_size),
-    kv_heads, head_dim."""
+# spx_paged_cache of the C header, and the strides of a [B, T, H, D] tensor
+_DESCRIPTION = struct.Struct("7Pq8i")
+_STRIDES = struct.Struct("4q")
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _check_cache(cache: PagedCache, device: int) -> tuple:
+    """(four pointers), pages, page_size, kv_heads, head_dim of a cache on this device index."""
     key, value, key_scales, value_scales = (cache.key_pages, cache.value_pages, cache.key_scales,
                                             cache.value_scales)
-    four = key_scales is not None
-    if four != (value_scales is not None):
-        raise ValueError("a 4-bit cache needs key_scales and value_scales, a bf16 cache neither")
     shape = key.shape
-    dtype = torch.uint8 if four else torch.bfloat16
-    if len(shape) != 4 or value.shape != shape or key.dtype != dtype or value.dtype != dtype \
-            or not key.is_contiguous() or not value.is_contiguous():
-        raise ValueError(f"pages must be contiguous {dtype} [pages, Hkv, page_size, D"
-                         f"{' // 2' if four else ''}] tensors of one shape, got {tuple(shape)} "
-                         f"{key.dtype} and {tuple(value.shape)} {value.dtype}")
+    dtype = torch.bfloat16 if key_scales is None else torch.uint8
+    if not (len(shape) == 4 and value.shape == shape and key.dtype is dtype and value.dtype is dtype
+            and key.is_contiguous() and value.is_contiguous()):
+        raise ValueError(f"pages must be contiguous {dtype} [pages, Hkv, page_size, "
+                         f"{'D' if key_scales is None else 'D // 2'}] tensors of one shape, got "
+                         f"{tuple(shape)} {key.dtype} and {tuple(value.shape)} {value.dtype}")
+    if not key.get_device() == value.get_device() == device:
+        raise ValueError(f"pages on {key.device} and {value.device}, the call's tensors on device "
+                         f"{device}")
     pages, kv_heads, page_size, width = shape
-    head_dim = 2 * width if four else width
-    if four:
-        groups = (pages, kv_heads, page_size, head_dim // SCALE_GROUP)
-        for s in (key_scales, value_scales):
-            if s.shape != groups or s.dtype != torch.uint8 or not s.is_contiguous():
-                raise ValueError(f"scales must be contiguous uint8 {groups}, got "
-                                 f"{tuple(s.shape)} {s.dtype}")
-            if s.device != device:
-                raise ValueError(f"tensors on different devices: {device} and {s.device}")
-    for x in (key, value):
-        if x.device != device:
-            raise ValueError(f"tensors on different devices: {device} and {x.device}")
-    return (key.data_ptr(), value.data_ptr(), _lib.ptr(key_scales), _lib.ptr(value_scales), pages,
-            page_size), kv_heads, head_dim
+    if key_scales is None:
+        if value_scales is not None:
+            raise ValueError("a 4-bit cache needs key_scales and value_scales, a bf16 cache neither")
+        return (key.data_ptr(), value.data_ptr(), 0, 0), pages, page_size, kv_heads, width
+    if value_scales is None:
+        raise ValueError("a 4-bit cache needs key_scales and value_scales, a bf16 cache neither")
+    groups = (pages, kv_heads, page_size, 2 * width // SCALE_GROUP)
+    for x in (key_scales, value_scales):
+        if not (x.shape == groups and x.dtype is torch.uint8 and x.is_contiguous()
+                and x.get_device() == device):
+            raise ValueError(f"scales must be contiguous uint8 {groups} on the pages' device, got "
+                             f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    return (key.data_ptr(), value.data_ptr(), key_scales.data_ptr(), value_scales.data_ptr()), \
+        pages, page_size, kv_heads, 2 * width
 
 
-def _check_map(page_table, starts, counts, batch: int, device: torch.device) -> tuple:
-    """(table, its stride, its width, starts, counts) as the entry points take them."""
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != batch:
-        raise ValueError(f"page_table must be int32 [{batch}, pages per sequence], got "
-                         f"{tuple(page_table.shape)} {page_table.dtype}")
-    for name, x in (("starts", starts), ("counts", counts)):
-        if x is None:
-            continue
-        if x.dtype != torch.int32 or x.shape != (batch,):
-            raise ValueError(f"{name} must be int32 [{batch}], got {tuple(x.shape)} {x.dtype}")
-        if x.device != device:
-            raise ValueError(f"tensors on different devices: {device} and {x.device}")
-        if x.stride(0) != 1 and batch > 1:
-            raise ValueError(f"{name} must be contiguous")
-    if page_table.device != device:
-        raise ValueError(f"tensors on different devices: {device} and {page_table.device}")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+def _lengths(name: str, x: torch.Tensor, batch: int, device: int) -> int:
+    if not (x.dtype is torch.int32 and x.shape == (batch,) and x.get_device() == device
+            and x.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 [{batch}] tensor on the pages' device, "
+                         f"got {tuple(x.shape)} {x.dtype} on {x.device}")
+    return x.data_ptr()
+
+
+def _describe(cache: PagedCache, page_table, starts, counts, batch: int, tokens: int,
+              device: int) -> tuple[bytes, int, int, tuple]:
+    """The C description of a call's cache and tokens, checked, its kv_heads and head_dim, and
+    what the size of a workspace depends on."""
+    pointers, pages, page_size, kv_heads, head_dim = _check_cache(cache, device)
+    shape = page_table.shape
+    if not (page_table.dtype is torch.int32 and len(shape) == 2 and shape[0] == batch
+            and page_table.get_device() == device):
+        raise ValueError(f"page_table must be an int32 [{batch}, pages per sequence] tensor on the "
+                         f"pages' device, got {tuple(shape)} {page_table.dtype} on "
+                         f"{page_table.device}")
+    row, unit = page_table.stride()
+    if unit != 1 and shape[1] > 1:
         raise ValueError("page_table must have unit stride within a row")
-    return (page_table.data_ptr(), page_table.stride(0), page_table.shape[1], starts.data_ptr(),
-            _lib.ptr(counts))
+    sizes = (shape[1], pages, page_size, kv_heads, head_dim, batch, tokens, 0)
+    return _DESCRIPTION.pack(*pointers, page_table.data_ptr(),
+                             _lengths("starts", starts, batch, device),
+                             0 if counts is None else _lengths("counts", counts, batch, device),
+                             row, *sizes), kv_heads, head_dim, sizes
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -151,16 +165,26 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return _lib.kernel_view(x.resolve_neg() if x.is_neg() else x)
 
 
-def _call(device: torch.device, name: str, *args) -> None:
+def _new_rows(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _call(device: int, name: str, *args) -> None:
     """Enqueue on the tensors' device (the launch needs it to be the current one)."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _lib.stream(device))
+    if device == _current_device():
+        _lib.call(name, *args, _lib.stream_of(device))
         return
     with torch.cuda.device(device):
-        _lib.call(name, *args, _lib.stream(device))
+        _lib.call(name, *args, _lib.stream_of(device))
 
 
-@torch.no_grad()
+@lru_cache(maxsize=256)
+def _workspace_bytes(four_bit: bool, sizes: tuple, q_heads: int, max_keys: int) -> int:
+    mark = 16 if four_bit else 0
+    return _lib.load().spx_paged_attention_workspace_bytes(
+        _DESCRIPTION.pack(16, 16, mark, mark, 16, 16, 0, 0, *sizes), q_heads, max_keys)
+
+
 def append_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Tensor,
                   k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                   rope: tuple[torch.Tensor, torch.Tensor] | None = None,
@@ -180,63 +204,60 @@ def append_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Ten
 
     Two tokens of a call must not have the same place: pages that are appended to belong to one
     sequence (full pages of a common prefix may be shared)."""
-    device = _lib.require_gpu(k, v, q)
+    device = _lib.require_gpu(k, v, q).index
     k, v = _rows(k), _rows(v)
-    if k.shape != v.shape:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    batch, tokens, kv_heads, head_dim = k.shape
-    pages, held_heads, held_dim = _check_cache(cache, device)
-    if (kv_heads, head_dim) != (held_heads, held_dim):
-        raise ValueError(f"k {tuple(k.shape)} does not fit a cache of {held_heads} heads of "
-                         f"{held_dim}")
-    place = _check_map(page_table, starts, counts, batch, device)
-    q_heads, q_out = 0, None
+    shape = k.shape
+    if shape != v.shape:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} differ")
+    batch, tokens, kv_heads, head_dim = shape
+    place, held_heads, held_dim, _ = _describe(cache, page_table, starts, counts, batch, tokens,
+                                               device)
+    if kv_heads != held_heads or head_dim != held_dim:
+        raise ValueError(f"k {tuple(shape)} does not fit a cache of {held_heads} heads of {held_dim}")
+    q_part, q_heads, q_out = (None, None), 0, None
     if q is not None:
         q = _rows(q)
         q_heads = q.shape[2]
         if q.shape != (batch, tokens, q_heads, head_dim) or q_heads == 0:
-            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
-        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
-    k_out = torch.empty(k.shape, dtype=torch.bfloat16, device=device) if return_keys else None
+            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(shape)}")
+        q_out = _new_rows(q)
+        q_part = (q.data_ptr(), _STRIDES.pack(*q.stride()))
+    k_out = _new_rows(k) if return_keys else None
     table = (None, None, 0, 0)
     if rope is not None:
         cos, sin = rope
-        for x in rope:
-            if x.dtype != torch.float32 or x.dim() != 2 or x.shape != cos.shape \
-                    or not x.is_contiguous():
-                raise ValueError("rope must be two contiguous float32 [positions, rotary_dim // 2] "
-                                 "tensors of one shape")
-            if x.device != device:
-                raise ValueError(f"tensors on different devices: {device} and {x.device}")
-        table = (cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1])
+        if not (cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.dim() == 2
+                and sin.shape == cos.shape and cos.is_contiguous() and sin.is_contiguous()
+                and cos.get_device() == sin.get_device() == device):
+            raise ValueError("rope must be two contiguous float32 [positions, rotary_dim // 2] "
+                             "tensors of one shape on the pages' device")
+        positions, half = cos.shape
+        table = (cos.data_ptr(), sin.data_ptr(), positions, 2 * half)
     if batch and tokens:
-        _call(device, "spx_paged_append", _lib.ptr(q), _lib.strides(q), k.data_ptr(),
-              _lib.strides(k), v.data_ptr(), _lib.strides(v), *table, int(interleaved), *place,
-              *pages, batch, tokens, q_heads, kv_heads, head_dim, _lib.ptr(q_out), _lib.ptr(k_out))
+        _call(device, "spx_paged_append", place, *q_part, k.data_ptr(), _STRIDES.pack(*k.stride()),
+              v.data_ptr(), _STRIDES.pack(*v.stride()), q_heads, *table, int(interleaved),
+              _lib.ptr(q_out), _lib.ptr(k_out))
     return q_out, k_out
 
 
-@torch.no_grad()
 def gather_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Tensor, tokens: int,
                   counts: torch.Tensor | None = None):
     """K and V of positions ``starts[b] .. starts[b] + tokens`` as contiguous bf16
     ``[B, tokens, Hkv, D]`` (4-bit values are exact in bf16); rows that are not live or have no
     place are 0."""
-    device = _lib.require_gpu(cache.key_pages, page_table)
-    pages, kv_heads, head_dim = _check_cache(cache, device)
-    batch = page_table.shape[0]
-    place = _check_map(page_table, starts, counts, batch, device)
+    device = _lib.require_gpu(cache.key_pages, page_table).index
     if tokens < 0:
         raise ValueError(f"tokens must not be negative, got {tokens}")
-    k = torch.empty(batch, tokens, kv_heads, head_dim, dtype=torch.bfloat16, device=device)
-    v = torch.empty_like(k)
+    batch = page_table.shape[0]
+    place, kv_heads, head_dim, _ = _describe(cache, page_table, starts, counts, batch, tokens, device)
+    shape = (batch, tokens, kv_heads, head_dim)
+    k = cache.key_pages.new_empty(shape, dtype=torch.bfloat16)
+    v = cache.key_pages.new_empty(shape, dtype=torch.bfloat16)
     if batch and tokens:
-        _call(device, "spx_paged_gather", *place, *pages, batch, tokens, kv_heads, head_dim,
-              k.data_ptr(), v.data_ptr())
+        _call(device, "spx_paged_gather", place, k.data_ptr(), v.data_ptr())
     return k, v
 
 
-@torch.no_grad()
 def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor,
                     starts: torch.Tensor, scale: float, counts: torch.Tensor | None = None,
                     max_keys: int | None = None, return_lse: bool = False):
@@ -248,23 +269,22 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     ``max_keys``: an upper bound of ``starts[b] + T`` where the caller has one; it only chooses
     how the work is divided. Meant for decode steps and a few drafted tokens: each 16 of the
     T x Hq / Hkv rows of a KV head read K and V anew."""
-    device = _lib.require_gpu(q, cache.key_pages)
+    device = _lib.require_gpu(q, cache.key_pages).index
     q = _rows(q)
-    batch, tokens, q_heads, head_dim = q.shape
-    pages, kv_heads, held_dim = _check_cache(cache, device)
+    shape = q.shape
+    batch, tokens, q_heads, head_dim = shape
+    place, kv_heads, held_dim, sizes = _describe(cache, page_table, starts, counts, batch, tokens,
+                                                 device)
     if head_dim != held_dim or q_heads == 0 or kv_heads == 0 or q_heads % kv_heads:
-        raise ValueError(f"q {tuple(q.shape)} does not fit a cache of {kv_heads} heads of {held_dim}")
-    place = _check_map(page_table, starts, counts, batch, device)
-    bound = 0 if max_keys is None else max_keys
+        raise ValueError(f"q {tuple(shape)} does not fit a cache of {kv_heads} heads of {held_dim}")
+    bound = 0 if max_keys is None else int(max_keys)
     if bound < 0:
         raise ValueError(f"max_keys must not be negative, got {max_keys}")
-    out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device) if return_lse else None
+    out = _new_rows(q)
+    lse = q.new_empty(shape[:3], dtype=torch.float32) if return_lse else None
     if batch and tokens:
-        shape = (batch, tokens, q_heads, kv_heads, head_dim)
-        nbytes = _lib.load().spx_paged_attention_workspace_bytes(
-            place[2], pages[5], bound, cache.four_bit, *shape)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
-        _call(device, "spx_paged_attention", q.data_ptr(), _lib.strides(q), *place, *pages, bound,
-              *shape, float(scale), _lib.ptr(workspace), out.data_ptr(), _lib.ptr(lse))
+        nbytes = _workspace_bytes(cache.key_scales is not None, sizes, q_heads, bound)
+        workspace = q.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None
+        _call(device, "spx_paged_attention", place, q.data_ptr(), _STRIDES.pack(*q.stride()), q_heads,
+              bound, float(scale), _lib.ptr(workspace), out.data_ptr(), _lib.ptr(lse))
     return (out, lse) if return_lse else out

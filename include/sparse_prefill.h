@@ -323,20 +323,39 @@ int spx_decode_attention(const void* q, const int64_t* q_strides, const void* k,
 
 /* ------------------------------------------------------- paged KV cache */
 
-/* A cache of fixed-size pages that sequences share out among themselves. key_pages,
- * value_pages: bf16 [pages, Hkv, page_size, D] contiguous, 16-byte aligned, or (key_scales
- * and value_scales not NULL) 4 bits: [pages, Hkv, page_size, D / 2] bytes of E2M1 values
- * (the even dim in the low half) with key_scales / value_scales
- * [pages, Hkv, page_size, D / 32], 8-byte aligned: E8M0, byte e scales by 2^(e - 127), 255
- * is NaN. page_size: a power of two from 16 to 1024.
- * page_table: int32, batch rows table_stride elements apart of table_width page ids.
- * Position p of sequence b is slot p % page_size of page page_table[b][p / page_size].
- * The `tokens` new tokens of sequence b have positions starts[b] + i. Token i is live if
+/* A cache of fixed-size pages that sequences share out among themselves, and the tokens that
+ * a call is about. All pointers are device pointers.
+ * key_pages, value_pages: bf16 [pages, kv_heads, page_size, head_dim] contiguous, 16-byte
+ * aligned, or (key_scales and value_scales not NULL) 4 bits:
+ * [pages, kv_heads, page_size, head_dim / 2] bytes of E2M1 values (the even dim in the low
+ * half) with scales [pages, kv_heads, page_size, head_dim / 32], 8-byte aligned: E8M0, byte e
+ * scales by 2^(e - 127), 255 is NaN. page_size: a power of two from 16 to 1024.
+ * page_table: `batch` rows, table_stride elements apart, of table_width page ids. Position p of
+ * sequence b is slot p % page_size of page page_table[b][p / page_size].
+ * The `tokens` tokens of sequence b have positions starts[b] + i. Token i is live if
  * starts[b] >= 0, i < counts[b] (counts may be NULL) and its position is below
  * table_width * page_size (at most 2^30); a position whose page id is outside [0, pages) has
- * no place. starts, counts: int32 [batch], device memory.
+ * no place.
  * The reference keeps its KV cache in transformers' DynamicCache (evaluate.py); these entry
  * points have no counterpart in it. */
+typedef struct spx_paged_cache {
+  void* key_pages;
+  void* value_pages;
+  void* key_scales;
+  void* value_scales;
+  const int32_t* page_table;
+  const int32_t* starts;     /* [batch] */
+  const int32_t* counts;     /* [batch] or NULL */
+  int64_t table_stride;
+  int32_t table_width;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t batch;
+  int32_t tokens;
+  int32_t reserved;          /* 0 */
+} spx_paged_cache;
 
 /* Append: rotate k (and q), store k and v. k, v: bf16 [B, T, Hkv, D], q: bf16 [B, T, Hq, D]
  * or NULL; strides in that order, 16-byte aligned bases, batch / token / head strides
@@ -351,42 +370,30 @@ int spx_decode_attention(const void* q, const int64_t* q_strides, const void* k,
  * into [3.5, 7) (scale bytes 2 to 252; 255 where one of them is not finite).
  * Nothing is written for tokens that are not live or have no place. Two tokens of one call
  * with the same place (a page that the table names twice) leave it unspecified. */
-int spx_paged_append(const void* q, const int64_t* q_strides, const void* k,
-                     const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                     const float* rope_cos, const float* rope_sin, int rope_positions,
-                     int rotary_dim, int interleaved, const int32_t* page_table,
-                     int64_t table_stride, int table_width, const int32_t* starts,
-                     const int32_t* counts, void* key_pages, void* value_pages, void* key_scales,
-                     void* value_scales, int pages, int page_size, int batch, int tokens,
-                     int q_heads, int kv_heads, int head_dim, void* q_out, void* k_out,
-                     void* stream);
+int spx_paged_append(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
+                     const void* k, const int64_t* k_strides, const void* v,
+                     const int64_t* v_strides, int q_heads, const float* rope_cos,
+                     const float* rope_sin, int rope_positions, int rotary_dim, int interleaved,
+                     void* q_out, void* k_out, void* stream);
 
-/* Read back: k_out, v_out contiguous bf16 [B, T, Hkv, D] of positions starts[b] + i; rows of
+/* Read back: k_out, v_out contiguous bf16 [B, T, Hkv, D] of the tokens' positions; rows of
  * tokens that are not live or have no place are 0. 4-bit values are exact in bf16. */
-int spx_paged_gather(const int32_t* page_table, int64_t table_stride, int table_width,
-                     const int32_t* starts, const int32_t* counts, const void* key_pages,
-                     const void* value_pages, const void* key_scales, const void* value_scales,
-                     int pages, int page_size, int batch, int tokens, int kv_heads, int head_dim,
-                     void* k_out, void* v_out, void* stream);
+int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out, void* stream);
 
-/* Attention of the new tokens over the cache that already holds them: token i of sequence b
+/* Attention of the tokens over the cache that already holds them: token i of sequence b
  * sees positions 0 .. starts[b] + i, out = softmax(scale q K^T) V. q: bf16 [B, T, Hq, D]
  * (strides as above); out: contiguous bf16 [B, T, Hq, D]; lse: natural-log LSE, contiguous
  * fp32 [B, T, Hq], or NULL. Positions without a place are not seen. Tokens that are not live,
  * or see nothing, give 0 and an LSE of -inf. max_keys: an upper bound of starts[b] + T that
  * the caller knows, or 0; it only chooses how the work is divided. workspace: device memory
- * of spx_paged_attention_workspace_bytes(...) bytes for the same max_keys (-1: unsupported
- * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after.
- * Results do not depend on the launch's timing. */
-int64_t spx_paged_attention_workspace_bytes(int table_width, int page_size, int max_keys,
-                                            int four_bit, int batch, int tokens, int q_heads, int kv_heads,
-                                            int head_dim);
-int spx_paged_attention(const void* q, const int64_t* q_strides, const int32_t* page_table,
-                        int64_t table_stride, int table_width, const int32_t* starts,
-                        const int32_t* counts, const void* key_pages, const void* value_pages,
-                        const void* key_scales, const void* value_scales, int pages,
-                        int page_size, int max_keys, int batch, int tokens, int q_heads,
-                        int kv_heads, int head_dim, float scale, void* workspace, void* out,
+ * of spx_paged_attention_workspace_bytes(...) bytes for the same arguments (-1: unsupported
+ * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after;
+ * the size depends on the cache's sizes only, not on its pointers (but on whether there are
+ * scales). Results do not depend on the launch's timing. */
+int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* cache, int q_heads,
+                                            int max_keys);
+int spx_paged_attention(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
+                        int q_heads, int max_keys, float scale, void* workspace, void* out,
                         float* lse, void* stream);
 
 /* ----------------------------------------------------------- accounting */

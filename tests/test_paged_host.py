@@ -10,67 +10,69 @@ from exp3_amd import _lib, paged
 import paged_reference as ref
 
 FAKE, OFF = 1 << 20, (1 << 20) + 8
-S4 = (ctypes.c_int64 * 4)(4096, 512, 128, 1)
-ODD = (ctypes.c_int64 * 4)(4096, 512, 132, 1)
+S4 = bytes((ctypes.c_int64 * 4)(4096, 512, 128, 1))
+ODD = bytes((ctypes.c_int64 * 4)(4096, 512, 132, 1))
 
 
-def _append(q=FAKE, k=FAKE, ks=S4, cos=FAKE, sin=FAKE, rope=(4096, 128, 0), table=(FAKE, 32, 32),
-            starts=FAKE, pages=(FAKE, FAKE, None, None), sizes=(64, 128), shape=(2, 1, 28, 4, 128),
-            q_out=FAKE, k_out=None):
-    return _lib.load().spx_paged_append(q, S4, k, ks, FAKE, S4, cos, sin, *rope, *table, starts,
-                                        None, *pages, *sizes, *shape, q_out, k_out, None)
+def _cache(pages=(FAKE, FAKE, 0, 0), table=FAKE, starts=FAKE, counts=0, stride=32, width=32, held=64,
+           page_size=128, kv_heads=4, dim=128, batch=2, tokens=1):
+    return paged._DESCRIPTION.pack(*pages, table, starts, counts, stride, width, held, page_size,
+                                   kv_heads, dim, batch, tokens, 0)
 
 
-def _gather(table=(FAKE, 32, 32), pages=(FAKE, FAKE, None, None), sizes=(64, 128),
-            shape=(2, 1, 4, 128), out=FAKE):
-    return _lib.load().spx_paged_gather(*table, FAKE, None, *pages, *sizes, *shape, out, FAKE, None)
+def _append(cache=None, q=FAKE, k=FAKE, ks=S4, q_heads=28, cos=FAKE, sin=FAKE, rope=(4096, 128, 0),
+            q_out=FAKE, k_out=None, **more):
+    return _lib.load().spx_paged_append(cache or _cache(**more), q, S4, k, ks, FAKE, S4, q_heads, cos,
+                                        sin, *rope, q_out, k_out, None)
 
 
-def _attention(q=FAKE, qs=S4, table=(FAKE, 32, 32), pages=(FAKE, FAKE, None, None), sizes=(64, 128),
-               max_keys=0, shape=(2, 1, 28, 4, 128), workspace=FAKE, out=FAKE):
-    return _lib.load().spx_paged_attention(q, qs, *table, FAKE, None, *pages, *sizes, max_keys,
-                                           *shape, 0.1, workspace, out, None, None)
+def _gather(out=FAKE, **more):
+    return _lib.load().spx_paged_gather(_cache(**more), out, FAKE, None)
 
 
-@pytest.mark.parametrize("call,heads", ((_append, (28, 4)), (_gather, (4,)), (_attention, (28, 4))))
-def test_shared_arguments(call, heads):
+def _attention(q=FAKE, qs=S4, q_heads=28, max_keys=0, workspace=FAKE, out=FAKE, **more):
+    return _lib.load().spx_paged_attention(_cache(**more), q, qs, q_heads, max_keys, 0.1, workspace,
+                                           out, None, None)
+
+
+@pytest.mark.parametrize("call", (_append, _gather, _attention))
+def test_shared_arguments(call):
     unsupported, invalid = _lib.SPX_EUNSUPPORTED, _lib.SPX_EINVAL
     for size in (8, 24, 100, 2048):
-        assert call(sizes=(64, size)) == unsupported and b"page_size" in _lib.load().spx_last_error()
-    assert call(shape=(2, 1, *heads, 64)) == unsupported
-    for shape in ((0, 1, *heads, 128), (2, 0, *heads, 128), (2, 1, *heads[:-1], 0, 128)):
-        assert call(shape=shape) == invalid
-    assert call(sizes=(0, 128)) == invalid
-    assert call(table=(None, 32, 32)) == call(table=(FAKE, 32, 0)) == invalid
-    assert call(table=(FAKE, 32, (1 << 23) + 1)) == invalid       # 2^30 + 128 positions
-    for pages in ((None, FAKE, None, None), (FAKE, OFF, None, None), (FAKE, FAKE, FAKE, None),
+        assert call(page_size=size) == unsupported and b"page_size" in _lib.load().spx_last_error()
+    assert call(dim=64) == unsupported
+    assert call(batch=0) == call(tokens=0) == call(kv_heads=0) == call(held=0) == invalid
+    assert call(table=0) == call(width=0) == call(starts=0) == invalid
+    assert call(width=(1 << 23) + 1) == invalid                   # 2^30 + 128 positions
+    for pages in ((0, FAKE, 0, 0), (FAKE, OFF, 0, 0), (FAKE, FAKE, FAKE, 0),
                   (FAKE, FAKE, FAKE, FAKE + 4)):
         assert call(pages=pages) == invalid
+    assert call(table=FAKE + 2) == call(starts=FAKE + 1) == call(counts=FAKE + 2) == invalid
 
 
 def test_append_arguments():
     unsupported, invalid = _lib.SPX_EUNSUPPORTED, _lib.SPX_EINVAL
-    assert _append(k=None) == _append(k=OFF) == _append(ks=ODD) == _append(starts=None) == invalid
-    assert _append(q_out=None) == _append(k_out=OFF) == _append(q=OFF) == invalid
+    assert _lib.load().spx_paged_append(None, *[None] * 6, 0, None, None, 0, 0, 0, None, None,
+                                        None) == invalid
+    assert _append(k=None) == _append(k=OFF) == _append(ks=ODD) == invalid
+    assert _append(q_out=None) == _append(k_out=OFF) == _append(q=OFF) == _append(q_heads=0) == invalid
     assert _append(sin=None) == _append(cos=OFF) == invalid
     assert _append(rope=(4095, 128, 0)) == invalid                # the table reaches 4096
     for rotary in (0, 8, 120, 144):
         assert _append(rope=(4096, rotary, 0)) == unsupported
-    assert _append(shape=(1 << 20, 1 << 10, 28, 4, 128)) == invalid
+    assert _append(batch=1 << 20, tokens=1 << 10) == invalid
 
 
 def test_gather_and_attention_arguments():
     invalid = _lib.SPX_EINVAL
-    assert _gather(out=None) == _gather(out=OFF) == invalid
+    assert _gather(out=None) == _gather(out=OFF) == _gather(batch=1 << 20, tokens=1 << 12) == invalid
     assert _attention(q=None) == _attention(q=OFF) == _attention(qs=ODD) == invalid
-    assert _attention(out=None) == _attention(max_keys=-1) == invalid
-    assert _attention(shape=(2, 1, 27, 4, 128)) == _attention(shape=(1 << 16, 1 << 10, 32, 4, 128)) \
-        == invalid
+    assert _attention(out=None) == _attention(max_keys=-1) == _attention(workspace=None) == invalid
+    assert _attention(q_heads=27) == _attention(batch=1 << 16, tokens=1 << 10, q_heads=32) == invalid
     size = _lib.load().spx_paged_attention_workspace_bytes
-    assert size(32, 128, 0, 0, 2, 1, 28, 4, 128) >= 0
-    for bad in ((32, 128, 0, 0, 2, 1, 27, 4, 128), (32, 128, 0, 1, 0, 1, 28, 4, 128),
-                (32, 128, 0, 0, 2, 1, 28, 4, 64), (32, 128, -1, 1, 2, 1, 28, 4, 128)):
-        assert size(*bad) == -1
+    assert size(_cache(), 28, 0) > 0 and size(_cache(), 28, 100) == 0
+    assert size(None, 28, 0) == size(_cache(), 27, 0) == size(_cache(), 28, -1) == -1
+    assert size(_cache(batch=0), 28, 0) == size(_cache(dim=64), 28, 0) == -1
 
 
 def test_wrappers_refuse():
@@ -89,31 +91,37 @@ def test_wrappers_refuse():
 
 def test_wrapper_checks_of_shapes():
     """The checks that need no GPU tensors of their own, on the CPU."""
-    cpu = torch.device("cpu")
+    cpu = -1                        # the index of a CPU tensor
     good = paged.empty_pages(4, 16, 2, 128, "cpu", four_bit=True)
-    assert paged._check_cache(good, cpu)[1:] == (2, 128)
+    assert paged._check_cache(good, cpu)[1:] == (4, 16, 2, 128)
     assert (good.page_size, good.kv_heads, good.head_dim, good.four_bit) == (16, 2, 128, True)
     half = paged.empty_pages(4, 16, 2, 256, "cpu")
-    assert paged._check_cache(half, cpu)[1:] == (2, 256) and half.head_dim == 256
+    assert paged._check_cache(half, cpu)[1:] == (4, 16, 2, 256) and half.head_dim == 256
     bad = (paged.PagedCache(good.key_pages, good.value_pages, good.key_scales),
+           paged.PagedCache(half.key_pages, half.value_pages, None, good.value_scales),
            paged.PagedCache(good.key_pages, good.value_pages),
            paged.PagedCache(half.key_pages, half.value_pages[:3]),
            paged.PagedCache(half.key_pages.transpose(1, 2), half.value_pages.transpose(1, 2)),
            paged.PagedCache(half.key_pages.half(), half.value_pages.half()),
+           paged.PagedCache(half.key_pages[0], half.value_pages[0]),
            paged.PagedCache(good.key_pages, good.value_pages, good.key_scales[..., :2],
                             good.value_scales[..., :2]))
     for cache in bad:
         with pytest.raises(ValueError):
             paged._check_cache(cache, cpu)
+    with pytest.raises(ValueError, match="device"):
+        paged._check_cache(half, 0)
     table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
-    paged._check_map(table, starts, starts, 2, cpu)
-    paged._check_map(torch.zeros(2, 9, dtype=torch.int32)[:, 2:6], starts, None, 2, cpu)
+    _, heads, dim, sizes = paged._describe(good, table, starts, starts, 2, 3, cpu)
+    assert (heads, dim) == (2, 128) and sizes == (4, 4, 16, 2, 128, 2, 3, 0)
+    assert paged._describe(good, torch.zeros(2, 9, dtype=torch.int32)[:, 2:6], starts, None, 2, 3,
+                           cpu)[3] == sizes
     for wrong in ((table.long(), starts, None), (table, starts.long(), None), (table[:1], starts, None),
                   (table, starts[:1], None), (table, starts, starts.long()),
                   (table.repeat(1, 2)[:, ::2], starts, None),
                   (table, torch.zeros(4, dtype=torch.int32)[::2], None)):
         with pytest.raises(ValueError):
-            paged._check_map(*wrong, 2, cpu)
+            paged._describe(good, *wrong, 2, 3, cpu)
 
 
 def test_rope_table_far_positions():
