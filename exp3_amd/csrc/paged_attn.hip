@@ -39,11 +39,13 @@ constexpr int kPaThreads = 256, kPaWaves = kPaThreads / 64;
 constexpr int kPaCols = 16;
 constexpr int kPaMaxGrid = 1024;         // workgroups that share the units (weights in the merge)
 constexpr int kPaCus = 256;
+constexpr int kPaMinUnit = 128;          // keys of the smallest unit
 
 template <int D, bool kFour>
 struct PagedShape {
   static constexpr int kTiles = kFour ? 4 : 2;                 // 16-key tiles per wave and unit
   static constexpr int kUnit = 16 * kTiles * kPaWaves;         // keys of a unit
+  static_assert(kUnit >= kPaMinUnit, "units are counted in 32 bits");
   static constexpr int kPerCu = D == 128 ? 3 : 2;              // resident workgroups
 };
 
@@ -64,6 +66,7 @@ struct PagedAttnArgs {
   float* lse;
   float* part_o;                         // [2 grid][16][D]
   float* part_ml;                        // [2 grid][16][2]
+  u32x2* parts;                          // [streams] first partial's slot, how many (1: written out)
 };
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -80,108 +83,106 @@ __device__ __forceinline__ float part_weight(float m, float top) {
 
 // ---------------------------------------------------------------- division of the work
 
+// Device data that no kernel of the stream writes meanwhile, at a uniform address.
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
 // Live tokens of a sequence: 0 .. live - 1.
-__device__ __forceinline__ int live_tokens(const PagedAttnArgs& a, int b, int& start) {
-  start = a.map.starts[b];
-  int live = a.map.counts ? min(a.map.counts[b], a.tokens) : a.tokens;
-  if (start < 0) live = 0;
+__device__ __forceinline__ int live_tokens(const PagedAttnArgs& a, int start, int count) {
   const int64_t room = a.map.capacity() - start;
-  return room < live ? (int)max(room, (int64_t)0) : max(live, 0);
+  const int live = min(min(count, a.tokens), (int)min(room, (int64_t)a.tokens));
+  return start < 0 ? 0 : max(live, 0);
+}
+
+// Tokens of a column tile: the first and the last.
+__device__ __forceinline__ int tile_first(const PagedAttnArgs& a, int tile) {
+  return a.col_tiles == 1 ? 0 : tile * kPaCols / a.group;
+}
+__device__ __forceinline__ int tile_last(const PagedAttnArgs& a, int tile) {
+  return a.col_tiles == 1 ? a.tokens - 1 : (min((tile + 1) * kPaCols, a.cols) - 1) / a.group;
 }
 
 // Keys that a column tile of a sequence sees at most.
 __device__ __forceinline__ int tile_keys(const PagedAttnArgs& a, int start, int live, int tile) {
-  const int first = tile * kPaCols / a.group;
-  const int last = min((min((tile + 1) * kPaCols, a.cols) - 1) / a.group, live - 1);
-  return last < first ? 0 : start + last + 1;
+  const int last = min(tile_last(a, tile), live - 1);
+  return last < tile_first(a, tile) ? 0 : start + last + 1;
 }
 
+// Units of a sequence's streams of one KV head.
 template <int kUnit>
-__device__ __forceinline__ int64_t head_units(const PagedAttnArgs& a, int b) {
-  int start;
-  const int live = live_tokens(a, b, start);
-  int64_t units = 0;
+__device__ __forceinline__ int head_units(const PagedAttnArgs& a, int start, int count) {
+  const int live = live_tokens(a, start, count);
+  int units = 0;
   for (int tile = 0; tile < a.col_tiles; ++tile)
     units += (tile_keys(a, start, live, tile) + kUnit - 1) / kUnit;
   return units;
 }
 
-struct Run {                             // units begin .. end of the workgroup w
-  int64_t per;
-  int rest;
-  __device__ __forceinline__ Run(int64_t total, int grid)
-      : per(total / grid), rest((int)(total % grid)) {}
-  __device__ __forceinline__ int64_t begin(int w) const { return w * per + min(w, rest); }
-  __device__ __forceinline__ int owner(int64_t u) const {
-    const int64_t wide = rest * (per + 1);
-    return (int)(u < wide ? u / (per + 1) : rest + (u - wide) / per);
-  }
-};
-
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-  const int lo = __builtin_amdgcn_readlane((int)x, lane);
-  const int hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
-  return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
-}
-
-__device__ __forceinline__ int64_t wave_prefix(int64_t x, int lane) {     // inclusive
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int64_t y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);    // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);    // row_bcast 15, 31
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
   return x;
 }
 
-// All units, and those of the sequences before b.
-template <int kUnit>
-__device__ __forceinline__ int64_t count_units(const PagedAttnArgs& a, int lane, int b,
-                                               int64_t& before) {
-  int64_t total = 0;
-  before = 0;
-  for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-    const int64_t units = b0 + lane < a.batch ? head_units<kUnit>(a, b0 + lane) * a.kv_heads : 0;
-    const int64_t sum = wave_prefix(units, lane);
-    if (b >= b0 && b < b0 + kWave) before = total + lane_value(sum - units, b - b0);
-    total += lane_value(sum, kWave - 1);
+// The units of 64 sequences, one a lane, and their prefix sums.
+struct UnitScan {
+  int units, sum, each;                  // each: of one KV head
+  template <int kUnit>
+  __device__ __forceinline__ void load(const PagedAttnArgs& a, int b) {
+    each = 0;
+    if (b < a.batch)
+      each = head_units<kUnit>(a, a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
+    units = each * a.kv_heads;
+    sum = wave_prefix(units);
   }
-  return total;
-}
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, kWave - 1); }
+};
+
+struct Run {                             // units begin(w) .. begin(w + 1) - 1 of workgroup w
+  int per, rest;
+  __device__ __forceinline__ Run(int total, int grid) : per(total / grid), rest(total % grid) {}
+  __device__ __forceinline__ int begin(int w) const { return w * per + min(w, rest); }
+  __device__ __forceinline__ int owner(int u) const {
+    const int wide = rest * (per + 1);
+    return u < wide ? u / (per + 1) : rest + (u - wide) / max(per, 1);
+  }
+};
 
 struct Stream {
   int b, kvh, tile, start, live, keys, units;
-  int64_t first;                         // of its units
+  int first;                             // of its units
 
   template <int kUnit>
   __device__ __forceinline__ void measure(const PagedAttnArgs& a) {
-    live = live_tokens(a, b, start);
-    start = first_lane(start);
-    live = first_lane(live);
+    start = scalar_load(a.map.starts + b);
+    live = live_tokens(a, start, a.map.counts ? scalar_load(a.map.counts + b) : a.tokens);
     keys = tile_keys(a, start, live, tile);
     units = (keys + kUnit - 1) / kUnit;
   }
-  // The stream of unit u. false: there is none (lengths that change under the launch must not
-  // make it loop).
+  // The stream of unit u; scan: that of the sequences 0 .. 63. false: there is none (lengths
+  // that change under the launch must not make it loop).
   template <int kUnit>
-  __device__ __forceinline__ bool find(const PagedAttnArgs& a, int lane, int64_t u) {
-    int64_t total = 0;
-    b = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += kWave) {
-      const int64_t units = b0 + lane < a.batch ? head_units<kUnit>(a, b0 + lane) * a.kv_heads : 0;
-      const int64_t sum = wave_prefix(units, lane);
-      const uint64_t past = __ballot(total + sum > u);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        b = b0 + l;
-        total += lane_value(sum - units, l);
-        break;
-      }
-      total += lane_value(sum, kWave - 1);
+  __device__ __forceinline__ bool find(const PagedAttnArgs& a, int lane, UnitScan scan, int u) {
+    int before = 0, b0 = 0;
+    uint64_t past;
+    while (!(past = __ballot(before + scan.sum > u))) {
+      before += scan.total();
+      b0 += kWave;
+      if (b0 >= a.batch) return false;
+      scan.load<kUnit>(a, b0 + lane);
     }
-    b = first_lane(b);
-    const int64_t each = max(head_units<kUnit>(a, b), (int64_t)1);
-    kvh = min(first_lane((int)((u - total) / each)), a.kv_heads - 1);
-    first = total + kvh * each;
+    const int l = __builtin_ctzll(past);
+    b = b0 + l;
+    before += __builtin_amdgcn_readlane(scan.sum - scan.units, l);
+    const int each = __builtin_amdgcn_readlane(scan.each, l);
+    kvh = (u - before) / each;
+    first = before + kvh * each;
     for (tile = 0; tile < a.col_tiles; ++tile) {
       measure<kUnit>(a);
       if (u < first + units) return true;
@@ -479,30 +480,39 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
   const int c = lane & 15, g = lane >> 4;
 
   Stream s;
-  int64_t u, end, begin;
+  Run run(0, 1);
+  int u, end;
   if (a.grid > 0) {
-    int64_t unused;
-    const Run run(count_units<Shape::kUnit>(a, lane, 0, unused), a.grid);
-    begin = u = run.begin(blockIdx.x);
+    UnitScan scan;
+    scan.load<Shape::kUnit>(a, lane);
+    int total = scan.total();
+    for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
+      UnitScan more;
+      more.load<Shape::kUnit>(a, b0 + lane);
+      total += more.total();
+    }
+    run = Run(total, a.grid);
+    u = run.begin(blockIdx.x);
     end = run.begin(blockIdx.x + 1);
-    if (u >= end) return;
-    if (!s.find<Shape::kUnit>(a, lane, u)) return;
+    if (u >= end || !s.find<Shape::kUnit>(a, lane, scan, u)) return;
   } else {
     const int stream = blockIdx.x;
     s.tile = stream % a.col_tiles;
     s.kvh = stream / a.col_tiles % a.kv_heads;
     s.b = stream / a.col_tiles / a.kv_heads;
-    s.first = begin = u = 0;
+    s.first = u = 0;
     s.measure<Shape::kUnit>(a);
     end = s.units;
   }
+  const int begin = u;
 
   for (;;) {
     const int cols = min(kPaCols, a.cols - s.tile * kPaCols);
     const int n = s.tile * kPaCols + min(c, cols - 1);    // columns past the last repeat it
-    const int token = n / a.group, head = s.kvh * a.group + n % a.group;
+    const int token = a.tokens == 1 ? 0 : n / a.group;
+    const int head = s.kvh * a.group + n - token * a.group;
     const int limit = s.start + token;
-    const int first_limit = s.start + s.tile * kPaCols / a.group;
+    const int first_limit = s.start + tile_first(a, s.tile);
     u32x4 q[KK];
     const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
 #pragma unroll
@@ -513,7 +523,7 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
     }
     Accumulator<D, kFour> acc;
     acc.clear();
-    const int j0 = (int)(u - s.first), j1 = (int)(min(end, s.first + s.units) - s.first);
+    const int j0 = u - s.first, j1 = min(end, s.first + s.units) - s.first;
     for (int jb = j0; jb < j1; jb += kIdUnits) {
       // page ids of the wave's tiles in units jb .. jb + kIdUnits - 1
       const int p = (jb + lane / T) * Shape::kUnit + (w * T + lane % T) * 16;
@@ -541,6 +551,11 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
     block_sync();
     const bool whole = j0 == 0 && j1 == s.units;
     const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
+    if (a.grid > 0 && j0 == 0 && threadIdx.x == 0) {
+      const int parts = whole ? 1 : run.owner(s.first + s.units - 1) - blockIdx.x + 1;
+      a.parts[(s.b * a.kv_heads + s.kvh) * a.col_tiles + s.tile] =
+          u32x2{(uint32_t)slot, (uint32_t)parts};
+    }
     for (int e = threadIdx.x; e < cols * (D / 4); e += kPaThreads) {
       const int col = e / (D / 4), d = (e % (D / 4)) * 4;
       float top = part_m[0][col];
@@ -557,14 +572,15 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
         for (int y = 0; y < 4; ++y) v[y] += wt * po[y];
       }
       const int cn = s.tile * kPaCols + col;
-      if (cn / a.group >= s.live) {      // not live: sees nothing, whatever step() added
+      const int ct = a.tokens == 1 ? 0 : cn / a.group;
+      if (ct >= s.live) {      // not live: sees nothing, whatever step() added
         v = f32x4{};
         sum = 0.0f;
         top = -INFINITY;
       }
       if (whole) {
-        const int64_t row = ((int64_t)s.b * a.tokens + cn / a.group) * a.q_heads +
-                            s.kvh * a.group + cn % a.group;
+        const int64_t row = ((int64_t)s.b * a.tokens + ct) * a.q_heads + s.kvh * a.group + cn -
+                            ct * a.group;
         const float inv = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
         u32x2 packed;
         packed[0] = pack_bf16x2(v[0] * inv, v[1] * inv);
@@ -590,9 +606,8 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
 // without keys are written here.
 constexpr int kPaMergeDims = 64;
 
-template <int D, bool kFour>
+template <int D>
 __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a) {
-  using Shape = PagedShape<D, kFour>;
   constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaThreads / kLanes;
   __shared__ float weight[kPaMaxGrid];
   __shared__ float red[2][kPaWaves];
@@ -600,32 +615,23 @@ __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int h = (int)(row % a.q_heads), i = (int)(row / a.q_heads % a.tokens);
-  Stream s;
-  s.b = (int)(row / a.q_heads / a.tokens);
-  s.kvh = h / a.group;
-  const int n = i * a.group + h % a.group;
-  int64_t before;
-  const Run run(count_units<Shape::kUnit>(a, lane, s.b, before), a.grid);
-  const int64_t each = head_units<Shape::kUnit>(a, s.b);
-  s.first = before + s.kvh * each;
-  for (s.tile = 0;; ++s.tile) {
-    s.measure<Shape::kUnit>(a);
-    if (s.tile == n / kPaCols) break;
-    s.first += s.units;
-  }
-  const int col = n % kPaCols, d0 = blockIdx.y * kPaMergeDims;
+  const int b = (int)(row / a.q_heads / a.tokens);
+  const int kvh = h / a.group, n = i * a.group + h - kvh * a.group;
+  const int tile = n / kPaCols, col = n % kPaCols, d0 = blockIdx.y * kPaMergeDims;
+  const int start = a.map.starts[b];
+  const int live = live_tokens(a, start, a.map.counts ? a.map.counts[b] : a.tokens);
+  const u32x2 held = a.parts[(b * a.kv_heads + kvh) * a.col_tiles + tile];
   const int dim = d0 + tid % kLanes * 4, gr = tid / kLanes;
-  if (s.units == 0) {
+  if (tile_keys(a, start, live, tile) == 0) {
     if (gr == 0) *reinterpret_cast<u32x2*>(a.out + row * D + dim) = u32x2{};
     if (tid == 0 && d0 == 0 && a.lse) a.lse[row] = -INFINITY;
     return;
   }
-  const int w0 = run.owner(s.first), w1 = run.owner(s.first + s.units - 1);
-  if (w0 == w1) return;
-  const int parts = w1 - w0 + 1;
-  // the stream is the first one of every workgroup but perhaps w0
-  const int slot0 = 2 * w0 + (run.begin(w0) == s.first ? 0 : 1);
-  auto slot = [&](int x) { return x == 0 ? slot0 : 2 * (w0 + x); };
+  const int slot0 = (int)min(held[0], 2u * a.grid - 1);          // in bounds whatever it holds
+  const int parts = min((int)held[1], a.grid - slot0 / 2);
+  if (parts == 1) return;
+  // the stream is the first one of every workgroup but perhaps the first
+  auto slot = [&](int x) { return x == 0 ? slot0 : (slot0 & ~1) + 2 * x; };
   float top = -INFINITY;
   for (int x = tid; x < parts; x += kPaThreads)
     top = fmaxf(top, a.part_ml[(slot(x) * kPaCols + col) * 2]);
@@ -691,9 +697,11 @@ static bool paged_sizes(const spx_paged_cache& z, int q_heads, int max_keys, Pag
   if ((double)z.batch * z.tokens * q_heads > 0x7fffffff) return false;
   s.rows = (int64_t)z.batch * z.tokens * q_heads;
   s.keys = (int64_t)z.table_width * z.page_size;
-  if (max_keys > 0) s.keys = std::min<int64_t>(s.keys, max_keys);
   const int64_t cols = (int64_t)z.tokens * (q_heads / z.kv_heads);
   s.streams = (int64_t)z.batch * z.kv_heads * ((cols + kPaCols - 1) / kPaCols);
+  // units are counted in 32 bits, also where max_keys is no bound after all
+  if ((s.keys + kPaMinUnit - 1) / kPaMinUnit > 0x7fffffff / s.streams) return false;
+  if (max_keys > 0) s.keys = std::min<int64_t>(s.keys, max_keys);
   return true;
 }
 
@@ -710,12 +718,12 @@ static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, h
                 SPX_EINVAL, "paged_attention: workspace null or not 16-byte aligned");
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
+    a.parts = reinterpret_cast<u32x2*>(a.part_ml + (int64_t)2 * a.grid * kPaCols * 2);
   }
   paged_attn_kernel<D, kFour>
       <<<(unsigned)(a.grid > 0 ? a.grid : z.streams), kPaThreads, 0, st>>>(a);
   if (a.grid > 0)
-    paged_merge_kernel<D, kFour>
-        <<<dim3((unsigned)z.rows, D / kPaMergeDims), kPaThreads, 0, st>>>(a);
+    paged_merge_kernel<D><<<dim3((unsigned)z.rows, D / kPaMergeDims), kPaThreads, 0, st>>>(a);
   return launch_status("paged_attention");
 }
 
@@ -729,8 +737,8 @@ extern "C" int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* ca
   if (cache == nullptr || !paged_sizes(*cache, q_heads, max_keys, z) ||
       (cache->head_dim != 128 && cache->head_dim != 256))
     return -1;
-  return (int64_t)2 * paged_grid_of(z, cache->head_dim, cache->key_scales != nullptr) * kPaCols *
-         (cache->head_dim + 2) * 4;
+  const int grid = paged_grid_of(z, cache->head_dim, cache->key_scales != nullptr);
+  return grid == 0 ? 0 : (int64_t)2 * grid * kPaCols * (cache->head_dim + 2) * 4 + z.streams * 8;
 }
 
 extern "C" int spx_paged_attention(const spx_paged_cache* cache, const void* q,

@@ -384,7 +384,8 @@ int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out, voi
  * sees positions 0 .. starts[b] + i, out = softmax(scale q K^T) V. q: bf16 [B, T, Hq, D]
  * (strides as above); out: contiguous bf16 [B, T, Hq, D]; lse: natural-log LSE, contiguous
  * fp32 [B, T, Hq], or NULL. Positions without a place are not seen. Tokens that are not live,
- * or see nothing, give 0 and an LSE of -inf. max_keys: an upper bound of starts[b] + T that
+ * or see nothing, give 0 and an LSE of -inf. batch * kv_heads * ceil(T Hq / Hkv / 16) times
+ * the table's reach / 128 must stay below 2^31. max_keys: an upper bound of starts[b] + T that
  * the caller knows, or 0; it only chooses how the work is divided. workspace: device memory
  * of spx_paged_attention_workspace_bytes(...) bytes for the same arguments (-1: unsupported
  * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after;
