@@ -20,13 +20,12 @@
 //     The order of the dims in the sum is free: with 4-bit pages a lane takes 32 consecutive
 //     dims of a row, which are 16 bytes and one scale, widened exactly to bf16 by
 //     v_cvt_scalef32_pk_bf16_fp4 (two values and their scale an instruction).
-//   * P V, 4-bit pages: v_mfma_f32_16x16x32_bf16 over the keys of two tiles. Their scores lie
-//     in the lane as the A operand wants them; a lane holds its dims of the eight rows it needs,
-//     and byte permutes pair the keys. P is split into two bf16 parts (2^-16 left over, below
-//     the output's rounding; one part alone would add as much error as that rounding). bf16
-//     pages: v_mfma_f32_16x16x4_f32 as in decode.hip, P as it is and V widened; an infinite
-//     value then stays infinite (a part of P that is 0 would make it NaN; 4-bit values are
-//     never infinite), and the lower rate is enough for four times the bytes.
+//   * P V: v_mfma_f32_16x16x32_bf16 over the keys of two tiles. Their scores lie in the lane as
+//     the A operand wants them; a lane holds its dims of the eight rows it needs, and byte
+//     permutes pair the keys. P is split into two bf16 parts (2^-16 left over, below the
+//     output's rounding; one part alone would add as much error as that rounding). Its sums
+//     are products with ones. Where that makes NaN (infinite values of bf16 pages meet a part
+//     of P that is 0) the wave runs again with P as it is, v_mfma_f32_16x16x4_f32.
 //   * The running maximum is raised, and O scaled, only in steps where it grows.
 #include <algorithm>
 #include <cmath>
@@ -35,18 +34,19 @@
 
 namespace spx {
 
-constexpr int kPaThreads = 256, kPaWaves = kPaThreads / 64;
 constexpr int kPaCols = 16;
 constexpr int kPaMaxGrid = 1024;         // workgroups that share the units (weights in the merge)
 constexpr int kPaCus = 256;
 constexpr int kPaMinUnit = 128;          // keys of the smallest unit
 
-template <int D, bool kFour>
+// W waves per workgroup.
+template <int D, bool kFour, int W>
 struct PagedShape {
-  static constexpr int kTiles = kFour ? 4 : 2;                 // 16-key tiles per wave and unit
-  static constexpr int kUnit = 16 * kTiles * kPaWaves;         // keys of a unit
+  static constexpr int kTiles = kFour && D == 128 && W == 8 ? 4 : 2;    // of a wave and unit
+  static constexpr int kUnit = 16 * kTiles * W;                // keys of a unit
   static_assert(kUnit >= kPaMinUnit, "units are counted in 32 bits");
-  static constexpr int kPerCu = D == 128 ? 3 : 2;              // resident workgroups
+  static constexpr int kPerCu = W == 8 ? 1 : D == 128 && kFour ? 3 : 2;  // resident workgroups
+  static constexpr bool kEarlyKeys = kFour || D == 128;        // registers for them
 };
 
 struct PagedAttnArgs {
@@ -60,8 +60,8 @@ struct PagedAttnArgs {
   int batch, tokens, q_heads, kv_heads, group;
   int cols, col_tiles;                   // tokens x group, tiles of 16 of them
   int grid;                              // workgroups sharing the units; 0: one per stream
-  float scale_log2;                      // >= 0: a negative scale is applied to q's sign
-  uint32_t q_sign;                       // 0 or 0x80008000
+  float scale_log2;                      // > 0: the sign of the scale, or a scale of 0, goes to q
+  uint32_t q_keep, q_flip;               // q & q_keep ^ q_flip
   uint16_t* out;
   float* lse;
   float* part_o;                         // [2 grid][16][D]
@@ -111,8 +111,7 @@ __device__ __forceinline__ int tile_keys(const PagedAttnArgs& a, int start, int 
 
 // Units of a sequence's streams of one KV head.
 template <int kUnit>
-__device__ __forceinline__ int head_units(const PagedAttnArgs& a, int start, int count) {
-  const int live = live_tokens(a, start, count);
+__device__ __forceinline__ int head_units(const PagedAttnArgs& a, int start, int live) {
   int units = 0;
   for (int tile = 0; tile < a.col_tiles; ++tile)
     units += (tile_keys(a, start, live, tile) + kUnit - 1) / kUnit;
@@ -132,12 +131,17 @@ __device__ __forceinline__ int wave_prefix(int x) {
 
 // The units of 64 sequences, one a lane, and their prefix sums.
 struct UnitScan {
-  int units, sum, each;                  // each: of one KV head
+  int start, live, each, units, sum;     // each: of one KV head
   template <int kUnit>
   __device__ __forceinline__ void load(const PagedAttnArgs& a, int b) {
-    each = 0;
-    if (b < a.batch)
-      each = head_units<kUnit>(a, a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
+    start = -1;
+    int count = a.tokens;
+    if (b < a.batch) {
+      start = a.map.starts[b];
+      if (a.map.counts) count = a.map.counts[b];
+    }
+    live = live_tokens(a, start, count);
+    each = head_units<kUnit>(a, start, live);
     units = each * a.kv_heads;
     sum = wave_prefix(units);
   }
@@ -158,10 +162,12 @@ struct Stream {
   int b, kvh, tile, start, live, keys, units;
   int first;                             // of its units
 
-  template <int kUnit>
-  __device__ __forceinline__ void measure(const PagedAttnArgs& a) {
+  __device__ __forceinline__ void lengths(const PagedAttnArgs& a) {
     start = scalar_load(a.map.starts + b);
     live = live_tokens(a, start, a.map.counts ? scalar_load(a.map.counts + b) : a.tokens);
+  }
+  template <int kUnit>
+  __device__ __forceinline__ void measure(const PagedAttnArgs& a) {
     keys = tile_keys(a, start, live, tile);
     units = (keys + kUnit - 1) / kUnit;
   }
@@ -181,6 +187,8 @@ struct Stream {
     b = b0 + l;
     before += __builtin_amdgcn_readlane(scan.sum - scan.units, l);
     const int each = __builtin_amdgcn_readlane(scan.each, l);
+    start = __builtin_amdgcn_readlane(scan.start, l);
+    live = __builtin_amdgcn_readlane(scan.live, l);
     kvh = (u - before) / each;
     first = before + kvh * each;
     for (tile = 0; tile < a.col_tiles; ++tile) {
@@ -200,6 +208,7 @@ struct Stream {
         if (++kvh == a.kv_heads) {
           kvh = 0;
           if (++b == a.batch) return false;
+          lengths(a);
         }
       }
       measure<kUnit>(a);
@@ -210,31 +219,78 @@ struct Stream {
 
 // ------------------------------------------------------------------------- one stream
 
+// The kernel arguments, read afresh: nothing derived from them is held across the loop over a
+// stream's units (held, they cost its scalar registers, and spills to vector lanes).
+__device__ __forceinline__ PagedAttnArgs fresh_args() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto p = (const __attribute__((address_space(4))) PagedAttnArgs*)
+      __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+#else
+  return {};
+#endif
+}
+
+// The start of a tile, opaque: added to a lane's offset it is the scalar base of the load. Seen
+// through, the compiler held lane offset + head in two vector registers for each of the loads.
+__device__ __forceinline__ const uint8_t* tile_base(const uint8_t* p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+s"(p));
+#endif
+  return p;
+}
+
 // Dims of the lane c in a V row and an O register.
 template <int D, bool kFour>
 __device__ __forceinline__ int value_dim(int c, int i) {
   return kFour ? D / 16 * c + i : 128 * (i / 8) + 8 * c + i % 8;
 }
 
+// One KV head of the page arrays.
+template <int D, bool kFour>
+struct HeadPages {
+  static constexpr int kRowBytes = kFour ? D / 2 : 2 * D, kRowScales = D / kPagedGroup;
+  const uint8_t* keys;
+  const uint8_t* values;
+  const uint8_t* key_scales;
+  const uint8_t* value_scales;
+  int page_rows, slot_mask;              // rows from one page to the next
+
+  __device__ __forceinline__ HeadPages(const PagedAttnArgs& a, int kvh) {
+    const int64_t first = (int64_t)kvh << a.map.page_shift;
+    keys = static_cast<const uint8_t*>(a.key_pages) + first * kRowBytes;
+    values = static_cast<const uint8_t*>(a.value_pages) + first * kRowBytes;
+    if constexpr (kFour) {
+      key_scales = a.key_scales + first * kRowScales;
+      value_scales = a.value_scales + first * kRowScales;
+    }
+    page_rows = a.kv_heads << a.map.page_shift;
+    slot_mask = (1 << a.map.page_shift) - 1;
+  }
+  __device__ __forceinline__ int64_t row(int page, int p) const {
+    return (int64_t)page * page_rows + (p & slot_mask);
+  }
+};
+
 template <int D, bool kFour>
 struct KeyTile {                         // a lane's part of 16 rows of K: row c
   u32x4 raw[D / (kFour ? 128 : 32)];
   uint32_t scale[kFour ? D / 128 : 1];
 
-  __device__ __forceinline__ void load(const PagedAttnArgs& a, int64_t row, int c, int g) {
+  __device__ __forceinline__ void load(const HeadPages<D, kFour>& h, int64_t row, int c, int g) {
+    const uint8_t* p = tile_base(h.keys + row * h.kRowBytes);
     if constexpr (kFour) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.key_pages) + row * (D / 2);
-      const uint8_t* s = a.key_scales + row * (D / kPagedGroup);
+      const uint8_t* s = tile_base(h.key_scales + row * h.kRowScales);
 #pragma unroll
       for (int x = 0; x < D / 128; ++x) {
         raw[x] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * (D / 2) + 64 * x + 16 * g));
         scale[x] = s[(uint32_t)(c * (D / kPagedGroup) + 4 * x + g)];
       }
     } else {
-      const uint16_t* p = static_cast<const uint16_t*>(a.key_pages) + row * D;
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk)
-        raw[kk] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * D + 32 * kk + 8 * g));
+        raw[kk] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * 2 * D + 64 * kk + 16 * g));
     }
   }
   // Eight dims of the row as A operand of product kk.
@@ -253,9 +309,10 @@ struct ValueRow {                        // a lane's dims of one row of V
   uint32_t raw[kFour ? D / 128 : D / 32];
   uint32_t scale;
 
-  __device__ __forceinline__ void load(const PagedAttnArgs& a, int64_t row, int at, int c) {
+  // Row `at` of the tile whose values start at p and whose scales start at s.
+  __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* s, int at, int c) {
+    constexpr int kRowScales = D / kPagedGroup;
     if constexpr (kFour) {
-      const uint8_t* p = static_cast<const uint8_t*>(a.value_pages) + row * (D / 2);
       if constexpr (D == 128) {
         raw[0] = *reinterpret_cast<const uint32_t*>(p + (uint32_t)(at * 64 + 4 * c));
       } else {
@@ -263,13 +320,12 @@ struct ValueRow {                        // a lane's dims of one row of V
         raw[0] = w[0];
         raw[1] = w[1];
       }
-      scale = a.value_scales[row * (D / kPagedGroup) +
-                             (uint32_t)(at * (D / kPagedGroup) + c * (D / 16) / kPagedGroup)];
+      scale = s[(uint32_t)(at * kRowScales + c * (D / 16) / kPagedGroup)];
     } else {
-      const uint16_t* p = static_cast<const uint16_t*>(a.value_pages) + row * D;
 #pragma unroll
       for (int x = 0; x < D / 128; ++x) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(p + (uint32_t)(at * D + 128 * x + 8 * c));
+        const u32x4 w =
+            *reinterpret_cast<const u32x4*>(p + (uint32_t)(at * 2 * D + 256 * x + 16 * c));
 #pragma unroll
         for (int e = 0; e < 4; ++e) raw[4 * x + e] = w[e];
       }
@@ -295,55 +351,108 @@ struct ValueRow {                        // a lane's dims of one row of V
   }
 };
 
-template <int D, bool kFour>
-struct Accumulator {
-  using Shape = PagedShape<D, kFour>;
-  static constexpr int T = Shape::kTiles, KK = D / 32, N = D / 16;
-  f32x4 o[N];                            // [query row 4 g + r][value_dim(c, i)]
-  float m, l;                            // of column c, m unscaled; l over this lane's keys
+// What a wave needs of its stream in the loop over the units.
+struct Limits {
+  int b, keys;                           // the sequence, keys that any column sees
+  int first;                             // the last key that the tile's first column sees
+  int column;                            // and the one that column c sees
+};
 
-  __device__ __forceinline__ void clear() {
+// A wave's tiles of a stream: page ids, keys and values of one unit, O and the softmax state.
+template <int D, bool kFour, int W>
+struct Wave {
+  using Shape = PagedShape<D, kFour, W>;
+  using Pages = HeadPages<D, kFour>;
+  static constexpr int T = Shape::kTiles, KK = D / 32, N = D / 16;
+  KeyTile<D, kFour> key[T];
+  ValueRow<D, kFour> value[T][4];
+  f32x4 o[N];                            // [query row 4 g + r][value_dim(c, i)]
+  f32x4 l;                               // sums of P, query row 4 g + r
+  float m;                               // maximum of column c, unscaled
+  int ids, id_base;                      // lane i: page of tile i % T in unit id_base + i / T
+  uint32_t bad;                          // tiles without a place
+
+  __device__ __forceinline__ void load_ids(const Limits& s, int j, int w, int lane) {
+    const PagedAttnArgs a = fresh_args();
+    id_base = j;
+    const int p = (j + lane / T) * Shape::kUnit + (w * T + lane % T) * 16;
+    ids = a.map.page(s.b, min(p, s.keys - 1));
+  }
+  __device__ __forceinline__ int page(int j, int t) const {
+    return __builtin_amdgcn_readlane(ids, (j - id_base) * T + t);
+  }
+  // Tiles without a place read page 0.
+  __device__ __forceinline__ void load_keys(const Pages& h, int j, int key0, int c, int g) {
+    bad = 0;
 #pragma unroll
-    for (auto& x : o) x = f32x4{};
-    m = -INFINITY;
-    l = 0.0f;
+    for (int t = 0; t < T; ++t) {
+      const int id = page(j, t);
+      bad |= (id < 0 ? 1u : 0u) << t;
+      key[t].load(h, h.row(max(id, 0), key0 + 16 * t), c, g);
+    }
+  }
+  __device__ __forceinline__ void load_values(const Pages& h, int j, int key0, int c, int g) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int64_t row = h.row(max(page(j, t), 0), key0 + 16 * t);
+      const uint8_t* p = tile_base(h.values + row * h.kRowBytes);
+      const uint8_t* s = kFour ? tile_base(h.value_scales + row * h.kRowScales) : nullptr;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) value[t][r].load(p, s, 4 * g + r, c);
+    }
   }
 
-  // One wave's tiles from key0 on. limit: the last key that column c sees, first_limit: that of
-  // the tile's first column.
-  __device__ __forceinline__ void step(const PagedAttnArgs& a, const Stream& s, const u32x4 (&q)[KK],
-                                       int ids, int id0, int key0, int limit, int first_limit,
-                                       int c, int g) {
-    KeyTile<D, kFour> key[T];
-    ValueRow<D, kFour> value[T][4];
-    bool placed = true;
-    uint32_t bad = 0;
+  // Units j .. end - 1. The next unit's keys are fetched as soon as the scores are formed, its
+  // values after the products. kWide: P V in fp32 products.
+  template <bool kWide>
+  __device__ __forceinline__ void run(const Pages& h, const Limits& s, const u32x4 (&q)[KK],
+                                      float scale, int j, int end, int w, int lane, int c, int g) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int id = __builtin_amdgcn_readlane(ids, id0 + t);
-      const int64_t row = a.map.row(max(id, 0), s.kvh, key0 + 16 * t);
-      bad |= (id < 0 ? 1u : 0u) << t;
-      key[t].load(a, row, c, g);
+    for (auto& x : o) x = f32x4{};
+    l = f32x4{};
+    m = -INFINITY;
+    const int offset = w * T * 16;       // the wave's first key in a unit
+    end = min(end, (s.keys - offset + Shape::kUnit - 1) / Shape::kUnit);
+    if (j >= end) return;
+    load_ids(s, j, w, lane);
+    load_keys(h, j, j * Shape::kUnit + offset, c, g);
+    load_values(h, j, j * Shape::kUnit + offset, c, g);
+    for (;;) {
+      const int key0 = j * Shape::kUnit + offset;
+      const bool more = j + 1 < end;
+      const uint32_t unplaced = bad;
+      f32x4 x[T];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < T; ++t) x[t] = f32x4{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+        for (int t = 0; t < T; ++t) x[t] = mfma16(key[t].operand(kk), q[kk], x[t]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (Shape::kEarlyKeys && more) {
+        if (j + 1 - id_base >= kWave / T) load_ids(s, j + 1, w, lane);
+        load_keys(h, j + 1, key0 + Shape::kUnit, c, g);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      softmax_products<kWide>(h, s, x, scale, key0, unplaced, c, g);
+      if (!more) return;
+      ++j;
+      __builtin_amdgcn_sched_barrier(0);
+      if (!Shape::kEarlyKeys) {
+        if (j - id_base >= kWave / T) load_ids(s, j, w, lane);
+        load_keys(h, j, key0 + Shape::kUnit, c, g);
+      }
+      load_values(h, j, key0 + Shape::kUnit, c, g);
     }
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int64_t row = a.map.row(max(__builtin_amdgcn_readlane(ids, id0 + t), 0), s.kvh,
-                                    key0 + 16 * t);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) value[t][r].load(a, row, 4 * g + r, c);
-    }
-    placed = bad == 0;
-    __builtin_amdgcn_sched_barrier(0);   // every load of the step is issued by now
-    f32x4 x[T];
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-      x[t] = f32x4{};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) x[t] = mfma16(key[t].operand(kk), q[kk], x[t]);
-    }
-    const bool masked = !placed || key0 + 16 * T - 1 > first_limit;
+  }
+
+  template <bool kWide>
+  __device__ __forceinline__ void softmax_products(const Pages& h, const Limits& s, f32x4 (&x)[T],
+                                                   float scale, int key0, uint32_t unplaced, int c,
+                                                   int g) {
     bool split = false;                  // V rows of some columns only, not finite: left out
-    if (masked) {
+    if (unplaced != 0 || key0 + 16 * T - 1 > s.first) {
       // scores of keys that a column does not see are -inf; rows that no column sees are 0, so
       // that what lies behind the last token does not meet a probability of 0
 #pragma unroll
@@ -351,11 +460,11 @@ struct Accumulator {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int p = key0 + 16 * t + 4 * g + r;
-          const bool here = !(bad >> t & 1);
-          if (!here || p > limit) x[t][r] = -INFINITY;
+          const bool here = !(unplaced >> t & 1);
+          if (!here || p > s.column) x[t][r] = -INFINITY;
           if (!here || p >= s.keys) {
             value[t][r].clear();
-          } else if (p > first_limit && !value[t][r].finite()) {
+          } else if (p > s.first && !value[t][r].finite()) {
             split = true;
             value[t][r].clear();
           }
@@ -370,27 +479,35 @@ struct Accumulator {
     mx = fmaxf(mx, __shfl_xor(mx, 32));
     if (__any(mx > m)) {
       const float m_new = fmaxf(m, mx);
-      const float corr = m == -INFINITY ? 0.0f : exp2_fast((m - m_new) * a.scale_log2);
-      l *= corr;
+      const float corr = m == -INFINITY ? 0.0f : exp2_fast((m - m_new) * scale);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float cr = __shfl(corr, 4 * g + r);
+        l[r] *= cr;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i][r] *= cr;
       }
       m = m_new;
     }
-    const float shift = m == -INFINITY ? 0.0f : m * a.scale_log2;
+    const float shift = m == -INFINITY ? 0.0f : m * scale;
 #pragma unroll
     for (int t = 0; t < T; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float p = exp2_fast(__builtin_fmaf(x[t][r], a.scale_log2, -shift));
-        if (masked && x[t][r] == -INFINITY) p = 0.0f;      // also with a scale of 0
-        x[t][r] = p;
-        l += p;
-      }
-    if constexpr (kFour) {
+      for (int r = 0; r < 4; ++r) x[t][r] = exp2_fast(__builtin_fmaf(x[t][r], scale, -shift));
+    if constexpr (kWide) {
+#pragma unroll
+      for (int t = 0; t < T; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          l = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], 1.0f, l, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const uint32_t v2 = value[t][r].raw[i / 2];
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_lo(v2), o[i], 0, 0, 0);
+            o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_hi(v2), o[i + 1], 0, 0, 0);
+          }
+        }
+    } else {
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
         u32x4 hi, lo;
@@ -400,6 +517,9 @@ struct Accumulator {
           hi[e] = pack_bf16x2(u, w);
           lo[e] = pack_bf16x2(u - bf16_lo(hi[e]), w - bf16_hi(hi[e]));
         }
+        const uint32_t ones = 0x3f803f80u;
+        l = mfma16(hi, u32x4{ones, ones, ones, ones}, l);
+        l = mfma16(lo, u32x4{ones, ones, ones, ones}, l);
 #pragma unroll
         for (int y = 0; y < N / 8; ++y) {
           u32x4 row[8];
@@ -417,32 +537,23 @@ struct Accumulator {
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int t = 0; t < T; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int i = 0; i < N; i += 2) {
-            const uint32_t v2 = value[t][r].raw[i / 2];
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_lo(v2), o[i], 0, 0, 0);
-            o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_hi(v2), o[i + 1], 0, 0, 0);
-          }
     }
-    if (__any(split)) add_split_rows(a, s, x, key0, limit, first_limit, c, g);
+    if (__any(split)) add_split_rows(h, s, x, key0, c, g);
   }
 
-  // The V rows that step() left out, one after the other: only into the columns that see them.
-  __device__ __forceinline__ void add_split_rows(const PagedAttnArgs& a, const Stream& s,
-                                                 const f32x4 (&p)[T], int key0, int limit,
-                                                 int first_limit, int c, int g) {
+  // The V rows that were left out, one after the other: only into the columns that see them.
+  __device__ __forceinline__ void add_split_rows(const Pages& h, const Limits& s,
+                                                 const f32x4 (&p)[T], int key0, int c, int g) {
+    const PagedAttnArgs a = fresh_args();
     const int last = min(key0 + 16 * T, s.keys);
 #pragma unroll 1
-    for (int at = max(key0, first_limit + 1); at < last; ++at) {
+    for (int at = max(key0, s.first + 1); at < last; ++at) {
       const int id = a.map.page(s.b, at);
       if (id < 0) continue;
       ValueRow<D, kFour> v;
-      v.load(a, a.map.row(id, s.kvh, at), 0, c);
+      const int64_t row = h.row(id, at);
+      v.load(h.values + row * h.kRowBytes, kFour ? h.value_scales + row * h.kRowScales : nullptr, 0,
+             c);
       const bool left_out = !v.finite();
       float mine = 0.0f;                 // the probability of key `at`, where this lane has it
 #pragma unroll
@@ -452,7 +563,7 @@ struct Accumulator {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float prob = __shfl(mine, 16 * (at / 4 % 4) + 4 * g + r);
-        const int seen = __shfl(limit, 4 * g + r);
+        const int seen = __shfl(s.column, 4 * g + r);
         const bool sees = left_out && at <= seen;
 #pragma unroll
         for (int y = 0; y < N / 8; ++y) {
@@ -466,88 +577,101 @@ struct Accumulator {
       }
     }
   }
+
+  __device__ __forceinline__ bool any_nan() const {
+    float sum = 0.0f;
+#pragma unroll
+    for (const auto& x : o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum = __builtin_fmaf(x[r], 0.0f, sum);
+    return __any(sum != sum);
+  }
 };
 
 // grid > 0: workgroup w takes its run of all units; grid == 0: workgroup w is stream w.
-template <int D, bool kFour>
-__global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void paged_attn_kernel(
-    PagedAttnArgs a) {
-  using Shape = PagedShape<D, kFour>;
-  constexpr int T = Shape::kTiles, KK = D / 32, kIdUnits = kWave / T;
-  __shared__ float part_m[kPaWaves][kPaCols], part_l[kPaWaves][kPaCols];
-  __shared__ __align__(16) float part_o[kPaWaves][kPaCols][D];
+template <int D, bool kFour, int W>
+__global__ __launch_bounds__(64 * W, (PagedShape<D, kFour, W>::kPerCu * W / 4)) void
+paged_attn_kernel(PagedAttnArgs args) {
+  using Shape = PagedShape<D, kFour, W>;
+  constexpr int KK = D / 32;
+  __shared__ float part_m[W][kPaCols], part_l[W][kPaCols];
+  __shared__ __align__(16) float part_o[W][kPaCols][D];
   const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
 
   Stream s;
   Run run(0, 1);
   int u, end;
-  if (a.grid > 0) {
+  if (args.grid > 0) {
     UnitScan scan;
-    scan.load<Shape::kUnit>(a, lane);
+    scan.load<Shape::kUnit>(args, lane);
     int total = scan.total();
-    for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
+    for (int b0 = kWave; b0 < args.batch; b0 += kWave) {
       UnitScan more;
-      more.load<Shape::kUnit>(a, b0 + lane);
+      more.load<Shape::kUnit>(args, b0 + lane);
       total += more.total();
     }
-    run = Run(total, a.grid);
+    run = Run(total, args.grid);
     u = run.begin(blockIdx.x);
     end = run.begin(blockIdx.x + 1);
-    if (u >= end || !s.find<Shape::kUnit>(a, lane, scan, u)) return;
+    if (u >= end || !s.find<Shape::kUnit>(args, lane, scan, u)) return;
   } else {
     const int stream = blockIdx.x;
-    s.tile = stream % a.col_tiles;
-    s.kvh = stream / a.col_tiles % a.kv_heads;
-    s.b = stream / a.col_tiles / a.kv_heads;
+    s.tile = stream % args.col_tiles;
+    s.kvh = stream / args.col_tiles % args.kv_heads;
+    s.b = stream / args.col_tiles / args.kv_heads;
     s.first = u = 0;
-    s.measure<Shape::kUnit>(a);
+    s.lengths(args);
+    s.measure<Shape::kUnit>(args);
     end = s.units;
   }
   const int begin = u;
 
   for (;;) {
-    const int cols = min(kPaCols, a.cols - s.tile * kPaCols);
-    const int n = s.tile * kPaCols + min(c, cols - 1);    // columns past the last repeat it
-    const int token = a.tokens == 1 ? 0 : n / a.group;
-    const int head = s.kvh * a.group + n - token * a.group;
-    const int limit = s.start + token;
-    const int first_limit = s.start + tile_first(a, s.tile);
-    u32x4 q[KK];
-    const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      q[kk] = *reinterpret_cast<const u32x4*>(qr + KeyTile<D, kFour>::dim(kk, g));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) q[kk][e] ^= a.q_sign;
-    }
-    Accumulator<D, kFour> acc;
-    acc.clear();
     const int j0 = u - s.first, j1 = min(end, s.first + s.units) - s.first;
-    for (int jb = j0; jb < j1; jb += kIdUnits) {
-      // page ids of the wave's tiles in units jb .. jb + kIdUnits - 1
-      const int p = (jb + lane / T) * Shape::kUnit + (w * T + lane % T) * 16;
-      const int ids = a.map.page(s.b, min(p, s.keys - 1));
-      const int je = min(j1, jb + kIdUnits);
-      for (int j = jb; j < je; ++j) {
-        const int key0 = j * Shape::kUnit + w * T * 16;
-        if (key0 >= s.keys) break;
-        acc.step(a, s, q, ids, (j - jb) * T, key0, limit, first_limit, c, g);
+    int cols;
+    {
+      const PagedAttnArgs a = fresh_args();
+      cols = min(kPaCols, a.cols - s.tile * kPaCols);
+      const int n = s.tile * kPaCols + min(c, cols - 1);    // columns past the last repeat it
+      const int token = a.tokens == 1 ? 0 : n / a.group;
+      const int head = s.kvh * a.group + n - token * a.group;
+      const Limits limits{s.b, s.keys, s.start + tile_first(a, s.tile), s.start + token};
+      u32x4 q[KK];
+      const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        q[kk] = *reinterpret_cast<const u32x4*>(qr + KeyTile<D, kFour>::dim(kk, g));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[kk][e] = (q[kk][e] & a.q_keep) ^ a.q_flip;
+      }
+      const HeadPages<D, kFour> pages(a, s.kvh);
+      Wave<D, kFour, W> acc;
+      acc.template run<false>(pages, limits, q, a.scale_log2, j0, j1, w, lane, c, g);
+      if (g == 0) part_m[w][c] = acc.m == -INFINITY ? -INFINITY : acc.m * a.scale_log2;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (c == 0) part_l[w][4 * g + r] = acc.l[r];
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 4)
+          *reinterpret_cast<f32x4*>(&part_o[w][4 * g + r][value_dim<D, kFour>(c, i)]) =
+              f32x4{acc.o[i][r], acc.o[i + 1][r], acc.o[i + 2][r], acc.o[i + 3][r]};
+      }
+      // an infinite value and a part of P that is 0 make NaN: those again, with P as it is
+      if constexpr (!kFour) {
+        if (acc.any_nan()) {
+          acc.template run<true>(pages, limits, q, a.scale_log2, j0, j1, w, lane, c, g);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              float& held = part_o[w][4 * g + r][value_dim<D, kFour>(c, i)];
+              if (held != held) held = acc.o[i][r];
+            }
+        }
       }
     }
-    float l = acc.l;
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (g == 0) {
-      part_m[w][c] = acc.m == -INFINITY ? -INFINITY : acc.m * a.scale_log2;
-      part_l[w][c] = l;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int i = 0; i < Accumulator<D, kFour>::N; i += 4)
-        *reinterpret_cast<f32x4*>(&part_o[w][4 * g + r][value_dim<D, kFour>(c, i)]) =
-            f32x4{acc.o[i][r], acc.o[i + 1][r], acc.o[i + 2][r], acc.o[i + 3][r]};
+    const PagedAttnArgs a = fresh_args();
     block_sync();
     const bool whole = j0 == 0 && j1 == s.units;
     const int slot = 2 * blockIdx.x + (u == begin ? 0 : 1);
@@ -556,15 +680,15 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
       a.parts[(s.b * a.kv_heads + s.kvh) * a.col_tiles + s.tile] =
           u32x2{(uint32_t)slot, (uint32_t)parts};
     }
-    for (int e = threadIdx.x; e < cols * (D / 4); e += kPaThreads) {
+    for (int e = threadIdx.x; e < cols * (D / 4); e += 64 * W) {
       const int col = e / (D / 4), d = (e % (D / 4)) * 4;
       float top = part_m[0][col];
 #pragma unroll
-      for (int x = 1; x < kPaWaves; ++x) top = fmaxf(top, part_m[x][col]);
+      for (int x = 1; x < W; ++x) top = fmaxf(top, part_m[x][col]);
       float sum = 0.0f;
       f32x4 v{};
 #pragma unroll
-      for (int x = 0; x < kPaWaves; ++x) {
+      for (int x = 0; x < W; ++x) {
         const float wt = part_weight(part_m[x][col], top);
         const f32x4 po = *reinterpret_cast<const f32x4*>(&part_o[x][col][d]);
         sum += wt * part_l[x][col];
@@ -604,13 +728,13 @@ __global__ __launch_bounds__(kPaThreads, (PagedShape<D, kFour>::kPerCu)) void pa
 // Join of the partial results of a row: one workgroup per (row, 64 dims), the partials in turn
 // over 16 groups of threads. Rows of one workgroup are written already; rows of streams
 // without keys are written here.
-constexpr int kPaMergeDims = 64;
+constexpr int kPaMergeDims = 64, kPaMergeThreads = 256;
 
 template <int D>
-__global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a) {
-  constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaThreads / kLanes;
+__global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnArgs a) {
+  constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaMergeThreads / kLanes;
   __shared__ float weight[kPaMaxGrid];
-  __shared__ float red[2][kPaWaves];
+  __shared__ float red[2][kPaMergeThreads / 64];
   __shared__ __align__(16) float acc_s[kGroups][kPaMergeDims];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -633,7 +757,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a
   // the stream is the first one of every workgroup but perhaps the first
   auto slot = [&](int x) { return x == 0 ? slot0 : (slot0 & ~1) + 2 * x; };
   float top = -INFINITY;
-  for (int x = tid; x < parts; x += kPaThreads)
+  for (int x = tid; x < parts; x += kPaMergeThreads)
     top = fmaxf(top, a.part_ml[(slot(x) * kPaCols + col) * 2]);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -641,7 +765,7 @@ __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a
   block_sync();
   top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float sum = 0.0f;
-  for (int x = tid; x < parts; x += kPaThreads) {
+  for (int x = tid; x < parts; x += kPaMergeThreads) {
     const float* ml = a.part_ml + (slot(x) * kPaCols + col) * 2;
     const float wt = part_weight(ml[0], top);
     weight[x] = wt;
@@ -676,14 +800,18 @@ __global__ __launch_bounds__(kPaThreads) void paged_merge_kernel(PagedAttnArgs a
 
 // ------------------------------------------------------------------------------- host
 
-// Workgroups that share the units, or 0: one per stream and no second launch, where a stream
-// has at most two units (the second launch costs more than it saves).
+// How a launch is divided: workgroups of `waves` waves, `grid` of them sharing the units, or
+// (grid 0) one per stream and no second launch.
+struct PagedPlan {
+  int grid, waves;
+};
+
 template <int D, bool kFour>
-static int paged_grid(int64_t keys, int64_t streams) {
-  using Shape = PagedShape<D, kFour>;
+static PagedPlan paged_plan(int64_t keys, int64_t streams) {
+  if (keys <= 4 * PagedShape<D, kFour, 8>::kUnit) return {0, 8};
+  using Shape = PagedShape<D, kFour, 4>;
   const int64_t units = (keys + Shape::kUnit - 1) / Shape::kUnit;
-  if (units <= 2) return 0;
-  return (int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units);
+  return {(int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units), 4};
 }
 
 struct PagedSizes {
@@ -705,25 +833,29 @@ static bool paged_sizes(const spx_paged_cache& z, int q_heads, int max_keys, Pag
   return true;
 }
 
-static int paged_grid_of(const PagedSizes& z, int head_dim, bool four) {
+static PagedPlan paged_plan_of(const PagedSizes& z, int head_dim, bool four) {
   if (head_dim == 128)
-    return four ? paged_grid<128, true>(z.keys, z.streams) : paged_grid<128, false>(z.keys, z.streams);
-  return four ? paged_grid<256, true>(z.keys, z.streams) : paged_grid<256, false>(z.keys, z.streams);
+    return four ? paged_plan<128, true>(z.keys, z.streams) : paged_plan<128, false>(z.keys, z.streams);
+  return four ? paged_plan<256, true>(z.keys, z.streams) : paged_plan<256, false>(z.keys, z.streams);
 }
 
 template <int D, bool kFour>
-static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, hipStream_t st) {
-  if (a.grid > 0) {
-    SPX_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
-                SPX_EINVAL, "paged_attention: workspace null or not 16-byte aligned");
-    a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
-    a.parts = reinterpret_cast<u32x2*>(a.part_ml + (int64_t)2 * a.grid * kPaCols * 2);
+static int launch_paged(PagedAttnArgs a, const PagedSizes& z, int waves, void* workspace,
+                        hipStream_t st) {
+  if (a.grid == 0) {
+    const unsigned streams = (unsigned)z.streams;
+    if (waves == 8) paged_attn_kernel<D, kFour, 8><<<streams, 512, 0, st>>>(a);
+    else paged_attn_kernel<D, kFour, 4><<<streams, 256, 0, st>>>(a);
+    return launch_status("paged_attention");
   }
-  paged_attn_kernel<D, kFour>
-      <<<(unsigned)(a.grid > 0 ? a.grid : z.streams), kPaThreads, 0, st>>>(a);
-  if (a.grid > 0)
-    paged_merge_kernel<D><<<dim3((unsigned)z.rows, D / kPaMergeDims), kPaThreads, 0, st>>>(a);
+  SPX_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, SPX_EINVAL,
+              "paged_attention: workspace null or not 16-byte aligned");
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
+  a.parts = reinterpret_cast<u32x2*>(a.part_ml + (int64_t)2 * a.grid * kPaCols * 2);
+  paged_attn_kernel<D, kFour, 4><<<(unsigned)a.grid, 256, 0, st>>>(a);
+  paged_merge_kernel<D>
+      <<<dim3((unsigned)z.rows, D / kPaMergeDims), kPaMergeThreads, 0, st>>>(a);
   return launch_status("paged_attention");
 }
 
@@ -737,7 +869,7 @@ extern "C" int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* ca
   if (cache == nullptr || !paged_sizes(*cache, q_heads, max_keys, z) ||
       (cache->head_dim != 128 && cache->head_dim != 256))
     return -1;
-  const int grid = paged_grid_of(z, cache->head_dim, cache->key_scales != nullptr);
+  const int grid = paged_plan_of(z, cache->head_dim, cache->key_scales != nullptr).grid;
   return grid == 0 ? 0 : (int64_t)2 * grid * kPaCols * (cache->head_dim + 2) * 4 + z.streams * 8;
 }
 
@@ -766,15 +898,17 @@ extern "C" int spx_paged_attention(const spx_paged_cache* cache, const void* q,
   a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.group = q_heads / cache->kv_heads;
   a.cols = cache->tokens * a.group;
   a.col_tiles = (a.cols + kPaCols - 1) / kPaCols;
-  a.grid = paged_grid_of(z, cache->head_dim, four);
-  a.scale_log2 = (float)(std::abs((double)scale) * 1.4426950408889634);
-  a.q_sign = scale < 0 ? 0x80008000u : 0;
+  const PagedPlan plan = paged_plan_of(z, cache->head_dim, four);
+  a.grid = plan.grid;
+  a.scale_log2 = scale == 0 ? 1.0f : (float)(std::abs((double)scale) * 1.4426950408889634);
+  a.q_keep = scale == 0 ? 0 : 0xffffffffu;
+  a.q_flip = scale < 0 ? 0x80008000u : 0;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 128)
-    return four ? launch_paged<128, true>(a, z, workspace, st)
-                : launch_paged<128, false>(a, z, workspace, st);
-  return four ? launch_paged<256, true>(a, z, workspace, st)
-              : launch_paged<256, false>(a, z, workspace, st);
+    return four ? launch_paged<128, true>(a, z, plan.waves, workspace, st)
+                : launch_paged<128, false>(a, z, plan.waves, workspace, st);
+  return four ? launch_paged<256, true>(a, z, plan.waves, workspace, st)
+              : launch_paged<256, false>(a, z, plan.waves, workspace, st);
 }
