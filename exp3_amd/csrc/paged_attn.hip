@@ -42,10 +42,10 @@ constexpr int kPaMinUnit = 128;          // keys of the smallest unit
 // W waves per workgroup.
 template <int D, bool kFour, int W>
 struct PagedShape {
-  static constexpr int kTiles = kFour && D == 128 && W == 8 ? 4 : 2;    // of a wave and unit
+  static constexpr int kTiles = kFour && D == 128 ? 4 : 2;     // of a wave and unit
   static constexpr int kUnit = 16 * kTiles * W;                // keys of a unit
   static_assert(kUnit >= kPaMinUnit, "units are counted in 32 bits");
-  static constexpr int kPerCu = W == 8 ? 1 : D == 128 && kFour ? 3 : 2;  // resident workgroups
+  static constexpr int kPerCu = W == 8 ? 1 : 2;                // resident workgroups
   static constexpr bool kEarlyKeys = kFour || D == 128;        // registers for them
 };
 
@@ -232,13 +232,41 @@ __device__ __forceinline__ PagedAttnArgs fresh_args() {
 #endif
 }
 
+// Page memory as global memory: an opaque pointer of no known address space would be read by
+// flat loads, which are waited for together with the LDS.
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+
+template <typename T>
+__device__ __forceinline__ T global_load(GlobalBytes p, uint32_t offset) {
+  return *(const __attribute__((address_space(1))) T*)(p + offset);
+}
+
 // The start of a tile, opaque: added to a lane's offset it is the scalar base of the load. Seen
 // through, the compiler held lane offset + head in two vector registers for each of the loads.
-__device__ __forceinline__ const uint8_t* tile_base(const uint8_t* p) {
+__device__ __forceinline__ GlobalBytes tile_base(GlobalBytes p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("" : "+s"(p));
 #endif
   return p;
+}
+
+// Byte x of four scale bytes as the scale operand of a widening conversion, which looks at bits
+// 23 to 30 alone.
+__device__ __forceinline__ float scale_of(uint32_t bytes, int x) {
+  return __uint_as_float(__builtin_amdgcn_alignbit(bytes, bytes, 8 * x + 9));
+}
+
+__device__ __forceinline__ uint32_t opaque_bits(uint32_t x) { return (uint32_t)opaque((int)x); }
+
+// The lane, recomputed where it is used: what rare paths derive from it is not held meanwhile.
+__device__ __forceinline__ int thread_lane() { return opaque((int)threadIdx.x) & 63; }
+
+// Maximum over the lanes c, c + 16, c + 32, c + 48.
+__device__ __forceinline__ float max_over_rows(float x) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+  const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
 // Dims of the lane c in a V row and an O register.
@@ -251,19 +279,16 @@ __device__ __forceinline__ int value_dim(int c, int i) {
 template <int D, bool kFour>
 struct HeadPages {
   static constexpr int kRowBytes = kFour ? D / 2 : 2 * D, kRowScales = D / kPagedGroup;
-  const uint8_t* keys;
-  const uint8_t* values;
-  const uint8_t* key_scales;
-  const uint8_t* value_scales;
+  GlobalBytes keys, values, key_scales, value_scales;
   int page_rows, slot_mask;              // rows from one page to the next
 
   __device__ __forceinline__ HeadPages(const PagedAttnArgs& a, int kvh) {
     const int64_t first = (int64_t)kvh << a.map.page_shift;
-    keys = static_cast<const uint8_t*>(a.key_pages) + first * kRowBytes;
-    values = static_cast<const uint8_t*>(a.value_pages) + first * kRowBytes;
+    keys = (GlobalBytes)a.key_pages + first * kRowBytes;
+    values = (GlobalBytes)a.value_pages + first * kRowBytes;
     if constexpr (kFour) {
-      key_scales = a.key_scales + first * kRowScales;
-      value_scales = a.value_scales + first * kRowScales;
+      key_scales = (GlobalBytes)a.key_scales + first * kRowScales;
+      value_scales = (GlobalBytes)a.value_scales + first * kRowScales;
     }
     page_rows = a.kv_heads << a.map.page_shift;
     slot_mask = (1 << a.map.page_shift) - 1;
@@ -276,27 +301,32 @@ struct HeadPages {
 template <int D, bool kFour>
 struct KeyTile {                         // a lane's part of 16 rows of K: row c
   u32x4 raw[D / (kFour ? 128 : 32)];
-  uint32_t scale[kFour ? D / 128 : 1];
+  uint32_t scale[kFour ? D / 128 : 1];   // four scale bytes of the row; the lane's is byte g
 
   __device__ __forceinline__ void load(const HeadPages<D, kFour>& h, int64_t row, int c, int g) {
-    const uint8_t* p = tile_base(h.keys + row * h.kRowBytes);
+    const GlobalBytes p = tile_base(h.keys + row * h.kRowBytes);
     if constexpr (kFour) {
-      const uint8_t* s = tile_base(h.key_scales + row * h.kRowScales);
+      const GlobalBytes s = tile_base(h.key_scales + row * h.kRowScales);
 #pragma unroll
-      for (int x = 0; x < D / 128; ++x) {
-        raw[x] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * (D / 2) + 64 * x + 16 * g));
-        scale[x] = s[(uint32_t)(c * (D / kPagedGroup) + 4 * x + g)];
+      for (int x = 0; x < D / 128; ++x)
+        raw[x] = global_load<u32x4>(p, c * (D / 2) + 64 * x + 16 * g);
+      if constexpr (D == 128) {
+        scale[0] = global_load<uint32_t>(s, c * 4);
+      } else {
+        const u32x2 w = global_load<u32x2>(s, c * 8);
+        scale[0] = w[0];
+        scale[1] = w[1];
       }
     } else {
 #pragma unroll
       for (int kk = 0; kk < D / 32; ++kk)
-        raw[kk] = *reinterpret_cast<const u32x4*>(p + (uint32_t)(c * 2 * D + 64 * kk + 16 * g));
+        raw[kk] = global_load<u32x4>(p, c * 2 * D + 64 * kk + 16 * g);
     }
   }
   // Eight dims of the row as A operand of product kk.
-  __device__ __forceinline__ u32x4 operand(int kk) const {
+  __device__ __forceinline__ u32x4 operand(int kk, int g) const {
     if constexpr (!kFour) return raw[kk];
-    else return widen8(raw[kk / 4][kk % 4], __uint_as_float(scale[kk / 4] << 23));
+    else return widen8(raw[kk / 4][kk % 4], scale_of(scale[kk / 4], g));
   }
   // Dim of the operand's first element.
   static __device__ __forceinline__ int dim(int kk, int g) {
@@ -305,49 +335,71 @@ struct KeyTile {                         // a lane's part of 16 rows of K: row c
 };
 
 template <int D, bool kFour>
-struct ValueRow {                        // a lane's dims of one row of V
-  uint32_t raw[kFour ? D / 128 : D / 32];
-  uint32_t scale;
+struct ValueTile {                       // a lane's dims of four rows of V: 4 g + r
+  static constexpr int kWords = kFour ? D / 128 : D / 32;
+  uint32_t raw[4][kWords];
+  uint32_t scale[kFour ? 4 : 1];         // four scale bytes of each row
 
-  // Row `at` of the tile whose values start at p and whose scales start at s.
-  __device__ __forceinline__ void load(const uint8_t* p, const uint8_t* s, int at, int c) {
-    constexpr int kRowScales = D / kPagedGroup;
+  // The lane's byte of them.
+  static __device__ __forceinline__ int scale_byte(int c) { return c * (D / 16) / kPagedGroup % 4; }
+
+  __device__ __forceinline__ void load_row(GlobalBytes p, GlobalBytes s, int r, int at, int c) {
     if constexpr (kFour) {
       if constexpr (D == 128) {
-        raw[0] = *reinterpret_cast<const uint32_t*>(p + (uint32_t)(at * 64 + 4 * c));
+        raw[r][0] = global_load<uint32_t>(p, at * 64 + 4 * c);
       } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(p + (uint32_t)(at * 128 + 8 * c));
-        raw[0] = w[0];
-        raw[1] = w[1];
+        const u32x2 w = global_load<u32x2>(p, at * 128 + 8 * c);
+        raw[r][0] = w[0];
+        raw[r][1] = w[1];
+        scale[r] = global_load<uint32_t>(s, at * 8 + 4 * (c / 8));
       }
-      scale = s[(uint32_t)(at * kRowScales + c * (D / 16) / kPagedGroup)];
     } else {
 #pragma unroll
       for (int x = 0; x < D / 128; ++x) {
-        const u32x4 w =
-            *reinterpret_cast<const u32x4*>(p + (uint32_t)(at * 2 * D + 256 * x + 16 * c));
+        const u32x4 w = global_load<u32x4>(p, at * 2 * D + 256 * x + 16 * c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) raw[4 * x + e] = w[e];
+        for (int e = 0; e < 4; ++e) raw[r][4 * x + e] = w[e];
       }
     }
   }
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void load(const HeadPages<D, kFour>& h, int64_t row, int c, int g) {
+    const GlobalBytes p = tile_base(h.values + row * h.kRowBytes);
+    GlobalBytes s = p;
+    if constexpr (kFour) s = tile_base(h.value_scales + row * h.kRowScales);
 #pragma unroll
-    for (auto& x : raw) x = 0;
-    scale = 127;
+    for (int r = 0; r < 4; ++r) load_row(p, s, r, 4 * g + r, c);
+    if constexpr (kFour && D == 128) {   // of the four rows: 16 bytes
+      const u32x4 w = global_load<u32x4>(s, 16 * g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) scale[r] = w[r];
+    }
   }
-  __device__ __forceinline__ bool finite() const {
-    if constexpr (kFour) return scale != 255;
+  __device__ __forceinline__ void clear(int r) {
+#pragma unroll
+    for (auto& x : raw[r]) x = 0;
+    if constexpr (kFour) scale[r] = 0x7f7f7f7fu;
+  }
+  __device__ __forceinline__ bool finite(int r, int c) const {
+    if constexpr (kFour) return (scale[r] >> (8 * scale_byte(c)) & 255) != 255;
     bool ok = true;
 #pragma unroll
-    for (uint32_t x : raw)
+    for (uint32_t x : raw[r])
       ok = ok && (x & 0x7f80u) != 0x7f80u && (x & 0x7f800000u) != 0x7f800000u;
     return ok;
   }
-  // Dims 8 x .. 8 x + 7 of the lane's as four bf16 pairs.
-  __device__ __forceinline__ u32x4 wide(int x) const {
-    if constexpr (kFour) return widen8(raw[x], __uint_as_float(scale << 23));
-    else return u32x4{raw[4 * x], raw[4 * x + 1], raw[4 * x + 2], raw[4 * x + 3]};
+  // Dims 2 x and 2 x + 1 of the lane's in row r as a bf16 pair.
+  __device__ __forceinline__ uint32_t pair(int r, int x, int c) const {
+    if constexpr (kFour) {
+      const float size = scale_of(scale[r], scale_byte(c));
+      const uint32_t w = raw[r][x / 4];
+      return __builtin_bit_cast(
+          uint32_t, x % 4 == 0   ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, size, 0)
+                    : x % 4 == 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, size, 1)
+                    : x % 4 == 2 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, size, 2)
+                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, size, 3));
+    } else {
+      return raw[r][x];
+    }
   }
 };
 
@@ -365,7 +417,7 @@ struct Wave {
   using Pages = HeadPages<D, kFour>;
   static constexpr int T = Shape::kTiles, KK = D / 32, N = D / 16;
   KeyTile<D, kFour> key[T];
-  ValueRow<D, kFour> value[T][4];
+  ValueTile<D, kFour> value[T];
   f32x4 o[N];                            // [query row 4 g + r][value_dim(c, i)]
   f32x4 l;                               // sums of P, query row 4 g + r
   float m;                               // maximum of column c, unscaled
@@ -393,13 +445,8 @@ struct Wave {
   }
   __device__ __forceinline__ void load_values(const Pages& h, int j, int key0, int c, int g) {
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int64_t row = h.row(max(page(j, t), 0), key0 + 16 * t);
-      const uint8_t* p = tile_base(h.values + row * h.kRowBytes);
-      const uint8_t* s = kFour ? tile_base(h.value_scales + row * h.kRowScales) : nullptr;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) value[t][r].load(p, s, 4 * g + r, c);
-    }
+    for (int t = 0; t < T; ++t)
+      value[t].load(h, h.row(max(page(j, t), 0), key0 + 16 * t), c, g);
   }
 
   // Units j .. end - 1. The next unit's keys are fetched as soon as the scores are formed, its
@@ -428,7 +475,7 @@ struct Wave {
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-        for (int t = 0; t < T; ++t) x[t] = mfma16(key[t].operand(kk), q[kk], x[t]);
+        for (int t = 0; t < T; ++t) x[t] = mfma16(key[t].operand(kk, g), q[kk], x[t]);
       __builtin_amdgcn_sched_barrier(0);
       if (Shape::kEarlyKeys && more) {
         if (j + 1 - id_base >= kWave / T) load_ids(s, j + 1, w, lane);
@@ -453,6 +500,7 @@ struct Wave {
                                                    int g) {
     bool split = false;                  // V rows of some columns only, not finite: left out
     if (unplaced != 0 || key0 + 16 * T - 1 > s.first) {
+      const int g = thread_lane() >> 4, c = thread_lane() & 15;
       // scores of keys that a column does not see are -inf; rows that no column sees are 0, so
       // that what lies behind the last token does not meet a probability of 0
 #pragma unroll
@@ -463,10 +511,10 @@ struct Wave {
           const bool here = !(unplaced >> t & 1);
           if (!here || p > s.column) x[t][r] = -INFINITY;
           if (!here || p >= s.keys) {
-            value[t][r].clear();
-          } else if (p > s.first && !value[t][r].finite()) {
+            value[t].clear(r);
+          } else if (p > s.first && !value[t].finite(r, c)) {
             split = true;
-            value[t][r].clear();
+            value[t].clear(r);
           }
         }
     }
@@ -475,14 +523,13 @@ struct Wave {
     for (int t = 0; t < T; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) mx = fmaxf(mx, x[t][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    mx = max_over_rows(mx);
     if (__any(mx > m)) {
       const float m_new = fmaxf(m, mx);
       const float corr = m == -INFINITY ? 0.0f : exp2_fast((m - m_new) * scale);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float cr = __shfl(corr, 4 * g + r);
+        const float cr = __shfl(corr, 4 * (thread_lane() >> 4) + r);
         l[r] *= cr;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i][r] *= cr;
@@ -502,7 +549,7 @@ struct Wave {
           l = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], 1.0f, l, 0, 0, 0);
 #pragma unroll
           for (int i = 0; i < N; i += 2) {
-            const uint32_t v2 = value[t][r].raw[i / 2];
+            const uint32_t v2 = value[t].raw[r][i / 2];
             o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_lo(v2), o[i], 0, 0, 0);
             o[i + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[t][r], bf16_hi(v2), o[i + 1], 0, 0, 0);
           }
@@ -514,47 +561,49 @@ struct Wave {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float u = x[t + e / 2][2 * (e % 2)], w = x[t + e / 2][2 * (e % 2) + 1];
-          hi[e] = pack_bf16x2(u, w);
+          hi[e] = opaque_bits(pack_bf16x2(u, w));
           lo[e] = pack_bf16x2(u - bf16_lo(hi[e]), w - bf16_hi(hi[e]));
         }
         const uint32_t ones = 0x3f803f80u;
         l = mfma16(hi, u32x4{ones, ones, ones, ones}, l);
         l = mfma16(lo, u32x4{ones, ones, ones, ones}, l);
 #pragma unroll
-        for (int y = 0; y < N / 8; ++y) {
-          u32x4 row[8];
+        for (int y = 0; y < N / 2; ++y) {
+          uint32_t row[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) row[j] = value[t + j / 4][j % 4].wide(y);
+          for (int j = 0; j < 8; ++j) row[j] = value[t + j / 4].pair(j % 4, y, c);
+          u32x4 even, odd;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            u32x4 b;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              b[e] = __builtin_amdgcn_perm(row[2 * e + 1][i / 2], row[2 * e][i / 2],
-                                           i % 2 ? 0x07060302u : 0x05040100u);
-            o[8 * y + i] = mfma16(hi, b, o[8 * y + i]);
-            o[8 * y + i] = mfma16(lo, b, o[8 * y + i]);
+          for (int e = 0; e < 4; ++e) {
+            even[e] = __builtin_amdgcn_perm(row[2 * e + 1], row[2 * e], 0x05040100u);
+            odd[e] = __builtin_amdgcn_perm(row[2 * e + 1], row[2 * e], 0x07060302u);
           }
+          o[2 * y] = mfma16(hi, even, o[2 * y]);
+          o[2 * y + 1] = mfma16(hi, odd, o[2 * y + 1]);
+          o[2 * y] = mfma16(lo, even, o[2 * y]);
+          o[2 * y + 1] = mfma16(lo, odd, o[2 * y + 1]);
         }
       }
     }
-    if (__any(split)) add_split_rows(h, s, x, key0, c, g);
+    if (__any(split)) add_split_rows(h, s, x, key0);
   }
 
   // The V rows that were left out, one after the other: only into the columns that see them.
   __device__ __forceinline__ void add_split_rows(const Pages& h, const Limits& s,
-                                                 const f32x4 (&p)[T], int key0, int c, int g) {
+                                                 const f32x4 (&p)[T], int key0) {
     const PagedAttnArgs a = fresh_args();
+    const int g = thread_lane() >> 4, c = thread_lane() & 15;
     const int last = min(key0 + 16 * T, s.keys);
 #pragma unroll 1
     for (int at = max(key0, s.first + 1); at < last; ++at) {
       const int id = a.map.page(s.b, at);
       if (id < 0) continue;
-      ValueRow<D, kFour> v;
       const int64_t row = h.row(id, at);
-      v.load(h.values + row * h.kRowBytes, kFour ? h.value_scales + row * h.kRowScales : nullptr, 0,
-             c);
-      const bool left_out = !v.finite();
+      ValueTile<D, kFour> v;             // its row 0
+      const GlobalBytes scales = kFour ? h.value_scales + row * h.kRowScales : h.values;
+      v.load_row(h.values + row * h.kRowBytes, scales, 0, 0, c);
+      if constexpr (kFour && D == 128) v.scale[0] = global_load<uint32_t>(scales, 0);
+      const bool left_out = !v.finite(0, c);
       float mine = 0.0f;                 // the probability of key `at`, where this lane has it
 #pragma unroll
       for (int t = 0; t < T; ++t)
@@ -566,13 +615,10 @@ struct Wave {
         const int seen = __shfl(s.column, 4 * g + r);
         const bool sees = left_out && at <= seen;
 #pragma unroll
-        for (int y = 0; y < N / 8; ++y) {
-          const u32x4 w = v.wide(y);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[8 * y + 2 * e][r] += sees ? prob * bf16_lo(w[e]) : 0.0f;
-            o[8 * y + 2 * e + 1][r] += sees ? prob * bf16_hi(w[e]) : 0.0f;
-          }
+        for (int y = 0; y < N / 2; ++y) {
+          const uint32_t w = v.pair(0, y, c);
+          o[2 * y][r] += sees ? prob * bf16_lo(w) : 0.0f;
+          o[2 * y + 1][r] += sees ? prob * bf16_hi(w) : 0.0f;
         }
       }
     }
