@@ -60,12 +60,12 @@ def test_append_arguments():
     assert _append(rope=(4095, 128, 0)) == invalid                # the table reaches 4096
     for rotary in (0, 8, 120, 144):
         assert _append(rope=(4096, rotary, 0)) == unsupported
-    assert _append(batch=1 << 20, tokens=1 << 10) == invalid
+    assert _append(tokens=(1 << 24) + 1) == _append(q_heads=1 << 20) == invalid
 
 
 def test_gather_and_attention_arguments():
     invalid = _lib.SPX_EINVAL
-    assert _gather(out=None) == _gather(out=OFF) == _gather(batch=1 << 20, tokens=1 << 12) == invalid
+    assert _gather(out=None) == _gather(out=OFF) == _gather(tokens=(1 << 24) + 1) == invalid
     assert _attention(q=None) == _attention(q=OFF) == _attention(qs=ODD) == invalid
     assert _attention(out=None) == _attention(max_keys=-1) == _attention(workspace=None) == invalid
     assert _attention(q_heads=27) == _attention(batch=1 << 16, tokens=1 << 10, q_heads=32) == invalid
