@@ -93,6 +93,19 @@ __device__ __forceinline__ double fma_of(double x, double y, double z) {
   return __builtin_fma(x, y, z);
 }
 
+// Outputs of 4 MB and more go past the caches: 16000 tokens appended (28/4 heads, rotated copies
+// of q and k) 77 -> 52 us, 4 x 12001 read back 51 -> 43; a dense prefill behind the append takes as
+// long in all (16000 tokens 1632 and 1632 us, 1089 43.6 and 42.8). Those of a decode step are
+// read at once: attention behind it 36.3 us with them in the cache, 37.1 past it.
+constexpr int64_t kStreamedBytes = 4 << 20;
+
+// (A template parameter: of a run-time choice the compiler makes one ordinary store.)
+template <bool kStreamed>
+__device__ __forceinline__ void store_row(uint16_t* p, const u32x4& x) {
+  if constexpr (kStreamed) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<u32x4*>(p) = x;
+}
+
 // A lane's part of the rotation of a token: its eight dims 8 piece .. 8 piece + 7.
 struct Rotation {
   bool turns, interleaved;
@@ -196,10 +209,10 @@ struct RowPart {
 // rows have in common (its place, cos and sin of the lane's dims) is found once, behind the
 // loads of the first rows; the next row is loaded while one is rotated. Measured against a row
 // per group of lanes and no loop: 32640 tokens (28/4 heads, bf16, rotated copies of q and k)
-// 159 -> 145 us, 4.5 TB/s where a copy reaches 4.7; three rows in flight per lane 167. With
-// 4-bit pages five waves per SIMD (the fp64 rotation has the registers of four) 50 -> 46.5 us
-// for 4 x 2113 padded tokens at D = 256, reading back included.
-template <int D, bool kFour>
+// 159 -> 145 us, 140 with streamed stores: 4.65 TB/s where a copy reaches 4.7. Three rows in
+// flight per lane: 167. With 4-bit pages five waves per SIMD (the fp64 rotation has the
+// registers of four): 4 x 2113 padded tokens at D = 256, reading back included, 48.5 -> 44 us.
+template <int D, bool kFour, bool kStreamed>
 __global__ __launch_bounds__(kPagedThreads, kFour ? 5 : 1) void paged_append_kernel(AppendArgs a) {
   constexpr int kPieces = D / 8, kRows = kWave / kPieces;        // lanes of a row, rows of a wave
   const int lane = threadIdx.x & 63, piece = lane % kPieces, d0 = 8 * piece;
@@ -227,7 +240,7 @@ __global__ __launch_bounds__(kPagedThreads, kFour ? 5 : 1) void paged_append_ker
                       : is_k && a.k_out ? a.k_out + (token * a.kv_heads + head) * D
                                         : nullptr;
       if (p < 0) {
-        if (out) *reinterpret_cast<u32x4*>(out + d0) = u32x4{};
+        if (out) store_row<kStreamed>(out + d0, u32x4{});
         continue;
       }
       const int64_t row = is_q || page < 0 ? -1 : a.map.row(page, head, p);
@@ -238,14 +251,14 @@ __global__ __launch_bounds__(kPagedThreads, kFour ? 5 : 1) void paged_append_ker
         rotation.apply<double>(now.own, now.other, y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = round_to_odd(y[e]);
-        if (out) *reinterpret_cast<u32x4*>(out + d0) = pack8(x);
+        if (out) store_row<kStreamed>(out + d0, pack8(x));
       } else {
         u32x4 packed = now.own;
         if ((is_q || is_k) && rotation.turns) {
           rotation.apply<float>(now.own, now.other, x);
           packed = pack8(x);
         }
-        if (out) *reinterpret_cast<u32x4*>(out + d0) = packed;
+        if (out) store_row<kStreamed>(out + d0, packed);
         if (kFour && !is_q) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -298,7 +311,7 @@ struct StoredPart {
 };
 
 // Waves and tokens as in the append kernel.
-template <int D, bool kFour>
+template <int D, bool kFour, bool kStreamed>
 __global__ __launch_bounds__(kPagedThreads) void paged_gather_kernel(GatherArgs a) {
   constexpr int kPieces = D / 8, kRows = kWave / kPieces;
   const int lane = threadIdx.x & 63, piece = lane % kPieces;
@@ -320,7 +333,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_gather_kernel(GatherArgs 
       const bool is_v = r >= a.kv_heads;
       uint16_t* out = is_v ? a.v_out : a.k_out;
       const int64_t row = token * a.kv_heads + (is_v ? r - a.kv_heads : r);
-      reinterpret_cast<u32x4*>(out)[row * kPieces + piece] = page < 0 ? u32x4{} : now.value();
+      store_row<kStreamed>(out + row * D + 8 * piece, page < 0 ? u32x4{} : now.value());
     }
   }
 }
@@ -350,6 +363,22 @@ static int row_source(RowSource& r, const void* base, const int64_t* strides, co
   r.s_t = strides[1];
   r.s_h = strides[2];
   return SPX_OK;
+}
+
+template <int D>
+static void launch_append(const AppendArgs& a, bool four, bool streamed, dim3 grid, hipStream_t st) {
+  if (four && streamed) paged_append_kernel<D, true, true><<<grid, kPagedThreads, 0, st>>>(a);
+  else if (four) paged_append_kernel<D, true, false><<<grid, kPagedThreads, 0, st>>>(a);
+  else if (streamed) paged_append_kernel<D, false, true><<<grid, kPagedThreads, 0, st>>>(a);
+  else paged_append_kernel<D, false, false><<<grid, kPagedThreads, 0, st>>>(a);
+}
+
+template <int D>
+static void launch_gather(const GatherArgs& a, bool four, bool streamed, dim3 grid, hipStream_t st) {
+  if (four && streamed) paged_gather_kernel<D, true, true><<<grid, kPagedThreads, 0, st>>>(a);
+  else if (four) paged_gather_kernel<D, true, false><<<grid, kPagedThreads, 0, st>>>(a);
+  else if (streamed) paged_gather_kernel<D, false, true><<<grid, kPagedThreads, 0, st>>>(a);
+  else paged_gather_kernel<D, false, false><<<grid, kPagedThreads, 0, st>>>(a);
 }
 
 }  // namespace spx
@@ -394,6 +423,8 @@ extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
   SPX_REQUIRE(rows <= 1 << 20 && cache->tokens <= 1 << 24, SPX_EINVAL,
               "more than 2^20 heads or 2^24 tokens in a call");
   a.wave_shift = token_waves((int64_t)a.batch * a.tokens, rows, cache->head_dim);
+  const bool streamed = (int64_t)a.batch * a.tokens * (a.q_rows + (k_out ? a.kv_heads : 0)) *
+                            cache->head_dim * 2 >= kStreamedBytes;
   a.key_pages = cache->key_pages; a.value_pages = cache->value_pages;
   a.key_scales = static_cast<uint8_t*>(cache->key_scales);
   a.value_scales = static_cast<uint8_t*>(cache->value_scales);
@@ -402,13 +433,8 @@ extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool four = cache->key_scales != nullptr;
   const dim3 grid = token_grid(a.batch, a.tokens, a.wave_shift);
-  if (cache->head_dim == 128) {
-    if (four) paged_append_kernel<128, true><<<grid, kPagedThreads, 0, st>>>(a);
-    else paged_append_kernel<128, false><<<grid, kPagedThreads, 0, st>>>(a);
-  } else {
-    if (four) paged_append_kernel<256, true><<<grid, kPagedThreads, 0, st>>>(a);
-    else paged_append_kernel<256, false><<<grid, kPagedThreads, 0, st>>>(a);
-  }
+  if (cache->head_dim == 128) launch_append<128>(a, four, streamed, grid, st);
+  else launch_append<256>(a, four, streamed, grid, st);
   return launch_status("paged_append");
 }
 
@@ -430,17 +456,14 @@ extern "C" int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void*
   SPX_REQUIRE(a.kv_heads <= 1 << 19 && a.tokens <= 1 << 24, SPX_EINVAL,
               "more than 2^19 heads or 2^24 tokens in a call");
   a.wave_shift = token_waves((int64_t)a.batch * a.tokens, 2 * a.kv_heads, cache->head_dim);
+  const bool streamed =
+      (int64_t)a.batch * a.tokens * 2 * a.kv_heads * cache->head_dim * 2 >= kStreamedBytes;
   a.k_out = static_cast<uint16_t*>(k_out);
   a.v_out = static_cast<uint16_t*>(v_out);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const bool four = cache->key_scales != nullptr;
   const dim3 grid = token_grid(a.batch, a.tokens, a.wave_shift);
-  if (cache->head_dim == 128) {
-    if (four) paged_gather_kernel<128, true><<<grid, kPagedThreads, 0, st>>>(a);
-    else paged_gather_kernel<128, false><<<grid, kPagedThreads, 0, st>>>(a);
-  } else {
-    if (four) paged_gather_kernel<256, true><<<grid, kPagedThreads, 0, st>>>(a);
-    else paged_gather_kernel<256, false><<<grid, kPagedThreads, 0, st>>>(a);
-  }
+  if (cache->head_dim == 128) launch_gather<128>(a, four, streamed, grid, st);
+  else launch_gather<256>(a, four, streamed, grid, st);
   return launch_status("paged_gather");
 }
