@@ -8,6 +8,7 @@ not on a ROCm GPU.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from pathlib import Path
 
 import torch
@@ -60,7 +61,7 @@ _PROTOTYPES = {
     "spx_sparse_attention_rescue": [_P, _S, _P, _P, _P, _S, _P, _S, _P, _P, _S, _P, _P, _I, _I,
                                     _I, _I, _I, _I, _I, _F, _P, _S, _P, _S, _P, _P],
     "spx_decode_attention": [_P, _S, _P, _S, _P, _S, _I, _I, _I, _I, _I, _F, _P, _P, _P],
-    # the first argument and the strides as packed bytes
+    # called by exp3_amd/csrc/paged_host.cpp; the first argument is a struct spx_paged_cache
     "spx_paged_append": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P],
     "spx_paged_gather": [_P, _P, _P, _P],
     "spx_paged_attention": [_P, _P, _P, _I, _I, _F, _P, _P, _P, _P],
@@ -105,6 +106,25 @@ def load() -> ctypes.CDLL:
                            f"bindings {ABI_VERSION}; rebuild the library")
     _lib = lib
     return lib
+
+
+_host = None
+
+
+def host_module():
+    """The extension module of the paged cache's host path (raises if it has not been built)."""
+    global _host
+    if _host is None:
+        load()
+        path = LIBRARY_PATH.parent / "_paged.so"
+        if not path.exists():
+            raise RuntimeError(f"exp3_amd host module not found at {path}; build it with "
+                               "`python -m exp3_amd.build`")
+        spec = importlib.util.spec_from_file_location("exp3_amd._C._paged", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _host = module
+    return _host
 
 
 def call(name: str, *args) -> None:

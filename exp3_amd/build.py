@@ -2,7 +2,9 @@
 
 Compiles every ``csrc/*.hip`` with hipcc for gfx950 only and links one shared
 library exporting the C ABI declared in ``include/sparse_prefill.h``. Packed
-FP32 instructions are disabled for all device code.
+FP32 instructions are disabled for all device code. ``csrc/paged_host.cpp``, the
+Python host path of the paged cache, becomes the extension module
+``exp3_amd/_C/_paged.so`` against that library and the installed torch.
 
 Usage: ``python -m exp3_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -14,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -21,6 +24,8 @@ REPO = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
 OUT_DIR = PACKAGE / "_C"
 LIBRARY = OUT_DIR / "libexp3_amd.so"
+HOST_MODULE = OUT_DIR / "_paged.so"
+HOST_SOURCE = CSRC / "paged_host.cpp"
 BUILD_DIR = REPO / "_build"
 ARCH = "gfx950"
 
@@ -76,6 +81,35 @@ def _compile(hipcc: str, source: Path) -> Path:
     return obj
 
 
+def _compile_host_module() -> Path:
+    """csrc/paged_host.cpp -> an object file (host code only: the C++ compiler)."""
+    import torch
+    from torch.utils import cpp_extension
+
+    obj = BUILD_DIR / (HOST_SOURCE.stem + ".host.o")
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], REPO / "include"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{path}" for path in includes), "-c", str(HOST_SOURCE), "-o", str(obj)]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for {HOST_SOURCE.name}:\n{proc.stderr}")
+    return obj
+
+
+def _link_host_module(obj: Path) -> None:
+    from torch.utils import cpp_extension
+
+    tmp = HOST_MODULE.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", str(tmp), str(obj), f"-L{OUT_DIR}",
+           f"-l:{LIBRARY.name}", f"-L{cpp_extension.TORCH_LIB_PATH}", "-lc10", "-ltorch_cpu",
+           "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"link failed:\n{proc.stderr}")
+    os.replace(tmp, HOST_MODULE)
+
+
 def build(verbose: bool = True) -> Path:
     """Compile all sources and link the shared library; returns its path."""
     hipcc = _hipcc()
@@ -84,15 +118,19 @@ def build(verbose: bool = True) -> Path:
     sources = sorted(CSRC.glob("*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
-    workers = min(len(sources), os.cpu_count() or 1, 8)
+    workers = min(len(sources) + 1, os.cpu_count() or 1, 8)
     with concurrent.futures.ThreadPoolExecutor(workers) as pool:
+        host = pool.submit(_compile_host_module)
         objects = list(pool.map(lambda s: _compile(hipcc, s), sources))
+        host_object = host.result()
     tmp = LIBRARY.with_suffix(".so.tmp")
-    cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objects)]
+    cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", f"-Wl,-soname,{LIBRARY.name}",
+           "-o", str(tmp), *map(str, objects)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stderr}")
     os.replace(tmp, LIBRARY)
+    _link_host_module(host_object)
     if verbose:
         print(f"built {LIBRARY.relative_to(REPO)} from {len(sources)} sources", flush=True)
     return LIBRARY

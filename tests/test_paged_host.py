@@ -2,6 +2,7 @@
 launch, and the 64-bit reference's 4-bit grid against its definition."""
 
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -16,8 +17,8 @@ ODD = bytes((ctypes.c_int64 * 4)(4096, 512, 132, 1))
 
 def _cache(pages=(FAKE, FAKE, 0, 0), table=FAKE, starts=FAKE, counts=0, stride=32, width=32, held=64,
            page_size=128, kv_heads=4, dim=128, batch=2, tokens=1):
-    return paged._DESCRIPTION.pack(*pages, table, starts, counts, stride, width, held, page_size,
-                                   kv_heads, dim, batch, tokens, 0)
+    return struct.pack("7Pq8i", *pages, table, starts, counts, stride, width, held, page_size,
+                       kv_heads, dim, batch, tokens, 0)
 
 
 def _append(cache=None, q=FAKE, k=FAKE, ks=S4, q_heads=28, cos=FAKE, sin=FAKE, rope=(4096, 128, 0),
@@ -80,6 +81,12 @@ def test_wrappers_refuse():
     x = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
     table, starts = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
     for call in (lambda: paged.append_tokens(cache, table, starts, x, x),
+                 lambda: _lib.host_module().append(*[cache.key_pages, cache.value_pages, None, None],
+                                                   table, starts, None, x, x, *[None] * 3, 0, 0, 0),
+                 lambda: _lib.host_module().gather(cache.key_pages, cache.value_pages, None, None,
+                                                   table, starts, None, 1, 0),
+                 lambda: _lib.host_module().attention(cache.key_pages, cache.value_pages, None, None,
+                                                      table, starts, None, x, 0.1, 0, 0, 0),
                  lambda: paged.gather_tokens(cache, table, starts, 1),
                  lambda: paged.paged_attention(x, cache, table, starts, 0.1)):
         with pytest.raises(ValueError, match="ROCm GPU"):
@@ -89,14 +96,20 @@ def test_wrappers_refuse():
             paged.empty_pages(*bad, "cpu")
 
 
-def test_wrapper_checks_of_shapes():
-    """The checks that need no GPU tensors of their own, on the CPU."""
-    cpu = -1                        # the index of a CPU tensor
+def _describe(cache, table, starts, counts, batch=2, tokens=3):
+    return _lib.host_module().describe(cache.key_pages, cache.value_pages, cache.key_scales,
+                                       cache.value_scales, table, starts, counts, batch, tokens)
+
+
+def test_checks_of_the_host_module():
+    """Its checks of cache and page table, which look at no device, on the CPU."""
     good = paged.empty_pages(4, 16, 2, 128, "cpu", four_bit=True)
-    assert paged._check_cache(good, cpu)[1:] == (4, 16, 2, 128)
-    assert (good.page_size, good.kv_heads, good.head_dim, good.four_bit) == (16, 2, 128, True)
     half = paged.empty_pages(4, 16, 2, 256, "cpu")
-    assert paged._check_cache(half, cpu)[1:] == (4, 16, 2, 256) and half.head_dim == 256
+    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    assert _describe(good, table, starts, starts) == (4, 16, 2, 128, 4)
+    assert _describe(half, table, starts, None) == (4, 16, 2, 256, 4)
+    assert (good.page_size, good.kv_heads, good.head_dim, good.four_bit) == (16, 2, 128, True)
+    assert half.head_dim == 256 and not half.four_bit
     bad = (paged.PagedCache(good.key_pages, good.value_pages, good.key_scales),
            paged.PagedCache(half.key_pages, half.value_pages, None, good.value_scales),
            paged.PagedCache(good.key_pages, good.value_pages),
@@ -104,24 +117,23 @@ def test_wrapper_checks_of_shapes():
            paged.PagedCache(half.key_pages.transpose(1, 2), half.value_pages.transpose(1, 2)),
            paged.PagedCache(half.key_pages.half(), half.value_pages.half()),
            paged.PagedCache(half.key_pages[0], half.value_pages[0]),
+           paged.PagedCache(half.key_pages, None), paged.PagedCache(None, half.value_pages),
            paged.PagedCache(good.key_pages, good.value_pages, good.key_scales[..., :2],
-                            good.value_scales[..., :2]))
+                            good.value_scales[..., :2]),
+           paged.PagedCache(half.key_pages, half.value_pages.to("meta")))
     for cache in bad:
         with pytest.raises(ValueError):
-            paged._check_cache(cache, cpu)
-    with pytest.raises(ValueError, match="device"):
-        paged._check_cache(half, 0)
-    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
-    _, heads, dim, sizes = paged._describe(good, table, starts, starts, 2, 3, cpu)
-    assert (heads, dim) == (2, 128) and sizes == (4, 4, 16, 2, 128, 2, 3, 0)
-    assert paged._describe(good, torch.zeros(2, 9, dtype=torch.int32)[:, 2:6], starts, None, 2, 3,
-                           cpu)[3] == sizes
+            _describe(cache, table, starts, None)
+    assert _describe(good, torch.zeros(2, 9, dtype=torch.int32)[:, 2:6], starts, None)[-1] == 4
     for wrong in ((table.long(), starts, None), (table, starts.long(), None), (table[:1], starts, None),
-                  (table, starts[:1], None), (table, starts, starts.long()),
-                  (table.repeat(1, 2)[:, ::2], starts, None),
-                  (table, torch.zeros(4, dtype=torch.int32)[::2], None)):
+                  (table, starts[:1], None), (table, starts, starts.long()), (table[0], starts, None),
+                  (table.repeat(1, 2)[:, ::2], starts, None), (table, starts[:, None], None),
+                  (table, torch.zeros(4, dtype=torch.int32)[::2], None), (table, None, None),
+                  (table, starts, [0, 0])):
         with pytest.raises(ValueError):
-            paged._describe(good, *wrong, 2, 3, cpu)
+            _describe(good, *wrong)
+    with pytest.raises(TypeError):
+        _lib.host_module().describe(1, 2)
 
 
 def test_rope_table_far_positions():
