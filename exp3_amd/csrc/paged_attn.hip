@@ -292,6 +292,11 @@ __device__ __forceinline__ uint32_t opaque_bits(uint32_t x) { return (uint32_t)o
 // The lane, recomputed where it is used: what rare paths derive from it is not held meanwhile.
 __device__ __forceinline__ int thread_lane() { return opaque((int)threadIdx.x) & 63; }
 
+__device__ __forceinline__ float sum_of_halves(float x) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+
 // Maximum over the lanes c, c + 16, c + 32, c + 48.
 __device__ __forceinline__ float max_over_rows(float x) {
   const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -442,7 +447,10 @@ struct Limits {
 };
 
 // A wave's tiles of a stream: page ids, keys and values of one unit, O and the softmax state.
-template <int D, bool kFour, int W>
+// kHalf (4-bit pages): at most eight columns; column c + 8 is column c again, and holds the second
+// part of its P in the products with V (the halves of O are added in the end), which saves half
+// of these.
+template <int D, bool kFour, int W, bool kHalf>
 struct Wave {
   using Shape = PagedShape<D, kFour, W>;
   using Pages = HeadPages<D, kFour>;
@@ -591,16 +599,20 @@ struct Wave {
     } else {
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
-        u32x4 hi, lo;
+        u32x4 hi, lo;                    // kHalf: hi holds the one or the other
+        const uint32_t second = c < kPaCols / 2 ? 0 : ~0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float u = x[t + e / 2][2 * (e % 2)], w = x[t + e / 2][2 * (e % 2) + 1];
-          hi[e] = opaque_bits(pack_bf16x2(u, w));
-          lo[e] = pack_bf16x2(u - bf16_lo(hi[e]), w - bf16_hi(hi[e]));
+          const uint32_t first_part = opaque_bits(pack_bf16x2(u, w));
+          const uint32_t off = kHalf ? first_part & second : first_part;
+          const uint32_t rest = pack_bf16x2(u - bf16_lo(off), w - bf16_hi(off));
+          hi[e] = kHalf ? rest : first_part;
+          lo[e] = rest;
         }
         const uint32_t ones = 0x3f803f80u;
         l = mfma16(hi, u32x4{ones, ones, ones, ones}, l);
-        l = mfma16(lo, u32x4{ones, ones, ones, ones}, l);
+        if constexpr (!kHalf) l = mfma16(lo, u32x4{ones, ones, ones, ones}, l);
 #pragma unroll
         for (int y = 0; y < N / 2; ++y) {
           uint32_t row[8];
@@ -614,8 +626,10 @@ struct Wave {
           }
           o[2 * y] = mfma16(hi, even, o[2 * y]);
           o[2 * y + 1] = mfma16(hi, odd, o[2 * y + 1]);
-          o[2 * y] = mfma16(lo, even, o[2 * y]);
-          o[2 * y + 1] = mfma16(lo, odd, o[2 * y + 1]);
+          if constexpr (!kHalf) {
+            o[2 * y] = mfma16(lo, even, o[2 * y]);
+            o[2 * y + 1] = mfma16(lo, odd, o[2 * y + 1]);
+          }
         }
       }
     }
@@ -647,7 +661,7 @@ struct Wave {
       for (int r = 0; r < 4; ++r) {
         const float prob = __shfl(mine, 16 * (at / 4 % 4) + 4 * g + r);
         const int seen = __shfl(s.column, 4 * g + r);
-        const bool sees = left_out && at <= seen;
+        const bool sees = left_out && at <= seen && (!kHalf || 4 * g + r < kPaCols / 2);
 #pragma unroll
         for (int y = 0; y < N / 2; ++y) {
           const uint32_t w = v.pair(0, y, c);
@@ -656,6 +670,16 @@ struct Wave {
         }
       }
     }
+  }
+
+  // kHalf: rows 8 to 15 of O and the sums added to rows 0 to 7 (lanes 32 apart).
+  __device__ __forceinline__ void add_halves() {
+#pragma unroll
+    for (auto& x : o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = sum_of_halves(x[r]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) l[r] = sum_of_halves(l[r]);
   }
 
   __device__ __forceinline__ bool any_nan() const {
@@ -669,13 +693,13 @@ struct Wave {
 };
 
 // grid > 0: workgroup w takes its run of all units; grid == 0: workgroup w is stream w.
-template <int D, bool kFour, int W>
+template <int D, bool kFour, int W, bool kHalf>
 __global__ __launch_bounds__(64 * W, (PagedShape<D, kFour, W>::kPerCu * W / 4)) void
 paged_attn_kernel(PagedAttnArgs args) {
   using Shape = PagedShape<D, kFour, W>;
   constexpr int KK = D / 32;
   __shared__ float part_m[W][kPaCols], part_l[W][kPaCols];
-  __shared__ __align__(16) float part_o[W][kPaCols][D];
+  __shared__ __align__(16) float part_o[W][kHalf ? kPaCols / 2 : kPaCols][D];
   const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   touch_args();
@@ -714,11 +738,11 @@ paged_attn_kernel(PagedAttnArgs args) {
     {
       const PagedAttnArgs a = fresh_args();
       cols = min(kPaCols, a.cols - s.tile * kPaCols);
-      const int n = s.tile * kPaCols + min(c, cols - 1);    // columns past the last repeat it
+      const int n = s.tile * kPaCols + min(kHalf ? c % (kPaCols / 2) : c, cols - 1);   // the last repeats
       const int token = column_token(a, n);
       const int head = s.kvh * a.group + n - token * a.group;
       const Limits limits{s.b, s.keys, s.start + tile_first(a, s.tile), s.start + token};
-      Wave<D, kFour, W> acc;
+      Wave<D, kFour, W, kHalf> acc;
       acc.load_ids(limits, j0, w, lane);
       u32x4 q[KK];
       const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
@@ -730,9 +754,11 @@ paged_attn_kernel(PagedAttnArgs args) {
       }
       const HeadPages<D, kFour> pages(a, s.kvh);
       acc.template run<false>(pages, limits, q, a.scale_log2, j0, j1, w, lane, c, g);
+      if constexpr (kHalf) acc.add_halves();
       if (g == 0) part_m[w][c] = acc.m == -INFINITY ? -INFINITY : acc.m * a.scale_log2;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        if (kHalf && g >= 2) break;
         if (c == 0) part_l[w][4 * g + r] = acc.l[r];
 #pragma unroll
         for (int i = 0; i < D / 16; i += 4)
@@ -965,18 +991,14 @@ __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnA
 // kernels, 1024 equal; 64 rows of 128 partials 21 against 41 us.
 constexpr int kPaWaveRows = 1024;
 
-// How a launch is divided: workgroups of `waves` waves, `grid` of them sharing the units, or
-// (grid 0) one per stream and no second launch.
-struct PagedPlan {
-  int grid, waves;
-};
-
+// Workgroups (of four waves) that share the units, or 0: one of eight waves per stream and no
+// second launch.
 template <int D, bool kFour>
-static PagedPlan paged_plan(int64_t keys, int64_t streams) {
-  if (keys <= 4 * PagedShape<D, kFour, 8>::kUnit) return {0, 8};
+static int paged_grid(int64_t keys, int64_t streams) {
+  if (keys <= 2 * PagedShape<D, kFour, 8>::kUnit) return 0;
   using Shape = PagedShape<D, kFour, 4>;
   const int64_t units = (keys + Shape::kUnit - 1) / Shape::kUnit;
-  return {(int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units), 4};
+  return (int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units);
 }
 
 struct PagedSizes {
@@ -998,19 +1020,17 @@ static bool paged_sizes(const spx_paged_cache& z, int q_heads, int max_keys, Pag
   return true;
 }
 
-static PagedPlan paged_plan_of(const PagedSizes& z, int head_dim, bool four) {
+static int paged_grid_of(const PagedSizes& z, int head_dim, bool four) {
   if (head_dim == 128)
-    return four ? paged_plan<128, true>(z.keys, z.streams) : paged_plan<128, false>(z.keys, z.streams);
-  return four ? paged_plan<256, true>(z.keys, z.streams) : paged_plan<256, false>(z.keys, z.streams);
+    return four ? paged_grid<128, true>(z.keys, z.streams) : paged_grid<128, false>(z.keys, z.streams);
+  return four ? paged_grid<256, true>(z.keys, z.streams) : paged_grid<256, false>(z.keys, z.streams);
 }
 
 template <int D, bool kFour>
-static int launch_paged(PagedAttnArgs a, const PagedSizes& z, int waves, void* workspace,
-                        hipStream_t st) {
+static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, hipStream_t st) {
   if (a.grid == 0) {
     const unsigned streams = (unsigned)z.streams;
-    if (waves == 8) paged_attn_kernel<D, kFour, 8><<<streams, 512, 0, st>>>(a);
-    else paged_attn_kernel<D, kFour, 4><<<streams, 256, 0, st>>>(a);
+    paged_attn_kernel<D, kFour, 8, false><<<streams, 512, 0, st>>>(a);
     return launch_status("paged_attention");
   }
   SPX_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, SPX_EINVAL,
@@ -1018,7 +1038,16 @@ static int launch_paged(PagedAttnArgs a, const PagedSizes& z, int waves, void* w
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
   a.parts = reinterpret_cast<u32x2*>(a.part_ml + (int64_t)2 * a.grid * kPaCols * 2);
-  paged_attn_kernel<D, kFour, 4><<<(unsigned)a.grid, 256, 0, st>>>(a);
+  const unsigned grid = (unsigned)a.grid;
+  // The half form where workgroups may run long: 64 sequences of 8192 keys (32/8 heads) 127 -> 121
+  // us; a workgroup's one unit of 32641 keys (28/4) would take 12.4 instead of 11.8, and D = 256 is
+  // as fast without it (44.1 and 44.3 us).
+  constexpr bool kCanHalve = D == 128 && kFour;
+  const int64_t units = z.streams * ((z.keys + PagedShape<D, kFour, 4>::kUnit - 1) /
+                                     PagedShape<D, kFour, 4>::kUnit);
+  if (kCanHalve && a.cols <= kPaCols / 2 && units >= (int64_t)8 * a.grid)
+    paged_attn_kernel<D, kFour, 4, kCanHalve><<<grid, 256, 0, st>>>(a);
+  else paged_attn_kernel<D, kFour, 4, false><<<grid, 256, 0, st>>>(a);
   if (z.rows >= kPaWaveRows || a.batch > 65535 || a.tokens > 65535) {
     const int waves = kPaMergeThreads / kWave;
     paged_merge_rows_kernel<D><<<dim3((unsigned)((a.q_heads + waves - 1) / waves),
@@ -1043,7 +1072,7 @@ extern "C" int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* ca
   if (cache == nullptr || !paged_sizes(*cache, q_heads, max_keys, z) ||
       (cache->head_dim != 128 && cache->head_dim != 256))
     return -1;
-  const int grid = paged_plan_of(z, cache->head_dim, cache->key_scales != nullptr).grid;
+  const int grid = paged_grid_of(z, cache->head_dim, cache->key_scales != nullptr);
   return grid == 0 ? 0 : (int64_t)2 * grid * kPaCols * (cache->head_dim + 2) * 4 + z.streams * 8;
 }
 
@@ -1072,9 +1101,8 @@ extern "C" int spx_paged_attention(const spx_paged_cache* cache, const void* q,
   a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.group = q_heads / cache->kv_heads;
   a.cols = cache->tokens * a.group;
   a.col_tiles = (a.cols + kPaCols - 1) / kPaCols;
-  const PagedPlan plan = paged_plan_of(z, cache->head_dim, four);
-  a.grid = plan.grid;
-  a.inv_grid = 1.0 / std::max(plan.grid, 1);
+  a.grid = paged_grid_of(z, cache->head_dim, four);
+  a.inv_grid = 1.0 / std::max(a.grid, 1);
   a.inv_group = 1.0 / a.group;
   a.scale_log2 = scale == 0 ? 1.0f : (float)(std::abs((double)scale) * 1.4426950408889634);
   a.q_keep = scale == 0 ? 0 : 0xffffffffu;
@@ -1083,8 +1111,8 @@ extern "C" int spx_paged_attention(const spx_paged_cache* cache, const void* q,
   a.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 128)
-    return four ? launch_paged<128, true>(a, z, plan.waves, workspace, st)
-                : launch_paged<128, false>(a, z, plan.waves, workspace, st);
-  return four ? launch_paged<256, true>(a, z, plan.waves, workspace, st)
-              : launch_paged<256, false>(a, z, plan.waves, workspace, st);
+    return four ? launch_paged<128, true>(a, z, workspace, st)
+                : launch_paged<128, false>(a, z, workspace, st);
+  return four ? launch_paged<256, true>(a, z, workspace, st)
+              : launch_paged<256, false>(a, z, workspace, st);
 }

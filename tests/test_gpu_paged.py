@@ -220,7 +220,9 @@ def test_attention_pages(gpu, page, bits):
 @pytest.mark.parametrize("bits", (16, 4))
 @pytest.mark.parametrize("batch,layout,keys,tokens", ((1, (4, 2, 128), 70001, 1),
                                                       (1, (2, 1, 256), 40003, 2),
-                                                      (40, (8, 8, 128), 1900, 1)))
+                                                      (40, (8, 8, 128), 1900, 1),
+                                                      (6, (16, 16, 128), 12000, 2),
+                                                      (5, (24, 3, 128), 66000, 1)))
 def test_attention_long_and_wide(gpu, batch, layout, keys, tokens, bits):
     starts = tuple(max(0, keys - tokens - 41 * b) for b in range(batch))
     s = ref.make(13, batch, tokens, *layout, 64, -(-keys // 64), starts, bits=bits, sharp=4.0,
