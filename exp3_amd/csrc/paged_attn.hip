@@ -305,10 +305,22 @@ __device__ __forceinline__ float max_over_rows(float x) {
   return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-// Dims of the lane c in a V row and an O register.
-template <int D, bool kFour>
+// Dims of the lane c in a V row and an O register: D / 16 consecutive ones.
+template <int D>
 __device__ __forceinline__ int value_dim(int c, int i) {
-  return kFour ? D / 16 * c + i : 128 * (i / 8) + 8 * c + i % 8;
+  return D / 16 * c + i;
+}
+
+// Partial results keep the lanes' groups of four dims side by side (in the order of the dims, 16
+// bytes every D / 4 from lane to lane, writing them to LDS met its banks four times): at `place`
+// (a multiple of 4) are the dims from here on.
+template <int D>
+__device__ __forceinline__ int place_of(int c, int i) {
+  return 4 * (16 * (i / 4) + c);
+}
+template <int D>
+__device__ __forceinline__ int dim_at(int place) {
+  return value_dim<D>(place / 4 % 16, place / 64 * 4);
 }
 
 // One KV head of the page arrays.
@@ -392,7 +404,7 @@ struct ValueTile {                       // a lane's dims of four rows of V: 4 g
     } else {
 #pragma unroll
       for (int x = 0; x < D / 128; ++x) {
-        const u32x4 w = global_load<u32x4>(p, at * 2 * D + 256 * x + 16 * c);
+        const u32x4 w = global_load<u32x4>(p, at * 2 * D + D / 8 * c + 16 * x);
 #pragma unroll
         for (int e = 0; e < 4; ++e) raw[r][4 * x + e] = w[e];
       }
@@ -762,7 +774,7 @@ paged_attn_kernel(PagedAttnArgs args) {
         if (c == 0) part_l[w][4 * g + r] = acc.l[r];
 #pragma unroll
         for (int i = 0; i < D / 16; i += 4)
-          *reinterpret_cast<f32x4*>(&part_o[w][4 * g + r][value_dim<D, kFour>(c, i)]) =
+          *reinterpret_cast<f32x4*>(&part_o[w][4 * g + r][place_of<D>(c, i)]) =
               f32x4{acc.o[i][r], acc.o[i + 1][r], acc.o[i + 2][r], acc.o[i + 3][r]};
       }
       // an infinite value and a part of P that is 0 make NaN: those again, with P as it is
@@ -774,7 +786,7 @@ paged_attn_kernel(PagedAttnArgs args) {
           for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-              float& held = part_o[w][4 * g + r][value_dim<D, kFour>(c, i)];
+              float& held = part_o[w][4 * g + r][place_of<D>(c, i) + i % 4];
               if (held != held) held = acc.o[i][r];
             }
         }
@@ -818,7 +830,7 @@ paged_attn_kernel(PagedAttnArgs args) {
         u32x2 packed;
         packed[0] = pack_bf16x2(v[0] * inv, v[1] * inv);
         packed[1] = pack_bf16x2(v[2] * inv, v[3] * inv);
-        *reinterpret_cast<u32x2*>(a.out + row * D + d) = packed;
+        *reinterpret_cast<u32x2*>(a.out + row * D + dim_at<D>(d)) = packed;
         if (d == 0 && a.lse) a.lse[row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
       } else {
         *reinterpret_cast<f32x4*>(a.part_o + ((int64_t)slot * kPaCols + col) * D + d) = v;
@@ -917,7 +929,7 @@ __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_rows_kernel(Paged
         for (int y = 0; y < 4; ++y) acc[y] += xor32(acc[y]);
       const float inv = top == -INFINITY && sum == 0.0f ? 0.0f : 1.0f / sum;
       if (gr == 0)
-        *reinterpret_cast<u32x2*>(a.out + r.row * D + dim) =
+        *reinterpret_cast<u32x2*>(a.out + r.row * D + dim_at<D>(dim)) =
             u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
       if (lane == 0 && a.lse) a.lse[r.row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
     }
@@ -980,7 +992,9 @@ __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnA
       x += acc_s[g][2 * tid];
       y += acc_s[g][2 * tid + 1];
     }
-    *reinterpret_cast<uint32_t*>(a.out + r.row * D + d0 + 2 * tid) = pack_bf16x2(x * inv, y * inv);
+    const int place = d0 + 2 * tid;
+    *reinterpret_cast<uint32_t*>(a.out + r.row * D + dim_at<D>(place) + place % 4) =
+        pack_bf16x2(x * inv, y * inv);
   }
   if (tid == 0 && d0 == 0 && a.lse) a.lse[r.row] = (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
