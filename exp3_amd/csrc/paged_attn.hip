@@ -942,7 +942,7 @@ constexpr int kPaMergeDims = 64;
 
 template <int D>
 __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnArgs a) {
-  constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaMergeThreads / kLanes;
+  constexpr int kLanes = kPaMergeDims / 4, kGroups = kPaMergeThreads / kLanes, kEarly = 4;
   __shared__ float weight[kPaMaxGrid];
   __shared__ float red[2][kPaMergeThreads / 64];
   __shared__ __align__(16) float acc_s[kGroups][kPaMergeDims];
@@ -956,6 +956,13 @@ __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnA
     return;
   }
   if (r.parts <= 1) return;
+  // a thread's first partials are under way while the weights are formed
+  f32x4 early[kEarly];
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int x = min(gr + kGroups * k, r.parts - 1);
+    early[k] = *reinterpret_cast<const f32x4*>(a.part_o + (int64_t)r.slot(x) * D + dim);
+  }
   float top = -INFINITY;
   for (int x = tid; x < r.parts; x += kPaMergeThreads)
     top = fmaxf(top, a.part_ml[(int64_t)r.slot(x) * 2]);
@@ -975,8 +982,15 @@ __global__ __launch_bounds__(kPaMergeThreads) void paged_merge_kernel(PagedAttnA
   if (lane == 0) red[1][w] = sum;
   block_sync();
   f32x4 acc{};
+#pragma unroll
+  for (int k = 0; k < kEarly; ++k) {
+    const int x = gr + kGroups * k;
+    if (x < r.parts)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[y] += weight[x] * early[k][y];
+  }
 #pragma unroll 4
-  for (int x = gr; x < r.parts; x += kGroups) {
+  for (int x = gr + kGroups * kEarly; x < r.parts; x += kGroups) {
     const f32x4 po = *reinterpret_cast<const f32x4*>(a.part_o + (int64_t)r.slot(x) * D + dim);
 #pragma unroll
     for (int y = 0; y < 4; ++y) acc[y] += weight[x] * po[y];
