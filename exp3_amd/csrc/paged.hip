@@ -33,6 +33,8 @@ int paged_map(PagedMap& m, const spx_paged_cache* cache) {
   SPX_REQUIRE(z.batch > 0 && z.tokens > 0 && z.kv_heads > 0 && z.pages > 0 && z.table_width > 0,
               SPX_EINVAL, "bad shape: batch %d tokens %d kv_heads %d pages %d table width %d",
               z.batch, z.tokens, z.kv_heads, z.pages, z.table_width);
+  SPX_REQUIRE(z.kv_heads <= 1 << 16, SPX_EINVAL, "%d KV heads are more than 2^16", z.kv_heads);
+  SPX_REQUIRE(z.reserved == 0, SPX_EINVAL, "reserved must be 0");
   SPX_REQUIRE((int64_t)z.table_width * z.page_size <= (1 << 30), SPX_EINVAL,
               "a table of %d pages of %d tokens exceeds 2^30 positions", z.table_width,
               z.page_size);
@@ -453,8 +455,7 @@ extern "C" int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void*
   a.batch = cache->batch;
   a.tokens = cache->tokens;
   a.kv_heads = cache->kv_heads;
-  SPX_REQUIRE(a.kv_heads <= 1 << 19 && a.tokens <= 1 << 24, SPX_EINVAL,
-              "more than 2^19 heads or 2^24 tokens in a call");
+  SPX_REQUIRE(a.tokens <= 1 << 24, SPX_EINVAL, "more than 2^24 tokens in a call");
   a.wave_shift = token_waves((int64_t)a.batch * a.tokens, 2 * a.kv_heads, cache->head_dim);
   const bool streamed =
       (int64_t)a.batch * a.tokens * 2 * a.kv_heads * cache->head_dim * 2 >= kStreamedBytes;

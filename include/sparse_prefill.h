@@ -350,7 +350,7 @@ typedef struct spx_paged_cache {
   int32_t table_width;
   int32_t pages;
   int32_t page_size;
-  int32_t kv_heads;
+  int32_t kv_heads;          /* at most 2^16 */
   int32_t head_dim;
   int32_t batch;
   int32_t tokens;

@@ -249,6 +249,71 @@ def test_attention_empty_rows(gpu, bits):
     _check_attention(s, 0.1)
 
 
+@pytest.mark.parametrize("bits", (16, 4))
+def test_attention_more_sequences_than_lanes(gpu, bits):
+    """The units of 150 sequences, free slots and padding among them, are found over three scans."""
+    starts = tuple(-1 if b % 7 == 3 else 37 * b % 1900 for b in range(150))
+    counts = tuple(b % 4 for b in range(150))
+    s = ref.make(24, 150, 3, 6, 3, 128, 128, 15, starts, counts, bits=bits, spare=0)
+    _check_attention(s, 0.1)
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+def test_attention_of_66000_sequences(gpu, bits):
+    """More sequences than a grid has rows, in both forms (eight waves per stream; shared units),
+    and as many appended and read back: every fifth one is the same."""
+    s = ref.make(25, 5, 1, 2, 1, 128, 64, 10, (600, 0, -1, 63, 311), bits=bits)
+    want, want_lse, off, lse_off = (x.cuda() for x in ref.attention(s, 0.1))
+    cache, table, starts, _ = ref.on_gpu(s)
+    many = [x.repeat(13200, *([1] * (x.dim() - 1))) for x in (s.q.cuda(), table, starts)]
+    for bound in (None, 601):
+        out, lse = paged.paged_attention(many[0], cache, *many[1:], 0.1, max_keys=bound,
+                                         return_lse=True)
+        out, lse = out.view(13200, 5, 1, 2, 128).double(), lse.view(13200, 5, 1, 2).double()
+        assert ((out - want).abs() <= 2.0 ** -8 * want.abs() + off).all()
+        assert ((lse == want_lse) | ((lse - want_lse).abs() <= lse_off)).all()
+    k, _ = paged.gather_tokens(cache, many[1], many[2], 1)
+    few, _ = paged.gather_tokens(cache, table, starts, 1)
+    assert (k.view(13200, *few.shape) == few).all()
+    q, k = paged.append_tokens(cache, many[1], torch.full_like(many[2], -1), k, k, many[0],
+                               return_keys=True)
+    assert not q.any() and not k.any()
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+def test_attention_of_a_long_chunk(gpu, bits):
+    """Many column tiles of one stream, each with keys of its own."""
+    s = ref.make(26, 2, 150, 7, 1, 128, 32, 10, (0, 130), (150, 77), bits=bits)
+    _check_attention(s, 0.1)
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+def test_pages_past_32_bit_offsets(gpu, bits):
+    """The same tokens in the first and in the last pages of a cache of more than 4 GiB an array."""
+    pages = 20000 if bits == 16 else 76000
+    cache = paged.empty_pages(pages, 128, 8, 128, "cuda", four_bit=bits == 4)
+    assert cache.key_pages.numel() * cache.key_pages.element_size() > 1 << 32
+    gen = torch.Generator("cuda").manual_seed(5)
+    q, k, v = (torch.randn(1, 700, h, 128, generator=gen, device="cuda").to(torch.bfloat16)
+               for h in (16, 8, 8))
+    start = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rope = paged.rope_table(768, 128, device="cuda")
+    seen = []
+    for first in (0, pages - 6):
+        table = torch.arange(first, first + 6, dtype=torch.int32, device="cuda")[None]
+        turned, _ = paged.append_tokens(cache, table, start, k, v, q, rope)
+        held = paged.gather_tokens(cache, table, start, 700)
+        out = paged.paged_attention(turned[:, -1:].contiguous(), cache, table, start + 699, 0.1)
+        seen.append((turned, *held, out))
+    assert all(torch.equal(a, b) for a, b in zip(*seen))
+    if bits == 16:
+        assert torch.equal(seen[0][2], v)
+    # the last pages were written, not the first ones again
+    cache.key_pages[:6] = 0
+    cache.value_pages[:6] = 0
+    assert torch.equal(paged.gather_tokens(cache, table, start, 700)[1], seen[0][2])
+
+
 @pytest.mark.parametrize("scale", (-0.2, 0.0, 3.0))
 @pytest.mark.parametrize("bits", (16, 4))
 def test_attention_scales(gpu, scale, bits):

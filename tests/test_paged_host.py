@@ -16,9 +16,9 @@ ODD = bytes((ctypes.c_int64 * 4)(4096, 512, 132, 1))
 
 
 def _cache(pages=(FAKE, FAKE, 0, 0), table=FAKE, starts=FAKE, counts=0, stride=32, width=32, held=64,
-           page_size=128, kv_heads=4, dim=128, batch=2, tokens=1):
+           page_size=128, kv_heads=4, dim=128, batch=2, tokens=1, reserved=0):
     return struct.pack("7Pq8i", *pages, table, starts, counts, stride, width, held, page_size,
-                       kv_heads, dim, batch, tokens, 0)
+                       kv_heads, dim, batch, tokens, reserved)
 
 
 def _append(cache=None, q=FAKE, k=FAKE, ks=S4, q_heads=28, cos=FAKE, sin=FAKE, rope=(4096, 128, 0),
@@ -44,6 +44,7 @@ def test_shared_arguments(call):
     assert call(dim=64) == unsupported
     assert call(batch=0) == call(tokens=0) == call(kv_heads=0) == call(held=0) == invalid
     assert call(table=0) == call(width=0) == call(starts=0) == invalid
+    assert call(kv_heads=(1 << 16) + 4) == call(reserved=1) == invalid
     assert call(width=(1 << 23) + 1) == invalid                   # 2^30 + 128 positions
     for pages in ((0, FAKE, 0, 0), (FAKE, OFF, 0, 0), (FAKE, FAKE, FAKE, 0),
                   (FAKE, FAKE, FAKE, FAKE + 4)):
@@ -70,6 +71,8 @@ def test_gather_and_attention_arguments():
     assert _attention(q=None) == _attention(q=OFF) == _attention(qs=ODD) == invalid
     assert _attention(out=None) == _attention(max_keys=-1) == _attention(workspace=None) == invalid
     assert _attention(q_heads=27) == _attention(batch=1 << 16, tokens=1 << 10, q_heads=32) == invalid
+    # units of 128 keys are counted in 32 bits: 2^23 of a table's reach for 256 streams
+    assert _attention(width=1 << 23, batch=64) == invalid and b"bad shape" in _lib.load().spx_last_error()
     size = _lib.load().spx_paged_attention_workspace_bytes
     assert size(_cache(), 28, 0) > 0 and size(_cache(), 28, 100) == 0
     assert size(None, 28, 0) == size(_cache(), 27, 0) == size(_cache(), 28, -1) == -1
