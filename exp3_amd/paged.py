@@ -21,7 +21,8 @@ A new token is live if its sequence is not a free slot, it is no padding, and th
 reaches its position. Positions whose page id is outside the cache have no place: nothing is
 stored for them and they are not seen. Nothing here reads these values on the host, so every
 call can be captured in a HIP graph and replayed with other lengths. There is no backward
-pass.
+pass: tensors that require a gradient are refused while gradients are recorded. q, k and v do
+not overlap the cache's memory, nor do its tensors each other's.
 """
 
 from __future__ import annotations
@@ -147,9 +148,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
 
     q: bf16 ``[B, T, Hq, D]`` (rotated); token i of sequence b sees positions
     ``0 .. starts[b] + i`` -> bf16 ``[B, T, Hq, D]``, with ``return_lse`` also the natural-log
-    LSE, fp32 ``[B, T, Hq]``. Tokens that are not live, or see nothing, give 0 and -inf.
-    ``max_keys``: an upper bound of ``starts[b] + T`` where the caller has one; it only chooses
-    how the work is divided. Meant for decode steps and a few drafted tokens: each 16 of the
-    T x Hq / Hkv rows of a KV head read K and V anew."""
+    LSE, fp32 ``[B, T, Hq]``. Tokens that are not live, see nothing, or have no score above -inf
+    give 0 and -inf. ``max_keys``: an upper bound of ``starts[b] + T`` where the caller has one;
+    it only chooses how the work is divided. Meant for decode steps and a few drafted tokens:
+    each 16 of the T x Hq / Hkv rows of a KV head read K and V anew."""
     return _run(q, "attention", cache, page_table, starts, counts, q, scale,
                 0 if max_keys is None else max_keys, return_lse)

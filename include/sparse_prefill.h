@@ -329,7 +329,8 @@ int spx_decode_attention(const void* q, const int64_t* q_strides, const void* k,
  * aligned, or (key_scales and value_scales not NULL) 4 bits:
  * [pages, kv_heads, page_size, head_dim / 2] bytes of E2M1 values (the even dim in the low
  * half) with scales [pages, kv_heads, page_size, head_dim / 32], 8-byte aligned: E8M0, byte e
- * scales by 2^(e - 127), 255 is NaN. page_size: a power of two from 16 to 1024.
+ * scales by 2^(e - 127), 255 is NaN; 0, 1, 253 and 254 are not supported (values that bf16 does
+ * not have as normal numbers). page_size: a power of two from 16 to 1024.
  * page_table: `batch` rows, table_stride elements apart, of table_width page ids. Position p of
  * sequence b is slot p % page_size of page page_table[b][p / page_size].
  * The `tokens` tokens of sequence b have positions starts[b] + i. Token i is live if
@@ -384,8 +385,8 @@ int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out, voi
  * sees positions 0 .. starts[b] + i, out = softmax(scale q K^T) V. q: bf16 [B, T, Hq, D]
  * (strides as above); out: contiguous bf16 [B, T, Hq, D]; lse: natural-log LSE, contiguous
  * fp32 [B, T, Hq], or NULL. Positions without a place are not seen. Tokens that are not live,
- * or see nothing, give 0 and an LSE of -inf. batch * kv_heads * ceil(T Hq / Hkv / 16) times
- * the table's reach / 128 must stay below 2^31. max_keys: an upper bound of starts[b] + T that
+ * see nothing, or have no score above -inf, give 0 and an LSE of -inf. batch * kv_heads *
+ * ceil(T Hq / Hkv / 16) times the table's reach / 128 must stay below 2^31. max_keys: an upper bound of starts[b] + T that
  * the caller knows, or 0; it only chooses how the work is divided. workspace: device memory
  * of spx_paged_attention_workspace_bytes(...) bytes for the same arguments (-1: unsupported
  * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after;

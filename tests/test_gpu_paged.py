@@ -553,3 +553,80 @@ def test_empty_calls_and_refusals(gpu):
                  lambda: paged.paged_attention(x.float(), cache, table, starts, 0.1)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_tensors_that_require_a_gradient(gpu):
+    """Refused while gradients are recorded, taken otherwise."""
+    cache = paged.empty_pages(8, 16, 2, 128, "cuda")
+    table = torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    starts = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.ones(1, 1, 2, 128, dtype=torch.bfloat16, device="cuda")
+    leaf = torch.ones_like(x).requires_grad_()
+    for call in (lambda y: paged.append_tokens(cache, table, starts, y, x),
+                 lambda y: paged.append_tokens(cache, table, starts, x, y),
+                 lambda y: paged.append_tokens(cache, table, starts, x, x, y),
+                 lambda y: paged.paged_attention(y, cache, table, starts, 0.1)):
+        for y in (leaf, leaf * 2):
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call(y)
+        for off in (torch.no_grad, torch.inference_mode):
+            with off():
+                call(leaf)
+                call(leaf * 2)
+        assert call(leaf.detach()) is not None
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+def test_sequences_with_a_common_prefix(gpu, bits):
+    """Pages that several sequences read, each with pages of its own behind them."""
+    s = ref.make(23, 3, 1, 8, 2, 128, 16, 20, (200, 150, 319), bits=bits)
+    s.table[1:, :9] = s.table[0, :9]
+    cache, table, starts, _ = ref.on_gpu(s)
+    want, want_lse, off, lse_off = ref.attention(s, 0.1)
+    got, lse = paged.paged_attention(s.q.cuda(), cache, table, starts, 0.1, return_lse=True)
+    assert ((got.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + off).all()
+    assert ((lse.double().cpu() - want_lse).abs() <= lse_off).all()
+
+
+@pytest.mark.parametrize("keys", (40, 700, 5000))
+def test_rows_without_a_score_above_minus_infinity(gpu, keys):
+    """Keys of -inf: such a row gives 0 and -inf where all its scores are -inf, and counts the
+    finite ones alone where some are."""
+    s = ref.make(24, 2, 1, 4, 2, 128, 16, keys // 16 + 1, (keys - 1, keys - 1), spare=0)
+    for page in s.table[0].tolist():
+        s.held[0][page, :, :, 0] = -float("inf")
+    mixed = s.table[1].tolist()
+    for page in mixed[1:]:
+        s.held[0][page, :, :, 0] = -float("inf")
+    s.q[..., 0] = 1.0
+    cache, table, starts, _ = ref.on_gpu(s)
+    got, lse = paged.paged_attention(s.q.cuda(), cache, table, starts, 0.1, return_lse=True)
+    assert not got[0].any() and torch.equal(lse[0], torch.full_like(lse[0], -float("inf")))
+    alone, alone_lse = paged.paged_attention(s.q[1:].cuda(), cache, table[1:], starts[1:] * 0 + 15,
+                                             0.1, return_lse=True)
+    # the same 16 keys, joined with empty parts: both round to bf16, and weights of 1 are exact
+    assert torch.equal(got[1:], alone) and torch.equal(lse[1:], alone_lse)
+
+
+def test_graphs_that_share_a_pool(gpu):
+    """Two captured calls whose workspaces may be the same memory, replayed in turn."""
+    calls = []
+    for seed, bits, lengths in ((25, 16, (3000, 900)), (26, 4, (700, 5100))):
+        s = ref.make(seed, 2, 1, 28, 4, 128, 64, 80, lengths, bits=bits, spare=0)
+        cache, table, starts, _ = ref.on_gpu(s)
+        calls.append((s.q.cuda(), cache, table, starts, 0.1))
+    want = [paged.paged_attention(*call) for call in calls]
+    torch.cuda.synchronize()
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for call in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            out = paged.paged_attention(*call)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, out), expected in zip(graphs, want):
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, expected)
+        assert torch.equal(paged.paged_attention(*calls[0]), want[0])
