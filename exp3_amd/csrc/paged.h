@@ -13,6 +13,11 @@ namespace spx {
 constexpr int kPagedGroup = 32;          // dims per scale of a 4-bit page
 constexpr int kPagedMinPage = 16, kPagedMaxPage = 1024;
 
+// Device data that no kernel of the stream writes meanwhile, at a uniform address.
+__device__ __forceinline__ int scalar_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
 // Which tokens a call is about and where they are: token i of sequence b has position
 // starts[b] + i and is live if starts[b] >= 0, i < counts[b] (counts may be null) and the
 // position is within the table.
@@ -24,12 +29,17 @@ struct PagedMap {
   int width, pages, page_shift, kv_heads;
 
   __device__ __forceinline__ int64_t capacity() const { return (int64_t)width << page_shift; }
-  // Position of token i of sequence b, or -1.
+  // Position of token i of sequence b, or -1; b and i are uniform.
   __device__ __forceinline__ int position(int b, int i) const {
-    const int start = starts[b];
-    if (start < 0 || (counts != nullptr && i >= counts[b])) return -1;
+    const int start = scalar_load(starts + b);
+    const int count = counts != nullptr ? scalar_load(counts + b) : i + 1;
     const int64_t p = (int64_t)start + i;
-    return p < capacity() ? (int)p : -1;
+    return start >= 0 && i < count && p < capacity() ? (int)p : -1;
+  }
+  // Page of a position, the same for all lanes, or -1 also for position -1.
+  __device__ __forceinline__ int uniform_page(int b, int p) const {
+    const int id = scalar_load(table + b * table_stride + (max(p, 0) >> page_shift));
+    return p >= 0 && (unsigned)id < (unsigned)pages ? id : -1;
   }
   // Page of a position, or -1 where the table names none.
   __device__ __forceinline__ int page(int b, int p) const {

@@ -88,11 +88,6 @@ __device__ __forceinline__ float part_weight(float m, float top) {
 
 // ---------------------------------------------------------------- division of the work
 
-// Device data that no kernel of the stream writes meanwhile, at a uniform address.
-__device__ __forceinline__ int scalar_load(const int32_t* p) {
-  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
-}
-
 // n / d for n >= 0, inv = 1.0 / d: the quotient is off by one at most before it is put right. (An
 // integer division takes some 40 dependent instructions.)
 __device__ __forceinline__ int divide(int n, int d, double inv) {

@@ -630,3 +630,40 @@ def test_graphs_that_share_a_pool(gpu):
             torch.cuda.synchronize()
             assert torch.equal(out, expected)
         assert torch.equal(paged.paged_attention(*calls[0]), want[0])
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+@pytest.mark.parametrize("layout", ((28, 4, 128), (16, 4, 256)))
+def test_calls_larger_than_the_caches(gpu, layout, bits):
+    """One call of 400 MB and more, with padding, against calls of a few tokens each."""
+    q_heads, kv_heads, dim = layout
+    heads, total, part, live = (q_heads, kv_heads, kv_heads), 28000, 875, 27001
+    gen = torch.Generator("cuda").manual_seed(27)
+    x = torch.randn(1, total, sum(heads), dim, generator=gen, device="cuda").to(torch.bfloat16)
+    rope = paged.rope_table(28032, dim // 2, device="cuda")
+    table = torch.randperm(500, generator=gen, device="cuda")[None, :438].int()
+    start, count = (torch.tensor([n], dtype=torch.int32, device="cuda") for n in (3, live))
+    one, many = (paged.PagedCache(*(None if t is None else t.zero_() for t in (
+        c.key_pages, c.value_pages, c.key_scales, c.value_scales))) for c in (
+            paged.empty_pages(500, 64, kv_heads, dim, "cuda", four_bit=bits == 4) for _ in range(2)))
+    q, k = paged.append_tokens(one, table, start, *x.split(heads, 2)[1:], x[:, :, :q_heads], rope,
+                               count, return_keys=True)
+    for at in range(0, total, part):
+        few = x[:, at:at + part].split(heads, 2)
+        few_q, few_k = paged.append_tokens(many, table, start + at, *few[1:], few[0], rope,
+                                           count - at, return_keys=True)
+        assert torch.equal(q[:, at:at + part], few_q) and torch.equal(k[:, at:at + part], few_k)
+    assert not q[:, live:].any() and not k[:, live:].any() and q[:, :live].any()
+    assert torch.equal(one.key_pages, many.key_pages)
+    assert torch.equal(one.value_pages, many.value_pages)
+    if bits == 4:
+        assert torch.equal(one.key_scales, many.key_scales)
+        assert torch.equal(one.value_scales, many.value_scales)
+    # read back in one call of as many bytes
+    times = 8
+    rows, starts = table.repeat(times, 1), start.repeat(times)
+    whole = paged.gather_tokens(one, rows, starts, total, count.repeat(times))
+    for at in range(0, total, part):
+        few = paged.gather_tokens(one, table, start + at, part, count - at)
+        for got, want in zip(whole, few):
+            assert torch.equal(got[:, at:at + part], want.expand(times, -1, -1, -1))
