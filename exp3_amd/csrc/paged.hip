@@ -95,11 +95,13 @@ __device__ __forceinline__ double fma_of(double x, double y, double z) {
   return __builtin_fma(x, y, z);
 }
 
-// A call that reads and writes more than the 256 MB last-level cache holds, and half as much
-// again, stores its outputs past the caches: 24000 tokens (28/4 heads, bf16; 442 MB) 90 -> 86 us,
-// 32640 120 -> 114, 4 x 16000 read back 96 -> 92. Below that they stay there for whoever reads them:
-// 16000 tokens (295 MB) as fast, 8000 29 against 31, 4 x up to 12001 read back 50 against 54.
-constexpr int64_t kStreamedBytes = 384 << 20;
+// Calls that read and write 8 MB and more store their outputs past the caches. Into memory that an
+// earlier call of the program used, as an allocator gives it: 4 x up to 2113 tokens appended in 4 bits
+// and read back 42 -> 30 us, 4 x up to 12001 read back 58 -> 49; into memory of each call's own, six in
+// turn: 32640 tokens appended 120 -> 114, 16000 as fast, 8000 29 -> 31. A dense prefill behind the
+// append takes as long in all (16000 tokens 1632 and 1632 us, 1089 43.6 and 42.8). What a decode step
+// writes is read at once and stays: attention behind it 36.3 us with it in the cache, 37.1 past it.
+constexpr int64_t kStreamedBytes = 8 << 20;
 
 // (A template parameter: of a run-time choice the compiler makes one ordinary store.)
 template <bool kStreamed>
