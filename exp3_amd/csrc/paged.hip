@@ -234,8 +234,8 @@ __global__ __launch_bounds__(kPagedThreads, kFour ? 6 : 1) void paged_append_ker
   const int chunks = q_chunks + 2 * kv_chunks, step = 1 << a.wave_shift;
   const int sub = lane / kPieces;
   const int from = lane - piece + Rotation::partner(a, d0) / 8;  // the lane of the paired dims
-  const int b = blockIdx.z * gridDim.y + blockIdx.y;
-  if (b >= a.batch || part >= chunks) return;
+  const unsigned b = blockIdx.z * gridDim.y + blockIdx.y;
+  if (b >= (unsigned)a.batch || part >= chunks) return;
   const auto head_of = [&](int chunk, int heads) { return min(chunk * kRows + sub, heads - 1); };
   const auto load = [&](int n) {       // chunks of v, of k, of q
     const bool is_v = n < kv_chunks, is_k = !is_v && n < 2 * kv_chunks;
@@ -369,8 +369,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_gather_kernel(GatherArgs 
   if (i >= a.tokens) return;
   const int rows = 2 * a.kv_heads, step = kRows << a.wave_shift;
   const int first = part * kRows + lane / kPieces;
-  const int b = blockIdx.z * gridDim.y + blockIdx.y;
-  if (b >= a.batch) return;
+  const unsigned b = blockIdx.z * gridDim.y + blockIdx.y;
+  if (b >= (unsigned)a.batch) return;
   const int p = a.map.position(b, i), page = a.map.uniform_page(b, p);
   const int64_t token = (int64_t)b * a.tokens + i;
   StoredPart<D, kFour> next;

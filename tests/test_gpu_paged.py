@@ -667,3 +667,20 @@ def test_calls_larger_than_the_caches(gpu, layout, bits):
         few = paged.gather_tokens(one, table, start + at, part, count - at)
         for got, want in zip(whole, few):
             assert torch.equal(got[:, at:at + part], want.expand(times, -1, -1, -1))
+
+
+def test_append_for_66000_sequences(gpu):
+    """More sequences than a grid has rows, each with a page of its own: what is read back is what
+    was appended."""
+    batch = 66000
+    gen = torch.Generator("cuda").manual_seed(28)
+    cache = paged.empty_pages(batch, 16, 1, 128, "cuda")
+    table = torch.randperm(batch, generator=gen, device="cuda")[:, None].int()
+    starts = torch.arange(batch, dtype=torch.int32, device="cuda") % 17 - 1      # some free
+    k, v = (torch.randn(batch, 1, 1, 128, generator=gen, device="cuda").to(torch.bfloat16)
+            for _ in range(2))
+    _, rotated = paged.append_tokens(cache, table, starts, k, v, return_keys=True)
+    live = (starts >= 0)[:, None, None, None]
+    assert torch.equal(rotated, k * live)
+    key, value = paged.gather_tokens(cache, table, starts, 1)
+    assert torch.equal(key, k * live) and torch.equal(value, v * live)
