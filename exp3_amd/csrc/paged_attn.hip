@@ -26,10 +26,12 @@
 //     v_cvt_scalef32_pk_bf16_fp4 (two values and their scale an instruction).
 //   * P V: v_mfma_f32_16x16x32_bf16 over the keys of two tiles. Their scores lie in the lane as
 //     the A operand wants them; a lane holds its dims of the eight rows it needs, and byte
-//     permutes pair the keys. P is split into two bf16 parts (2^-16 left over, below the
-//     output's rounding; one part alone would add as much error as that rounding). Its sums
-//     are products with ones. Where that makes NaN (infinite values of bf16 pages meet a part
-//     of P that is 0) the wave runs again with P as it is, v_mfma_f32_16x16x4_f32.
+//     permutes pair the keys. P goes through in three bf16 parts, 24 bits as in fp32, and its sums
+//     are products of the same parts with ones: products and LSE are those of an fp32 P. (Two parts
+//     leave 2^-18: an LSE off by up to 2^-17, which no rounding of the output covers. The third
+//     costs 2 to 6 % with 4-bit pages, 64 sequences of 8192 keys 114 -> 121 us, 131072 keys 25.3 ->
+//     26.8, and nothing with bf16 pages.) Where that makes NaN (infinite values of bf16 pages meet a
+//     part of P that is 0) the wave runs again with P as it is, v_mfma_f32_16x16x4_f32.
 //   * The running maximum is raised, and O scaled, only in steps where it grows.
 #include <algorithm>
 #include <cmath>
@@ -459,13 +461,14 @@ struct Limits {
 
 // A wave's tiles of a stream: page ids, keys and values of one unit, O and the softmax state.
 // kHalf (4-bit pages): at most eight columns; column c + 8 is column c again, and holds the second
-// part of its P in the products with V (the halves of O are added in the end), which saves half
-// of these.
+// part of its P in the products with V (the halves of O are added in the end): two of these
+// instead of three.
 template <int D, bool kFour, int W, bool kHalf>
 struct Wave {
   using Shape = PagedShape<D, kFour, W>;
   using Pages = HeadPages<D, kFour>;
   static constexpr int T = Shape::kTiles, KK = D / 32, N = D / 16;
+  static constexpr int kParts = kHalf ? 2 : 3;             // operands that hold P
   KeyTile<D, kFour> key[T];
   ValueTile<D, kFour> value[T];
   f32x4 o[N];                            // [query row 4 g + r][value_dim(c, i)]
@@ -610,20 +613,30 @@ struct Wave {
     } else {
 #pragma unroll
       for (int t = 0; t < T; t += 2) {
-        u32x4 hi, lo;                    // kHalf: hi holds the one or the other
-        const uint32_t second = c < kPaCols / 2 ? 0 : ~0u;
+        // Three bf16 parts hold the 24 bits of an fp32 probability. kHalf: the first of column c and
+        // the second of column c + 8 are one operand, the third and zeros the other.
+        u32x4 part[kParts];
+        const uint32_t upper = c < kPaCols / 2 ? 0 : ~0u;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float u = x[t + e / 2][2 * (e % 2)], w = x[t + e / 2][2 * (e % 2) + 1];
-          const uint32_t first_part = opaque_bits(pack_bf16x2(u, w));
-          const uint32_t off = kHalf ? first_part & second : first_part;
-          const uint32_t rest = pack_bf16x2(u - bf16_lo(off), w - bf16_hi(off));
-          hi[e] = kHalf ? rest : first_part;
-          lo[e] = rest;
+          float u = x[t + e / 2][2 * (e % 2)], w = x[t + e / 2][2 * (e % 2) + 1];
+          const uint32_t p1 = opaque_bits(pack_bf16x2(u, w));
+          u -= bf16_lo(p1);
+          w -= bf16_hi(p1);
+          const uint32_t p2 = opaque_bits(pack_bf16x2(u, w));
+          const uint32_t p3 = pack_bf16x2(u - bf16_lo(p2), w - bf16_hi(p2));
+          if constexpr (kHalf) {
+            part[0][e] = (p1 & ~upper) | (p2 & upper);
+            part[1][e] = p3 & ~upper;
+          } else {
+            part[0][e] = p1;
+            part[1][e] = p2;
+            part[2][e] = p3;
+          }
         }
         const uint32_t ones = 0x3f803f80u;
-        l = mfma16(hi, u32x4{ones, ones, ones, ones}, l);
-        if constexpr (!kHalf) l = mfma16(lo, u32x4{ones, ones, ones, ones}, l);
+#pragma unroll
+        for (const auto& p : part) l = mfma16(p, u32x4{ones, ones, ones, ones}, l);
 #pragma unroll
         for (int y = 0; y < N / 2; ++y) {
           uint32_t row[8];
@@ -635,11 +648,10 @@ struct Wave {
             even[e] = __builtin_amdgcn_perm(row[2 * e + 1], row[2 * e], 0x05040100u);
             odd[e] = __builtin_amdgcn_perm(row[2 * e + 1], row[2 * e], 0x07060302u);
           }
-          o[2 * y] = mfma16(hi, even, o[2 * y]);
-          o[2 * y + 1] = mfma16(hi, odd, o[2 * y + 1]);
-          if constexpr (!kHalf) {
-            o[2 * y] = mfma16(lo, even, o[2 * y]);
-            o[2 * y + 1] = mfma16(lo, odd, o[2 * y + 1]);
+#pragma unroll
+          for (const auto& p : part) {
+            o[2 * y] = mfma16(p, even, o[2 * y]);
+            o[2 * y + 1] = mfma16(p, odd, o[2 * y + 1]);
           }
         }
       }
@@ -1067,9 +1079,9 @@ static int launch_paged(PagedAttnArgs a, const PagedSizes& z, void* workspace, h
   a.part_ml = a.part_o + (int64_t)2 * a.grid * kPaCols * D;
   a.parts = reinterpret_cast<u32x2*>(a.part_ml + (int64_t)2 * a.grid * kPaCols * 2);
   const unsigned grid = (unsigned)a.grid;
-  // The half form where workgroups may run long: 64 sequences of 8192 keys (32/8 heads) 127 -> 121
-  // us; a workgroup's one unit of 32641 keys (28/4) would take 12.4 instead of 11.8, and D = 256 is
-  // as fast without it (44.1 and 44.3 us).
+  // The half form where workgroups may run long: 64 sequences of 8192 keys (32/8 heads) 123 -> 121
+  // us; with two parts of P a workgroup's one unit of 32641 keys (28/4) took 12.4 instead of 11.8 in
+  // it, and D = 256 was as fast without it (44.1 and 44.3 us).
   constexpr bool kCanHalve = D == 128 && kFour;
   const int64_t units = z.streams * ((z.keys + PagedShape<D, kFour, 4>::kUnit - 1) /
                                      PagedShape<D, kFour, 4>::kUnit);
