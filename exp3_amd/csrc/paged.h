@@ -41,9 +41,10 @@ struct PagedMap {
     const int id = scalar_load(table + b * table_stride + (max(p, 0) >> page_shift));
     return p >= 0 && (unsigned)id < (unsigned)pages ? id : -1;
   }
-  // Page of a position, or -1 where the table names none.
-  __device__ __forceinline__ int page(int b, int p) const {
-    const int id = table[b * table_stride + (p >> page_shift)];
+  // Page of a position, or -1 where the table names none, also for position -1 (the last one of a
+  // sequence without keys), which reads nothing in front of the table.
+  __host__ __device__ __forceinline__ int page(int b, int p) const {
+    const int id = table[b * table_stride + ((p > 0 ? p : 0) >> page_shift)] | p >> 31;
     return (unsigned)id < (unsigned)pages ? id : -1;
   }
   // Row (of D elements) of a position of a KV head in the page arrays.
