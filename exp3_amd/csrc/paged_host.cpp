@@ -52,6 +52,12 @@ void require_device(const at::Tensor& x, const c10::Device& device) {
   if (x.device() != device) refuse("tensors on different devices: ", device, " and ", x.device());
 }
 
+// No gradient would reach x.
+void require_no_gradient(const at::Tensor& x, const char* name) {
+  if (x.requires_grad() && c10::GradMode::is_enabled())
+    refuse(name, " requires a gradient: the paged cache has no backward pass (torch.no_grad())");
+}
+
 int small(int64_t x, const char* name) {
   if (x > INT_MAX) refuse(name, " of ", x, " is more than 2^31 - 1");
   return (int)x;
@@ -79,6 +85,8 @@ struct Description {
              value.sizes(), " ", value.scalar_type());
     require_device(key, device);
     require_device(value, device);
+    require_no_gradient(key, "key_pages");
+    require_no_gradient(value, "value_pages");
     c.key_pages = pointer(key);
     c.value_pages = pointer(value);
     c.pages = small(key.size(0), "pages");
@@ -128,10 +136,9 @@ struct Description {
 };
 
 // A [B, T, H, D] bf16 tensor that the kernels read in place: unit dim stride, 16-byte rows, no
-// lazy negation; any other layout is copied. No gradient would reach it.
+// lazy negation; any other layout is copied.
 at::Tensor rows(const at::Tensor& x, const char* name) {
-  if (x.requires_grad() && c10::GradMode::is_enabled())
-    refuse(name, " requires a gradient: the paged cache has no backward pass (torch.no_grad())");
+  require_no_gradient(x, name);
   if (x.scalar_type() != at::kBFloat16)
     refuse("expected a bfloat16 tensor, got ", x.scalar_type(), " (", name, ")");
   if (x.dim() != 4)
@@ -246,6 +253,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
           refuse("rope must be two contiguous float32 [positions, rotary_dim // 2] tensors of one "
                  "shape, got ", x.sizes(), " ", x.scalar_type());
         require_device(x, d.device);
+        require_no_gradient(x, "rope");
         table[i] = static_cast<const float*>(pointer(x));
       }
       positions = first.size(0);

@@ -170,3 +170,18 @@ def test_reference_grid():
     assert torch.isnan(out[0, :32]).all() and torch.isnan(out[1, 32:]).all()
     assert (out[0, 32:] == 0).all() and (out[1, :32] == 0).all()
     assert ref.four_bit(torch.full((1, 32), 3.3e38, dtype=torch.float64)).max() == 6 * 2.0 ** 125
+
+
+@pytest.mark.parametrize("which", (0, 1))
+def test_pages_that_require_a_gradient(which):
+    """Refused while gradients are recorded, as q, k and v: no output would carry one."""
+    cache = paged.empty_pages(4, 16, 2, 128, "cpu")
+    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    page = (cache.key_pages, cache.value_pages)[which].requires_grad_()
+    with pytest.raises(ValueError, match="requires a gradient"):
+        _describe(cache, table, starts, None)
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            _describe(cache, table, starts, None)
+    page.requires_grad_(False)
+    _describe(cache, table, starts, None)
