@@ -16,6 +16,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -52,10 +53,12 @@ void require_device(const at::Tensor& x, const c10::Device& device) {
   if (x.device() != device) refuse("tensors on different devices: ", device, " and ", x.device());
 }
 
-// No gradient would reach x.
+// No gradient would reach x, and no tangent of x the outputs.
 void require_no_gradient(const at::Tensor& x, const char* name) {
   if (x.requires_grad() && c10::GradMode::is_enabled())
     refuse(name, " requires a gradient: the paged cache has no backward pass (torch.no_grad())");
+  if (x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse(name, " has a forward-mode tangent: the paged cache has no derivatives");
 }
 
 int small(int64_t x, const char* name) {

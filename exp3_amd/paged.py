@@ -20,9 +20,10 @@ Common arguments:
 A new token is live if its sequence is not a free slot, it is no padding, and the table
 reaches its position. Positions whose page id is outside the cache have no place: nothing is
 stored for them and they are not seen. Nothing here reads these values on the host, so every
-call can be captured in a HIP graph and replayed with other lengths. There is no backward
-pass: tensors that require a gradient are refused while gradients are recorded. q, k and v do
-not overlap the cache's memory, nor do its tensors each other's.
+call can be captured in a HIP graph and replayed with other lengths. There is no derivative in
+either mode: tensors that require a gradient are refused while gradients are recorded, and
+those that carry a forward-mode tangent. q, k and v do not overlap the cache's memory, nor do
+its tensors each other's.
 """
 
 from __future__ import annotations

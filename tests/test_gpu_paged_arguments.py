@@ -41,3 +41,31 @@ def test_rope_tables_that_require_a_gradient(gpu, which):
         paged.append_tokens(cache, table, starts, x, x, x, rope)
     with torch.no_grad():
         paged.append_tokens(cache, table, starts, x, x, x, rope)
+
+
+def test_forward_tangents(gpu):
+    """Refused wherever they come in: the outputs would carry none."""
+    cache, table, starts, x, rope = _call()
+
+    def dual(y):
+        return torch.autograd.forward_ad.make_dual(y, torch.ones_like(y))
+
+    with torch.autograd.forward_ad.dual_level():
+        paged.append_tokens(cache, table, starts, x, x, x, rope)
+        pages = paged.PagedCache(dual(cache.key_pages), cache.value_pages)
+        for call in (lambda: paged.append_tokens(cache, table, starts, dual(x), x),
+                     lambda: paged.append_tokens(cache, table, starts, x, dual(x)),
+                     lambda: paged.append_tokens(cache, table, starts, x, x, dual(x)),
+                     lambda: paged.append_tokens(cache, table, starts, x, x, x, (rope[0], dual(rope[1]))),
+                     lambda: paged.append_tokens(pages, table, starts, x, x),
+                     lambda: paged.gather_tokens(pages, table, starts, 1),
+                     lambda: paged.paged_attention(x, pages, table, starts, 0.1),
+                     lambda: paged.paged_attention(dual(x), cache, table, starts, 0.1)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.jvp(lambda y: paged.paged_attention(y, cache, table, starts, 0.1), (x,), (x,))
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.func.grad(lambda y: paged.paged_attention(y, cache, table, starts, 0.1).sum())(x)
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.vmap(lambda y: paged.paged_attention(y, cache, table, starts, 0.1))(x[None].expand(2, -1, -1, -1, -1))

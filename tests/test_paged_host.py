@@ -185,3 +185,19 @@ def test_pages_that_require_a_gradient(which):
             _describe(cache, table, starts, None)
     page.requires_grad_(False)
     _describe(cache, table, starts, None)
+
+
+@pytest.mark.parametrize("which", (0, 1))
+def test_pages_with_a_forward_tangent(which):
+    """Refused: the tangent would be dropped."""
+    cache = paged.empty_pages(4, 16, 2, 128, "cpu")
+    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    pages = [cache.key_pages, cache.value_pages]
+    with torch.autograd.forward_ad.dual_level():
+        _describe(cache, table, starts, None)
+        pages[which] = torch.autograd.forward_ad.make_dual(pages[which], torch.ones_like(pages[which]))
+        dual = paged.PagedCache(*pages)
+        with pytest.raises(ValueError, match="tangent"):
+            _describe(dual, table, starts, None)
+        pages[which] = torch.autograd.forward_ad.unpack_dual(pages[which]).primal
+        _describe(paged.PagedCache(*pages), table, starts, None)
