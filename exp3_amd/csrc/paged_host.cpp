@@ -14,10 +14,12 @@
 #include <sstream>
 #include <stdexcept>
 
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "sparse_prefill.h"
@@ -59,6 +61,19 @@ void require_no_gradient(const at::Tensor& x, const char* name) {
     refuse(name, " requires a gradient: the paged cache has no backward pass (torch.no_grad())");
   if (x._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
     refuse(name, " has a forward-mode tangent: the paged cache has no derivatives");
+}
+
+// Where torch records a graph, it records the allocation of the outputs and not the kernel that
+// fills them. (Modes that only look on may be there.)
+void require_eager() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool traced = at::tracer::impl::is_dispatch_enabled();
+  if (!traced && TorchDispatchModeTLS::any_modes_set())
+    for (auto key : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY,
+                     TorchDispatchModeKey::FUNCTIONAL})
+      traced = traced || TorchDispatchModeTLS::get_mode(key).has_value();
+  if (traced) refuse("the paged cache's functions cannot be traced into a graph");
 }
 
 int small(int64_t x, const char* name) {
@@ -199,6 +214,7 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t wanted, const Body& body) {
     return nullptr;
   }
   try {
+    require_eager();
     return body();
   } catch (const Invalid& e) {
     PyErr_SetString(PyExc_ValueError, e.what());

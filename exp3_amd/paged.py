@@ -22,8 +22,9 @@ reaches its position. Positions whose page id is outside the cache have no place
 stored for them and they are not seen. Nothing here reads these values on the host, so every
 call can be captured in a HIP graph and replayed with other lengths. There is no derivative in
 either mode: tensors that require a gradient are refused while gradients are recorded, and
-those that carry a forward-mode tangent. q, k and v do not overlap the cache's memory, nor do
-its tensors each other's.
+those that carry a forward-mode tangent. The calls are refused while torch traces a graph
+(``torch.jit.trace``, ``make_fx``, ``torch.export``); ``torch.compile`` breaks its graph at
+them. q, k and v do not overlap the cache's memory, nor do its tensors each other's.
 """
 
 from __future__ import annotations

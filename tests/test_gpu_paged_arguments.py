@@ -69,3 +69,19 @@ def test_forward_tangents(gpu):
         torch.func.grad(lambda y: paged.paged_attention(y, cache, table, starts, 0.1).sum())(x)
     with pytest.raises((ValueError, RuntimeError)):
         torch.vmap(lambda y: paged.paged_attention(y, cache, table, starts, 0.1))(x[None].expand(2, -1, -1, -1, -1))
+
+
+def test_refused_while_a_graph_is_traced(gpu):
+    """torch records the outputs' allocation and not the kernel: what was traced would return
+    uninitialised memory. A compiled function takes the calls as they are."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    cache, table, starts, x, rope = _call()
+    for step in (lambda y: paged.append_tokens(cache, table, starts, y, y, y, rope)[0],
+                 lambda y: paged.gather_tokens(cache, table, starts, 1)[0] + y,
+                 lambda y: paged.paged_attention(y, cache, table, starts, 0.1)):
+        want = step(x)
+        for trace in (lambda: torch.jit.trace(step, (x,)), lambda: make_fx(step)(x)):
+            with pytest.raises(ValueError, match="traced"):
+                trace()
+        assert torch.equal(torch.compile(step, backend="eager")(x), want)

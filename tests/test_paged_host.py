@@ -201,3 +201,29 @@ def test_pages_with_a_forward_tangent(which):
             _describe(dual, table, starts, None)
         pages[which] = torch.autograd.forward_ad.unpack_dual(pages[which]).primal
         _describe(paged.PagedCache(*pages), table, starts, None)
+
+
+def test_refused_while_a_graph_is_traced():
+    """torch records the outputs' allocation and not the kernel: what was traced would return
+    uninitialised memory."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    cache = paged.empty_pages(4, 16, 2, 128, "cpu")
+    table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+
+    def step(x):
+        _describe(cache, table, x, None)
+        return x + 1
+
+    step(starts)
+    with FlopCounterMode(display=False):          # a mode that only looks on
+        step(starts)
+    for trace in (lambda: torch.jit.trace(step, (starts,)), lambda: make_fx(step)(starts),
+                  lambda: make_fx(step, tracing_mode="fake")(starts)):
+        with pytest.raises(ValueError, match="traced"):
+            trace()
+    with FakeTensorMode(), pytest.raises(ValueError, match="traced"):
+        _describe(cache, table, starts, None)
+    step(starts)
