@@ -39,9 +39,20 @@ template <typename... Parts>
   throw Invalid(text.str());
 }
 
-const at::Tensor& tensor(PyObject* object, const char* name) {
+// Dispatch keys of tensors that are not what their storage holds: lazily zero ones, subclasses that
+// compute by themselves, those of function transforms; and lazily negated ones.
+constexpr c10::DispatchKeySet kNotPlain{
+    c10::DispatchKey::ZeroTensor,       c10::DispatchKey::Python,
+    c10::DispatchKey::Functionalize,    c10::DispatchKey::FuncTorchBatched,
+    c10::DispatchKey::FuncTorchGradWrapper};
+constexpr c10::DispatchKeySet kNegated{c10::DispatchKey::Negative};
+
+const at::Tensor& tensor(PyObject* object, const char* name, bool may_be_negated = false) {
   if (!THPVariable_Check(object)) refuse(name, " must be a tensor, got ", Py_TYPE(object)->tp_name);
-  return THPVariable_Unpack(object);
+  const at::Tensor& x = THPVariable_Unpack(object);
+  if (x.key_set().has_any(may_be_negated ? kNotPlain : kNotPlain | kNegated))
+    refuse(name, " must be a plain tensor: the kernels read its storage (clone() makes one)");
+  return x;
 }
 
 void* pointer(const at::Tensor& x) { return x.data_ptr(); }
@@ -236,8 +247,8 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t wanted, const Body& body) {
 // return_keys, stream -> (rotated q or None, rotated k or None)
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 15, [&]() -> PyObject* {
-    const at::Tensor& k_in = tensor(args[7], "k");
-    const at::Tensor& v_in = tensor(args[8], "v");
+    const at::Tensor& k_in = tensor(args[7], "k", true);
+    const at::Tensor& v_in = tensor(args[8], "v", true);
     require_gpu(k_in);
     require_gpu(v_in);
     Description d(k_in.device());
@@ -250,7 +261,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
       refuse("k ", k.sizes(), " does not fit a cache of ", d.c.kv_heads, " heads of ", d.c.head_dim);
     at::Tensor q, q_out, k_out;
     if (args[9] != Py_None) {
-      const at::Tensor& q_in = tensor(args[9], "q");
+      const at::Tensor& q_in = tensor(args[9], "q", true);
       require_gpu(q_in);
       require_device(q_in, d.device);
       q = rows(q_in, "q");
@@ -319,7 +330,7 @@ PyObject* gather(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // pages x 4, page_table, starts, counts, q, scale, max_keys, return_lse, stream -> out or (out, lse)
 PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(n, 12, [&]() -> PyObject* {
-    const at::Tensor& q_in = tensor(args[7], "q");
+    const at::Tensor& q_in = tensor(args[7], "q", true);
     require_gpu(q_in);
     Description d(q_in.device());
     const at::Tensor q = rows(q_in, "q");

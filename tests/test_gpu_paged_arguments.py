@@ -85,3 +85,30 @@ def test_refused_while_a_graph_is_traced(gpu):
             with pytest.raises(ValueError, match="traced"):
                 trace()
         assert torch.equal(torch.compile(step, backend="eager")(x), want)
+
+
+def test_tensors_that_are_not_their_storage(gpu):
+    """Lazily negated rope tables are refused, queries, keys and values are read with the sign; lazily
+    zero ones are refused."""
+    cache, table, starts, x, rope = _call()
+    want = [*paged.append_tokens(cache, table, starts, x, x, x, rope, return_keys=True),
+            cache.key_pages.clone(), cache.value_pages.clone()]
+    minus = torch._neg_view(-x)
+    got = [*paged.append_tokens(cache, table, starts, minus, minus, minus, rope, return_keys=True),
+           cache.key_pages, cache.value_pages]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(paged.paged_attention(minus, cache, table, starts, 0.1),
+                       paged.paged_attention(x, cache, table, starts, 0.1))
+    for i in range(2):
+        for other in (torch._neg_view(rope[i]),
+                      torch._efficientzerotensor(rope[i].shape, dtype=torch.float32, device="cuda")):
+            with pytest.raises(ValueError, match="plain"):
+                paged.append_tokens(cache, table, starts, x, x, x, (other, rope[1]) if i == 0 else
+                                    (rope[0], other))
+    zero = torch._efficientzerotensor(x.shape, dtype=x.dtype, device="cuda")
+    for call in (lambda: paged.append_tokens(cache, table, starts, zero, x),
+                 lambda: paged.append_tokens(cache, table, starts, x, zero),
+                 lambda: paged.append_tokens(cache, table, starts, x, x, zero),
+                 lambda: paged.paged_attention(zero, cache, table, starts, 0.1)):
+        with pytest.raises(ValueError, match="plain"):
+            call()

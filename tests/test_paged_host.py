@@ -227,3 +227,41 @@ def test_refused_while_a_graph_is_traced():
     with FakeTensorMode(), pytest.raises(ValueError, match="traced"):
         _describe(cache, table, starts, None)
     step(starts)
+
+
+class _Wrapped(torch.Tensor):
+    """A subclass that computes by itself."""
+
+    @classmethod
+    def __torch_dispatch__(cls, function, types, args=(), kwargs=None):
+        raise AssertionError("not called")
+
+
+def test_tensors_that_are_not_their_storage():
+    """Lazily negated or zero tensors and subclasses: the kernels would read something else."""
+    for four in (False, True):
+        cache = paged.empty_pages(4, 16, 2, 128, "cpu", four_bit=four)
+        table, starts = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+        good = [cache.key_pages, cache.value_pages, cache.key_scales, cache.value_scales, table, starts,
+                starts.clone()]
+
+        def describe(*args):
+            return _describe(paged.PagedCache(*args[:4]), *args[4:])
+
+        describe(*good)
+        for i, x in enumerate(good):
+            if x is None:
+                continue
+            for other in (torch._neg_view(x), torch._efficientzerotensor(x.shape, dtype=x.dtype),
+                          torch.Tensor._make_subclass(_Wrapped, x)):
+                with pytest.raises(ValueError, match="plain"):
+                    describe(*good[:i], other, *good[i + 1:])
+    param = torch.nn.Parameter(cache.key_scales, requires_grad=False)     # plain for all that
+    describe(*good[:2], param, *good[3:])
+
+    def functional(x):
+        with pytest.raises(ValueError, match="plain"):
+            describe(*good[:6], x)
+        return x
+
+    torch.func.functionalize(functional)(starts)
