@@ -87,6 +87,12 @@ void require_eager() {
   if (traced) refuse("the paged cache's functions cannot be traced into a graph");
 }
 
+// x has been written in place: a backward pass that saved it has to find out. (Tensors made in
+// inference mode have no version.)
+void written(const at::Tensor& x) {
+  if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();
+}
+
 int small(int64_t x, const char* name) {
   if (x > INT_MAX) refuse(name, " of ", x, " is more than 2^31 - 1");
   return (int)x;
@@ -293,7 +299,7 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const bool interleaved = truth(args[12]);
     void* stream = reinterpret_cast<void*>(integer(args[14]));
-    if (d.c.batch > 0 && d.c.tokens > 0)
+    if (d.c.batch > 0 && d.c.tokens > 0) {
       check(spx_paged_append(&d.c, q.defined() ? pointer(q) : nullptr,
                              q.defined() ? q.strides().data() : nullptr, pointer(k),
                              k.strides().data(), pointer(v), v.strides().data(),
@@ -302,6 +308,9 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                              interleaved, q_out.defined() ? pointer(q_out) : nullptr,
                              k_out.defined() ? pointer(k_out) : nullptr, stream),
             "spx_paged_append");
+      for (int i = 0; i < 4; ++i)
+        if (args[i] != Py_None) written(tensor(args[i], "pages"));
+    }
     return pair(q_out, k_out);
   });
 }

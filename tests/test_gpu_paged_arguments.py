@@ -112,3 +112,31 @@ def test_tensors_that_are_not_their_storage(gpu):
                  lambda: paged.paged_attention(zero, cache, table, starts, 0.1)):
         with pytest.raises(ValueError, match="plain"):
             call()
+
+
+@pytest.mark.parametrize("four", (False, True))
+def test_append_counts_as_a_write(gpu, four):
+    """The versions by which autograd finds that a saved tensor was written over: those of the pages
+    and scales that an append writes, and no others."""
+    _, table, starts, x, rope = _call()
+    cache = paged.empty_pages(8, 16, 2, 128, "cuda", four_bit=four)
+    tensors = [t for t in vars(cache).values() if t is not None] + [table, starts, x, *rope]
+    before = [t._version for t in tensors]
+    paged.gather_tokens(cache, table, starts, 1)
+    paged.paged_attention(x, cache, table, starts, 0.1)
+    paged.append_tokens(cache, table, starts, x[:, :0], x[:, :0])
+    assert [t._version for t in tensors] == before
+    paged.append_tokens(cache, table, starts, x, x, x, rope)
+    written = 4 if four else 2
+    assert all(t._version > v for t, v in zip(tensors[:written], before))
+    assert [t._version for t in tensors[written:]] == before[written:]
+    if not four:
+        leaf = torch.ones((), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+        product = (cache.key_pages * leaf).sum()
+        paged.append_tokens(cache, table, starts, x, x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()
+    with torch.inference_mode():               # tensors without a version
+        inner = paged.empty_pages(8, 16, 2, 128, "cuda", four_bit=four)
+        paged.append_tokens(inner, table, starts, x, x)
+    paged.append_tokens(inner, table, starts, x, x)
