@@ -1032,10 +1032,11 @@ constexpr int kPaWaveRows = 1024;
 
 // Workgroups (of four waves) that share the units, or 0: one of eight waves per stream and no
 // second launch. At 28/4 heads in bf16, 500 keys: 9.7 us so, 9.4 shared, but 2 us less on the host;
-// 1090 keys: 14.7 and 9.1 (a step of the eight waves is about 2 us).
+// 1090 keys: 14.7 and 9.1 (a step of the eight waves is about 2 us). A launch has fewer than 2^32
+// threads: more streams than that share their units, however short.
 template <int D, bool kFour>
 static int paged_grid(int64_t keys, int64_t streams) {
-  if (keys <= 2 * PagedShape<D, kFour, 8>::kUnit) return 0;
+  if (keys <= 2 * PagedShape<D, kFour, 8>::kUnit && streams <= 0xffffffffll / 512) return 0;
   using Shape = PagedShape<D, kFour, 4>;
   const int64_t units = (keys + Shape::kUnit - 1) / Shape::kUnit;
   return (int)std::min<int64_t>(std::min(kPaMaxGrid, kPaCus * Shape::kPerCu), streams * units);
@@ -1047,7 +1048,7 @@ struct PagedSizes {
 
 static bool paged_sizes(const spx_paged_cache& z, int q_heads, int max_keys, PagedSizes& s) {
   if (z.table_width <= 0 || z.page_size <= 0 || max_keys < 0 || z.batch <= 0 || z.tokens <= 0 ||
-      q_heads <= 0 || z.kv_heads <= 0 || q_heads % z.kv_heads != 0)
+      q_heads <= 0 || q_heads > 1 << 20 || z.kv_heads <= 0 || q_heads % z.kv_heads != 0)
     return false;
   if ((double)z.batch * z.tokens * q_heads > 0x7fffffff) return false;
   s.rows = (int64_t)z.batch * z.tokens * q_heads;

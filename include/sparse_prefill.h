@@ -386,8 +386,9 @@ int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out, voi
  * (strides as above); out: contiguous bf16 [B, T, Hq, D]; lse: natural-log LSE, contiguous
  * fp32 [B, T, Hq], or NULL. Positions without a place are not seen. Tokens that are not live,
  * see nothing, or have no score above -inf, give 0 and an LSE of -inf. batch * kv_heads *
- * ceil(T Hq / Hkv / 16) times the table's reach / 128 must stay below 2^31. max_keys: an upper bound of starts[b] + T that
- * the caller knows, or 0; it only chooses how the work is divided. workspace: device memory
+ * ceil(T Hq / Hkv / 16) times the table's reach / 128 must stay below 2^31, q_heads is at most
+ * 2^20. max_keys: an upper bound of starts[b] + T that the caller knows, or 0; it only chooses
+ * how the work is divided. workspace: device memory
  * of spx_paged_attention_workspace_bytes(...) bytes for the same arguments (-1: unsupported
  * shape; 0: none needed, may be NULL), 16-byte aligned, contents undefined before and after;
  * the size depends on the cache's sizes only, not on its pointers (but on whether there are

@@ -265,3 +265,17 @@ def test_tensors_that_are_not_their_storage():
         return x
 
     torch.func.functionalize(functional)(starts)
+
+
+def test_more_streams_than_one_launch_of_workgroups():
+    """2^32 threads and more do not fit a launch of one workgroup of 512 per stream: such calls share
+    their units, which takes a workspace. More heads than a join's launch has threads for: refused."""
+    size = _lib.load().spx_paged_attention_workspace_bytes
+    few = dict(width=4, page_size=128, kv_heads=8)               # 512 positions
+    assert size(_cache(batch=(1 << 20) - 1, **few), 8, 0) == 0
+    for batch in (1 << 20, 1 << 21):
+        assert size(_cache(batch=batch, **few), 8, 0) > batch * 8 * 8
+        assert size(_cache(batch=batch, **few), 8, 300) > batch * 8 * 8
+    assert size(_cache(batch=1, width=32, kv_heads=1 << 16), 1 << 20, 0) > 0
+    assert size(_cache(batch=1, width=32, kv_heads=1 << 16), 1 << 21, 0) == -1
+    assert _attention(batch=1, kv_heads=1 << 16, q_heads=1 << 21) == _lib.SPX_EINVAL
