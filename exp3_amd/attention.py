@@ -448,7 +448,9 @@ class AttentionBackend:
         **kwargs,
     ):
         """Reference attention.py:154-339. query [B, Hq, S, D], key / value
-        [B, Hkv, S, D] -> (output [B, S, Hq, D], None)."""
+        [B, Hkv, S, D] -> (output [B, S, Hq, D], None). Fewer queries than keys are a decode
+        step as in the reference: every query sees every key. Several tokens behind cached
+        ones, each seeing those up to itself: ``paged.paged_attention``."""
         record = {
             "layer": getattr(module, "layer_idx", None),
             "method": self.method,

@@ -4,8 +4,10 @@ back, and attention of new tokens over the pages, in bf16 or in 4 bits.
 The serving side of the prefill backend: a prompt's projections go through
 ``append_tokens`` (which stores K and V and returns the rotated Q and K that
 ``attention.AttentionBackend`` takes for the prefill), and every later step appends its
-tokens and calls ``paged_attention``. The reference keeps its cache in transformers'
-DynamicCache (evaluate.py) and has no counterpart of these functions.
+tokens and calls ``paged_attention``. So does a chunk of a prompt behind a cached prefix: the
+backend takes fewer queries than keys for a decode step and applies no mask. The reference
+keeps its cache in transformers' DynamicCache (evaluate.py) and has no counterpart of these
+functions.
 
 Common arguments:
 
