@@ -92,6 +92,8 @@ def empty_pages(pages: int, page_size: int, kv_heads: int, head_dim: int, device
 def rope_table(positions: int, rotary_dim: int, theta: float = 1.0e6, device=None):
     """fp32 (cos, sin) ``[positions, rotary_dim // 2]``, the angles formed in fp64 (in fp32
     those of positions near 131072 are off by up to 2^-8)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim} must be even and positive")
     inv = theta ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * inv
     return angle.cos().float(), angle.sin().float()

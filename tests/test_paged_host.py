@@ -279,3 +279,10 @@ def test_more_streams_than_one_launch_of_workgroups():
     assert size(_cache(batch=1, width=32, kv_heads=1 << 16), 1 << 20, 0) > 0
     assert size(_cache(batch=1, width=32, kv_heads=1 << 16), 1 << 21, 0) == -1
     assert _attention(batch=1, kv_heads=1 << 16, q_heads=1 << 21) == _lib.SPX_EINVAL
+
+
+def test_rope_table_sizes():
+    """rotary_dim is a number of dims that pair: an odd one gave a table of other angles."""
+    for size in (127, 1, 0, -2):
+        with pytest.raises(ValueError, match="rotary_dim"):
+            paged.rope_table(16, size)
