@@ -105,7 +105,9 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 def _run(tensor: torch.Tensor, name: str, cache: PagedCache, *args):
     """A function of the host module on the tensor's device (the launch needs it to be the
     current one)."""
-    if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
+    if not isinstance(tensor, torch.Tensor):
+        raise ValueError(f"expected a tensor, got {type(tensor).__name__}")
+    if not tensor.is_cuda:
         _lib.require_gpu(tensor)
     device = tensor.get_device()
     if device != _current_device():

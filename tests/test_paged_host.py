@@ -286,3 +286,13 @@ def test_rope_table_sizes():
     for size in (127, 1, 0, -2):
         with pytest.raises(ValueError, match="rotary_dim"):
             paged.rope_table(16, size)
+
+
+def test_wrappers_refuse_what_is_no_tensor():
+    cache = paged.empty_pages(4, 16, 2, 128, "cpu")
+    for x in (None, [1], 2.0):
+        for call in (lambda: paged.append_tokens(cache, None, None, x, x),
+                     lambda: paged.gather_tokens(cache, x, None, 1),
+                     lambda: paged.paged_attention(x, cache, None, None, 0.1)):
+            with pytest.raises(ValueError, match="tensor"):
+                call()
