@@ -35,6 +35,7 @@ int paged_map(PagedMap& m, const spx_paged_cache* cache) {
               SPX_EINVAL, "bad shape: batch %d tokens %d kv_heads %d pages %d table width %d",
               z.batch, z.tokens, z.kv_heads, z.pages, z.table_width);
   SPX_REQUIRE(z.kv_heads <= 1 << 16, SPX_EINVAL, "%d KV heads are more than 2^16", z.kv_heads);
+  SPX_REQUIRE(z.batch <= 1 << 30, SPX_EINVAL, "%d sequences are more than 2^30", z.batch);
   SPX_REQUIRE(z.reserved == 0, SPX_EINVAL, "reserved must be 0");
   SPX_REQUIRE((int64_t)z.table_width * z.page_size <= (1 << 30), SPX_EINVAL,
               "a table of %d pages of %d tokens exceeds 2^30 positions", z.table_width,

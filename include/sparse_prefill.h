@@ -353,7 +353,7 @@ typedef struct spx_paged_cache {
   int32_t page_size;
   int32_t kv_heads;          /* at most 2^16 */
   int32_t head_dim;
-  int32_t batch;
+  int32_t batch;             /* at most 2^30 */
   int32_t tokens;
   int32_t reserved;          /* 0 */
 } spx_paged_cache;

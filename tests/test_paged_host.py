@@ -296,3 +296,10 @@ def test_wrappers_refuse_what_is_no_tensor():
                      lambda: paged.paged_attention(x, cache, None, None, 0.1)):
             with pytest.raises(ValueError, match="tensor"):
                 call()
+
+
+@pytest.mark.parametrize("call", (_append, _gather))
+def test_batches_near_the_end_of_32_bits(call):
+    """Refused before the launch, whose size a batch above 2^31 - 65535 overflowed."""
+    for batch in (2**31 - 1, (1 << 30) + 1):
+        assert call(batch=batch) == _lib.SPX_EINVAL and b"2^30" in _lib.load().spx_last_error()
