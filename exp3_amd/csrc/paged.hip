@@ -97,12 +97,19 @@ __device__ __forceinline__ double fma_of(double x, double y, double z) {
   return __builtin_fma(x, y, z);
 }
 
-// Calls that read and write 8 MB and more store their outputs past the caches. Into memory that an
-// earlier call of the program used, as an allocator gives it: 4 x up to 2113 tokens appended in 4 bits
-// and read back 42 -> 30 us, 4 x up to 12001 read back 58 -> 49; into memory of each call's own, six in
-// turn: 32640 tokens appended 120 -> 114, 16000 as fast, 8000 29 -> 31. A dense prefill behind the
-// append takes as long in all (16000 tokens 1632 and 1632 us, 1089 43.6 and 42.8). What a decode step
-// writes is read at once and stays: attention behind it 36.3 us with it in the cache, 37.1 past it.
+// Calls of 8 MB and more store their outputs past the caches. The size is that of all rows in bf16,
+// read and written, also where pages of 4 bits make it less. Through the caches and past them, us (28/4
+// heads, six calls in turn; the first figure into memory that the calls hand on to each other, the
+// second into memory of each call's own):
+//              append, bf16           append, 4 bits         gather, bf16           gather, 4 bits
+//     4 MB   5.2  5.2 ->  5.1  5.1  5.2  5.2 ->  5.1  5.0  3.9  3.7 ->  3.4  3.5  3.8  3.7 ->  3.8  3.6
+//     8 MB   5.6  5.5 ->  5.4  5.4  5.5  5.4 ->  5.4  5.3  4.4  4.4 ->  4.3  4.3  4.1  4.1 ->  4.0  4.0
+//    16 MB   6.8  6.8 ->  6.3  6.3  6.8  6.8 ->  6.4  6.4  5.6  5.6 ->  5.4  5.4  5.0  4.9 ->  4.4  4.4
+//    64 MB  16.2 18.0 -> 16.3 16.2 15.9 17.1 -> 13.8 13.6 12.4 16.3 -> 12.3 12.3 10.1 10.6 ->  9.3  9.4
+//   128 MB  26.8 30.3 -> 29.0 28.8 27.8 30.8 -> 30.3 30.1 25.0 28.0 -> 26.4 26.3 16.1 22.7 -> 15.8 15.4
+// Below 4 MB both are equal. A dense prefill behind the append takes as long in all (16000 tokens 1632
+// and 1632 us, 1089 43.6 and 42.8). What a decode step writes is read at once and stays: attention
+// behind it 36.3 us with it in the cache, 37.1 past it.
 constexpr int64_t kStreamedBytes = 8 << 20;
 
 // (A template parameter: of a run-time choice the compiler makes one ordinary store.)
@@ -153,7 +160,6 @@ struct Rotation {
         for (int e = 0; e < 8; ++e) s[e] = -s[e];
     }
   }
-  // R = float or double; `other`: the partner dims (or the same ones).
   // Dim e; R = float or double; `other`: the partner dims (or the same ones).
   template <typename R>
   __device__ __forceinline__ R dim(const u32x4& own, const u32x4& other, int e) const {
@@ -220,7 +226,7 @@ __device__ __forceinline__ void store_4bit(void* pages, uint8_t* scales, int64_t
 // the same again). The next chunk is loaded while one is rotated, and every chunk of q is one load and
 // one store: the wait for the load then counts past the store behind it. (A row per group of lanes of
 // any kind, stores under conditions, waited for each store as well: 32640 tokens, 28/4 heads, bf16,
-// rotated copies of q and k, 142 -> 122 us; 8000 tokens 48 -> 34, in 4 bits 54 -> 37.) What a token's
+// rotated copies of q and k, 142 -> 120 us; 8000 tokens 48 -> 29, 4 x up to 2113 in 4 bits 62 -> 35.) What a token's
 // chunks have in common (its place, cos and sin of the lane's dims) is found once, behind the first
 // load. Two chunks ahead: no change.
 template <int D, bool kFour, bool kStreamed>

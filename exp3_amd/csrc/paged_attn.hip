@@ -6,11 +6,11 @@
 // ceil(keys / unit) units.
 //
 // Bound: HBM (each visible row of K and V once per column tile); with 4-bit pages the unpacking
-// is close behind (some 110 vector instructions per 16 keys); with one unit per workgroup the chain
+// is close behind (some 120 vector instructions per 16 keys); with one unit per workgroup the chain
 // lengths -> page ids -> K and V -> merge. Measured, main kernel + merge: 8 ragged sequences of up
-// to 16000 keys (32/8 heads, bf16) 51 + 4.8 us, the 314 MB at 5.6 TB/s; 64 of up to 8192 in 4 bits
-// 64.5 + 4.8, 301 MB at 4.7 TB/s; 131072 keys (28/4, 4 bits) 17.5 + 4.3;
-// 32641 keys 8.0 + 3.1; 1090 keys in bf16 5.9 + 3.1.
+// to 16000 keys (32/8 heads, bf16) 50 + 4.8 us, the 314 MB at 5.7 TB/s; 64 of up to 8192 in 4 bits
+// 71 + 4.8, 301 MB at 4.0 TB/s; 131072 keys (28/4, 4 bits) 20 + 4.0;
+// 32641 keys 8.3 + 3.7; 1090 keys in bf16 6.0 + 3.7.
 //   * The streams' units, in order, are dealt in equal runs to the workgroups of one grid that
 //     fills the chip. The lengths are device data, so every workgroup finds its run itself:
 //     a prefix sum over the batch in one wave (a load and some shuffles), no host
@@ -240,7 +240,9 @@ struct Stream {
 // ------------------------------------------------------------------------- one stream
 
 // The kernel arguments, read afresh: nothing derived from them is held across the loop over a
-// stream's units (held, they cost its scalar registers, and spills to vector lanes).
+// stream's units (held, they cost its scalar registers, and spills to vector lanes inside the loop).
+// What is left is kept outside it, stored before and read behind a stream: 19 to 23 scalar registers
+// in vector lanes (4 bits, D = 128), 4 or 5 vector registers in scratch (bf16, D = 256).
 __device__ __forceinline__ PagedAttnArgs fresh_args() {
 #if defined(__HIP_DEVICE_COMPILE__)
   auto p = (const __attribute__((address_space(4))) PagedAttnArgs*)
@@ -829,7 +831,7 @@ paged_attn_kernel(PagedAttnArgs args) {
       }
       const int cn = s.tile * kPaCols + col;
       const int ct = column_token(a, cn);
-      if (ct >= s.live) {      // not live: sees nothing, whatever step() added
+      if (ct >= s.live) {      // not live: sees nothing, whatever was added
         v = f32x4{};
         sum = 0.0f;
         top = -INFINITY;

@@ -158,7 +158,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     ``0 .. starts[b] + i`` -> bf16 ``[B, T, Hq, D]``, with ``return_lse`` also the natural-log
     LSE, fp32 ``[B, T, Hq]``. Tokens that are not live, see nothing, or have no score above -inf
     give 0 and -inf. ``max_keys``: an upper bound of ``starts[b] + T`` where the caller has one;
-    it only chooses how the work is divided. Meant for decode steps and a few drafted tokens:
-    each 16 of the T x Hq / Hkv rows of a KV head read K and V anew."""
+    it only chooses how the work is divided, and pays where the table reaches far and all
+    sequences are short (up to 512 keys, 1024 in 4 bits at D = 128). Meant for decode steps and
+    a few drafted tokens: each 16 of the T x Hq / Hkv rows of a KV head read K and V anew."""
     return _run(q, "attention", cache, page_table, starts, counts, q, scale,
                 0 if max_keys is None else max_keys, return_lse)
