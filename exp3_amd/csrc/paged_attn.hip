@@ -7,10 +7,11 @@
 //
 // Bound: HBM (each visible row of K and V once per column tile); with 4-bit pages the unpacking
 // is close behind (some 120 vector instructions per 16 keys); with one unit per workgroup the chain
-// lengths -> page ids -> K and V -> merge. Measured, main kernel + merge: 8 ragged sequences of up
-// to 16000 keys (32/8 heads, bf16) 50 + 4.8 us, the 314 MB at 5.7 TB/s; 64 of up to 8192 in 4 bits
-// 71 + 4.8, 301 MB at 4.0 TB/s; 131072 keys (28/4, 4 bits) 20 + 4.0;
-// 32641 keys 8.3 + 3.7; 1090 keys in bf16 6.0 + 3.7.
+// lengths -> page ids -> K and V -> merge (bf16 pages: lengths -> Q -> page ids, whose load the
+// compiler moves behind the wait for Q). Measured, main kernel + merge: 8 ragged sequences of up to
+// 16000 keys (32/8 heads, bf16) 50 + 4.8 us, the 314 MB at 5.7 TB/s; 64 of up to 8192 in 4 bits
+// 71 + 4.8, 301 MB at 4.0 TB/s; 131072 keys (28/4, 4 bits) 20 + 4.0; 32641 keys 8.3 + 3.7; 1090 keys
+// in bf16 6.0 + 3.7.
 //   * The streams' units, in order, are dealt in equal runs to the workgroups of one grid that
 //     fills the chip. The lengths are device data, so every workgroup finds its run itself:
 //     a prefix sum over the batch in one wave (a load and some shuffles), no host
