@@ -19,7 +19,7 @@ SPX_OK = 0
 SPX_EINVAL = -1
 SPX_EUNSUPPORTED = -2
 SPX_ELAUNCH = -3
-ABI_VERSION = 10
+ABI_VERSION = 11
 # int32 counters behind the attention entry points' work_queue (SPX_WORK_QUEUE_INTS)
 WORK_QUEUE_INTS = 16
 
@@ -65,12 +65,21 @@ _PROTOTYPES = {
     "spx_paged_append": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P],
     "spx_paged_gather": [_P, _P, _P, _P],
     "spx_paged_attention": [_P, _P, _P, _I, _I, _F, _P, _P, _P, _P],
+    "spx_paged_append_at": [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P],
+    "spx_draft_tree": [_P, _I, _I, _P, _P, _P],
+    "spx_paged_tree_attention": [_P, _P, _P, _I, _P, _I, _F, _P, _P, _P, _P],
+    "spx_paged_keep_path": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P],
+    "spx_paged_accumulate_weights": [_P, _P, _P, _I, _P, _F, _P, _P, ctypes.c_int64, _P],
+    "spx_paged_evict": [_P, _P, _P, ctypes.c_int64, _P, _I, _I, _I, _P, _P, _P, _P, _P],
 }
 
 # helpers without a status: sizes (int64)
 _SIZE_FUNCTIONS = {"spx_selector_workspace_bytes": [_I, _I, _I, _I],
                    "spx_decode_workspace_bytes": [_I, _I, _I, _I, _I],
                    "spx_paged_attention_workspace_bytes": [_P, _I, _I],
+                   "spx_paged_tree_attention_workspace_bytes": [_P, _I, _I],
+                   "spx_paged_accumulate_weights_workspace_bytes": [_P, _I],
+                   "spx_paged_evict_workspace_bytes": [_P, _I],
                    "spx_attention_queue_ints": [_I, _I, _I, _I, _I]}
 
 EXPORTED_SYMBOLS = tuple(_PROTOTYPES) + tuple(_SIZE_FUNCTIONS) + ("spx_last_error",

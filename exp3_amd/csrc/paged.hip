@@ -73,6 +73,8 @@ struct AppendArgs {
   const float* cos;
   const float* sin;                      // [positions, rotary / 2]; null: no rotation
   int rotary, interleaved;
+  const int32_t* positions;              // [B, T] of the rotation; null: the tokens' places
+  int rope_positions;
   int batch, tokens, q_rows, kv_heads;   // q_rows: query heads, 0 without q
   int wave_shift;                        // 2^wave_shift waves share a token's rows
   void* key_pages;
@@ -159,6 +161,11 @@ struct Rotation {
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[e] = -s[e];
     }
+  }
+  // Of a position that the tables do not reach.
+  __device__ __forceinline__ void undefined() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = s[e] = __builtin_nanf("");
   }
   // Dim e; R = float or double; `other`: the partner dims (or the same ones).
   template <typename R>
@@ -279,7 +286,10 @@ __global__ __launch_bounds__(kPagedThreads, kFour ? 6 : 1) void paged_append_ker
     }
     return;
   }
-  const Rotation rotation(a, d0, p);
+  const int at = a.positions ? scalar_load(a.positions + token) : p;
+  const bool reached = (unsigned)at < (unsigned)a.rope_positions;
+  Rotation rotation(a, d0, reached ? at : 0);
+  if (!reached) rotation.undefined();
   while (n < kv_chunks) {
     const int64_t row = a.map.row(page, head_of(n, a.kv_heads), p);
     const u32x4 own = advance();
@@ -442,12 +452,10 @@ static void launch_gather(const GatherArgs& a, bool four, bool streamed, dim3 gr
 
 using namespace spx;
 
-extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
-                                const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                                const void* v, const int64_t* v_strides, int q_heads,
-                                const float* rope_cos, const float* rope_sin, int rope_positions,
-                                int rotary_dim, int interleaved, void* q_out, void* k_out,
-                                void* stream) {
+static int append(const spx_paged_cache* cache, const void* q, const int64_t* q_strides, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides, int q_heads,
+                  const float* rope_cos, const float* rope_sin, int rope_positions, int rotary_dim,
+                  int interleaved, const int32_t* positions, void* q_out, void* k_out, void* stream) {
   AppendArgs a{};
   int status = paged_map(a.map, cache);
   if (status != SPX_OK) return status;
@@ -461,7 +469,9 @@ extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
     SPX_REQUIRE(rotary_dim > 0 && rotary_dim <= cache->head_dim && rotary_dim % 16 == 0,
                 SPX_EUNSUPPORTED, "rotary_dim %d unsupported (a multiple of 16 up to head_dim %d)",
                 rotary_dim, cache->head_dim);
-    SPX_REQUIRE(rope_positions >= (int64_t)cache->table_width * cache->page_size, SPX_EINVAL,
+    SPX_REQUIRE(rope_positions > 0 &&
+                    (positions || rope_positions >= (int64_t)cache->table_width * cache->page_size),
+                SPX_EINVAL,
                 "the rope table has %d positions, the page table reaches %lld", rope_positions,
                 (long long)cache->table_width * cache->page_size);
     SPX_REQUIRE(((reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin)) &
@@ -469,7 +479,12 @@ extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
   }
   SPX_REQUIRE(((reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out)) & 15) == 0,
               SPX_EINVAL, "outputs must be 16-byte aligned");
+  SPX_REQUIRE(positions == nullptr || rope_cos != nullptr, SPX_EINVAL, "positions need a rope table");
+  SPX_REQUIRE((reinterpret_cast<uintptr_t>(positions) & 3) == 0, SPX_EINVAL,
+              "positions must be 4-byte aligned");
   a.cos = rope_cos; a.sin = rope_sin;
+  a.positions = positions;
+  a.rope_positions = rope_cos ? rope_positions : 0x7fffffff;
   a.rotary = rope_cos ? rotary_dim : 0;
   a.interleaved = interleaved;
   a.batch = cache->batch;
@@ -493,6 +508,27 @@ extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
   if (cache->head_dim == 128) launch_append<128>(a, four, streamed, grid, st);
   else launch_append<256>(a, four, streamed, grid, st);
   return launch_status("paged_append");
+}
+
+extern "C" int spx_paged_append(const spx_paged_cache* cache, const void* q,
+                                const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, int q_heads,
+                                const float* rope_cos, const float* rope_sin, int rope_positions,
+                                int rotary_dim, int interleaved, void* q_out, void* k_out,
+                                void* stream) {
+  return append(cache, q, q_strides, k, k_strides, v, v_strides, q_heads, rope_cos, rope_sin,
+                rope_positions, rotary_dim, interleaved, nullptr, q_out, k_out, stream);
+}
+
+extern "C" int spx_paged_append_at(const spx_paged_cache* cache, const void* q,
+                                   const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                   const void* v, const int64_t* v_strides, int q_heads,
+                                   const float* rope_cos, const float* rope_sin, int rope_positions,
+                                   int rotary_dim, int interleaved, const int32_t* positions,
+                                   void* q_out, void* k_out, void* stream) {
+  SPX_REQUIRE(positions != nullptr, SPX_EINVAL, "null pointer (positions)");
+  return append(cache, q, q_strides, k, k_strides, v, v_strides, q_heads, rope_cos, rope_sin,
+                rope_positions, rotary_dim, interleaved, positions, q_out, k_out, stream);
 }
 
 extern "C" int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out,

@@ -37,7 +37,7 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.h"
+#include "paged_tiles.h"
 
 namespace spx {
 
@@ -77,12 +77,6 @@ struct PagedAttnArgs {
   u32x2* parts;                          // [streams] first partial's slot, how many (1: written out)
 };
 
-__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
-}
-
-__device__ __forceinline__ int first_lane(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // Weight of a partial with maximum m in a merge with maximum top: an empty partial
 // (m = -inf) counts nothing, also where every partial is empty.
 __device__ __forceinline__ float part_weight(float m, float top) {
@@ -90,14 +84,6 @@ __device__ __forceinline__ float part_weight(float m, float top) {
 }
 
 // ---------------------------------------------------------------- division of the work
-
-// n / d for n >= 0, inv = 1.0 / d: the quotient is off by one at most before it is put right. (An
-// integer division takes some 40 dependent instructions.)
-__device__ __forceinline__ int divide(int n, int d, double inv) {
-  const int q = (int)((double)n * inv);
-  const int r = n - q * d;
-  return q + (r >= d ? 1 : 0) - (r < 0 ? 1 : 0);
-}
 
 // Live tokens of a sequence: 0 .. live - 1.
 __device__ __forceinline__ int live_tokens(const PagedAttnArgs& a, int start, int count) {
@@ -133,17 +119,6 @@ __device__ __forceinline__ int head_units(const PagedAttnArgs& a, int start, int
   for (int tile = 0; tile < a.col_tiles; ++tile)
     units += (tile_keys(a, start, live, tile) + kUnit - 1) / kUnit;
   return units;
-}
-
-// Sum over the lanes up to this one.
-__device__ __forceinline__ int wave_prefix(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);    // row_shr 1, 2, 4, 8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);    // row_bcast 15, 31
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
-  return x;
 }
 
 // The units of 64 sequences, one a lane, and their prefix sums.
@@ -267,30 +242,6 @@ __device__ __forceinline__ void touch_args() {
 #endif
 }
 
-// Page memory as global memory: an opaque pointer of no known address space would be read by
-// flat loads, which are waited for together with the LDS.
-typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
-
-template <typename T>
-__device__ __forceinline__ T global_load(GlobalBytes p, uint32_t offset) {
-  return *(const __attribute__((address_space(1))) T*)(p + offset);
-}
-
-// The start of a tile, opaque: added to a lane's offset it is the scalar base of the load. Seen
-// through, the compiler held lane offset + head in two vector registers for each of the loads.
-__device__ __forceinline__ GlobalBytes tile_base(GlobalBytes p) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("" : "+s"(p));
-#endif
-  return p;
-}
-
-// Byte x of four scale bytes as the scale operand of a widening conversion, which looks at bits
-// 23 to 30 alone.
-__device__ __forceinline__ float scale_of(uint32_t bytes, int x) {
-  return __uint_as_float(__builtin_amdgcn_alignbit(bytes, bytes, 8 * x + 9));
-}
-
 __device__ __forceinline__ uint32_t opaque_bits(uint32_t x) { return (uint32_t)opaque((int)x); }
 
 // The lane, recomputed where it is used: what rare paths derive from it is not held meanwhile.
@@ -326,65 +277,6 @@ template <int D>
 __device__ __forceinline__ int dim_at(int place) {
   return value_dim<D>(place / 4 % 16, place / 64 * 4);
 }
-
-// One KV head of the page arrays.
-template <int D, bool kFour>
-struct HeadPages {
-  static constexpr int kRowBytes = kFour ? D / 2 : 2 * D, kRowScales = D / kPagedGroup;
-  GlobalBytes keys, values, key_scales, value_scales;
-  int page_rows, slot_mask;              // rows from one page to the next
-
-  __device__ __forceinline__ HeadPages(const PagedAttnArgs& a, int kvh) {
-    const int64_t first = (int64_t)kvh << a.map.page_shift;
-    keys = (GlobalBytes)a.key_pages + first * kRowBytes;
-    values = (GlobalBytes)a.value_pages + first * kRowBytes;
-    if constexpr (kFour) {
-      key_scales = (GlobalBytes)a.key_scales + first * kRowScales;
-      value_scales = (GlobalBytes)a.value_scales + first * kRowScales;
-    }
-    page_rows = a.kv_heads << a.map.page_shift;
-    slot_mask = (1 << a.map.page_shift) - 1;
-  }
-  __device__ __forceinline__ int64_t row(int page, int p) const {
-    return (int64_t)page * page_rows + (p & slot_mask);
-  }
-};
-
-template <int D, bool kFour>
-struct KeyTile {                         // a lane's part of 16 rows of K: row c
-  u32x4 raw[D / (kFour ? 128 : 32)];
-  uint32_t scale[kFour ? D / 128 : 1];   // four scale bytes of the row; the lane's is byte g
-
-  __device__ __forceinline__ void load(const HeadPages<D, kFour>& h, int64_t row, int c, int g) {
-    const GlobalBytes p = tile_base(h.keys + row * h.kRowBytes);
-    if constexpr (kFour) {
-      const GlobalBytes s = tile_base(h.key_scales + row * h.kRowScales);
-#pragma unroll
-      for (int x = 0; x < D / 128; ++x)
-        raw[x] = global_load<u32x4>(p, c * (D / 2) + 64 * x + 16 * g);
-      if constexpr (D == 128) {
-        scale[0] = global_load<uint32_t>(s, c * 4);
-      } else {
-        const u32x2 w = global_load<u32x2>(s, c * 8);
-        scale[0] = w[0];
-        scale[1] = w[1];
-      }
-    } else {
-#pragma unroll
-      for (int kk = 0; kk < D / 32; ++kk)
-        raw[kk] = global_load<u32x4>(p, c * 2 * D + 64 * kk + 16 * g);
-    }
-  }
-  // Eight dims of the row as A operand of product kk.
-  __device__ __forceinline__ u32x4 operand(int kk, int g) const {
-    if constexpr (!kFour) return raw[kk];
-    else return widen8(raw[kk / 4][kk % 4], scale_of(scale[kk / 4], g));
-  }
-  // Dim of the operand's first element.
-  static __device__ __forceinline__ int dim(int kk, int g) {
-    return kFour ? 128 * (kk / 4) + 32 * g + 8 * (kk % 4) : 32 * kk + 8 * g;
-  }
-};
 
 template <int D, bool kFour>
 struct ValueTile {                       // a lane's dims of four rows of V: 4 g + r

@@ -13,6 +13,7 @@
 
 #include <sstream>
 #include <stdexcept>
+#include <vector>
 
 #include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
@@ -27,6 +28,7 @@
 namespace {
 
 constexpr int kScaleGroup = 32;          // dims per scale of a 4-bit page
+constexpr int kTreeTokens = 256;         // nodes of a tree of drafted tokens
 
 struct Invalid : std::runtime_error {
   using std::runtime_error::runtime_error;
@@ -249,10 +251,22 @@ PyObject* guarded(Py_ssize_t got, Py_ssize_t wanted, const Body& body) {
   return nullptr;
 }
 
+// A contiguous tensor of this type and shape on the call's device.
+const at::Tensor& exactly(PyObject* object, const char* name, at::ScalarType type,
+                          at::IntArrayRef shape, const c10::Device& device) {
+  const at::Tensor& x = tensor(object, name);
+  if (x.scalar_type() != type || x.sizes() != shape || !x.is_contiguous())
+    refuse(name, " must be a contiguous ", type, " tensor of shape ", shape, ", got ", x.sizes(), " ",
+           x.scalar_type());
+  require_device(x, device);
+  require_no_gradient(x, name);
+  return x;
+}
+
 // pages x 4, page_table, starts, counts, k, v, q or None, cos or None, sin or None, interleaved,
-// return_keys, stream -> (rotated q or None, rotated k or None)
+// return_keys, stream, [positions] -> (rotated q or None, rotated k or None)
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded(n, 15, [&]() -> PyObject* {
+  return guarded(n, n == 16 ? 16 : 15, [&]() -> PyObject* {
     const at::Tensor& k_in = tensor(args[7], "k", true);
     const at::Tensor& v_in = tensor(args[8], "v", true);
     require_gpu(k_in);
@@ -299,15 +313,29 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const bool interleaved = truth(args[12]);
     void* stream = reinterpret_cast<void*>(integer(args[14]));
+    const int32_t* at_positions = nullptr;
+    if (n == 16) {
+      if (table[0] == nullptr) refuse("positions without a rope table");
+      at_positions = static_cast<const int32_t*>(
+          pointer(exactly(args[15], "positions", at::kInt, k.sizes().slice(0, 2), d.device)));
+    }
     if (d.c.batch > 0 && d.c.tokens > 0) {
-      check(spx_paged_append(&d.c, q.defined() ? pointer(q) : nullptr,
-                             q.defined() ? q.strides().data() : nullptr, pointer(k),
-                             k.strides().data(), pointer(v), v.strides().data(),
-                             q.defined() ? small(q.size(2), "query heads") : 0, table[0], table[1],
-                             small(positions, "rope positions"), small(2 * half, "rotary_dim"),
-                             interleaved, q_out.defined() ? pointer(q_out) : nullptr,
-                             k_out.defined() ? pointer(k_out) : nullptr, stream),
-            "spx_paged_append");
+      void* q_ptr = q.defined() ? pointer(q) : nullptr;
+      const int64_t* q_strides = q.defined() ? q.strides().data() : nullptr;
+      const int q_heads = q.defined() ? small(q.size(2), "query heads") : 0;
+      const int reach = small(positions, "rope positions"), rotary = small(2 * half, "rotary_dim");
+      void* q_to = q_out.defined() ? pointer(q_out) : nullptr;
+      void* k_to = k_out.defined() ? pointer(k_out) : nullptr;
+      if (at_positions == nullptr)
+        check(spx_paged_append(&d.c, q_ptr, q_strides, pointer(k), k.strides().data(), pointer(v),
+                               v.strides().data(), q_heads, table[0], table[1], reach, rotary,
+                               interleaved, q_to, k_to, stream),
+              "spx_paged_append");
+      else
+        check(spx_paged_append_at(&d.c, q_ptr, q_strides, pointer(k), k.strides().data(), pointer(v),
+                                  v.strides().data(), q_heads, table[0], table[1], reach, rotary,
+                                  interleaved, at_positions, q_to, k_to, stream),
+              "spx_paged_append_at");
       for (int i = 0; i < 4; ++i)
         if (args[i] != Py_None) written(tensor(args[i], "pages"));
     }
@@ -370,6 +398,256 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// parents, stream -> (depths, masks)
+PyObject* draft_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 2, [&]() -> PyObject* {
+    const at::Tensor& parents = tensor(args[0], "parents");
+    require_gpu(parents);
+    if (parents.dim() != 2 || parents.scalar_type() != at::kInt || !parents.is_contiguous() ||
+        parents.size(1) == 0 || parents.size(1) > kTreeTokens)
+      refuse("parents must be a contiguous int32 [batch, tokens] tensor of 1 to ", kTreeTokens,
+             " tokens, got ", parents.sizes(), " ", parents.scalar_type());
+    const int64_t shape[3] = {parents.size(0), parents.size(1), (parents.size(1) + 63) / 64};
+    const at::Tensor depths = empty(parents.sizes(), at::kInt, parents.device());
+    const at::Tensor masks = empty(shape, at::kLong, parents.device());
+    if (shape[0] > 0)
+      check(spx_draft_tree(static_cast<const int32_t*>(pointer(parents)), small(shape[0], "batch"),
+                           (int)shape[1], static_cast<int32_t*>(pointer(depths)),
+                           static_cast<uint64_t*>(pointer(masks)),
+                           reinterpret_cast<void*>(integer(args[1]))),
+            "spx_draft_tree");
+    return pair(depths, masks);
+  });
+}
+
+// pages x 4, page_table, starts, counts, q, masks, scale, max_keys, return_lse, stream -> out or
+// (out, lse)
+PyObject* tree_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 13, [&]() -> PyObject* {
+    const at::Tensor& q_in = tensor(args[7], "q", true);
+    require_gpu(q_in);
+    Description d(q_in.device());
+    const at::Tensor q = rows(q_in, "q");
+    d.pages(args);
+    d.map(args + 4, q.size(0), q.size(1));
+    if (q.size(3) != d.c.head_dim || q.size(2) == 0 || d.c.kv_heads == 0 ||
+        q.size(2) % d.c.kv_heads != 0)
+      refuse("q ", q.sizes(), " does not fit a cache of ", d.c.kv_heads, " heads of ", d.c.head_dim);
+    if (q.size(1) > kTreeTokens) refuse(q.size(1), " drafted tokens are more than ", kTreeTokens);
+    const int64_t shape[3] = {q.size(0), q.size(1), (q.size(1) + 63) / 64};
+    const at::Tensor& masks = exactly(args[8], "masks", at::kLong, shape, d.device);
+    const double scale = PyFloat_AsDouble(args[9]);
+    if (scale == -1.0 && PyErr_Occurred()) throw std::bad_exception();
+    const int64_t max_keys = integer(args[10]);
+    if (max_keys < 0) refuse("max_keys must not be negative, got ", max_keys);
+    const int bound = (int)std::min<int64_t>(max_keys, INT_MAX);
+    const int q_heads = small(q.size(2), "query heads");
+    const at::Tensor out = empty(q.sizes(), at::kBFloat16, d.device);
+    at::Tensor lse;
+    if (truth(args[11])) lse = empty(q.sizes().slice(0, 3), at::kFloat, d.device);
+    void* stream = reinterpret_cast<void*>(integer(args[12]));
+    if (d.c.batch > 0 && d.c.tokens > 0) {
+      const int64_t bytes = spx_paged_tree_attention_workspace_bytes(&d.c, q_heads, bound);
+      const at::Tensor workspace = empty({std::max<int64_t>(bytes, 16)}, at::kByte, d.device);
+      check(spx_paged_tree_attention(&d.c, pointer(q), q.strides().data(), q_heads,
+                                     static_cast<const uint64_t*>(pointer(masks)), bound, (float)scale,
+                                     pointer(workspace), pointer(out),
+                                     lse.defined() ? static_cast<float*>(pointer(lse)) : nullptr,
+                                     stream),
+            "spx_paged_tree_attention");
+    }
+    return lse.defined() ? pair(out, lse) : wrap(out);
+  });
+}
+
+// The pages of one PagedCache object.
+void cache_pages(PyObject* cache, PyObject* (&held)[4]) {
+  static PyObject* names[4] = {
+      PyUnicode_InternFromString("key_pages"), PyUnicode_InternFromString("value_pages"),
+      PyUnicode_InternFromString("key_scales"), PyUnicode_InternFromString("value_scales")};
+  for (int i = 0; i < 4; ++i) {
+    held[i] = PyObject_GetAttr(cache, names[i]);
+    if (held[i] == nullptr) throw std::bad_exception();
+  }
+}
+
+// tuple of PagedCaches, page_table, starts, counts, then either parents, drafts, targets, stream ->
+// (accepted, path, following), or path, stream -> None
+PyObject* keep_path(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  const bool walk = n == 8;
+  return guarded(n, walk ? 8 : 6, [&]() -> PyObject* {
+    if (!PyTuple_Check(args[0]) || PyTuple_GET_SIZE(args[0]) == 0) refuse("no caches");
+    const Py_ssize_t count = PyTuple_GET_SIZE(args[0]);
+    const at::Tensor& first = tensor(args[4], walk ? "parents" : "path");
+    require_gpu(first);
+    if (first.dim() != 2 || first.size(1) > kTreeTokens)
+      refuse(walk ? "parents" : "path", " must be an int32 [batch, tokens] tensor of at most ",
+             kTreeTokens, " tokens, got ", first.sizes());
+    Description d(first.device());
+    const auto shape = first.sizes();
+    exactly(args[4], walk ? "parents" : "path", at::kInt, shape, d.device);
+    struct Pages {
+      PyObject* held[4] = {};
+      ~Pages() {
+        for (PyObject* x : held) Py_XDECREF(x);
+      }
+    };
+    std::vector<Pages> objects(count);
+    std::vector<spx_paged_cache> caches(count);
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      cache_pages(PyTuple_GET_ITEM(args[0], i), objects[i].held);
+      d.pages(objects[i].held);
+      if (i == 0) d.map(args + 1, shape[0], shape[1]);
+      if (objects[i].held[2] == Py_None) d.c.key_scales = d.c.value_scales = nullptr;
+      caches[i] = d.c;
+    }
+    at::Tensor accepted, path, following;
+    const int64_t *drafts = nullptr, *targets = nullptr;
+    if (walk) {
+      drafts = static_cast<const int64_t*>(
+          pointer(exactly(args[5], "drafts", at::kLong, shape, d.device)));
+      targets = static_cast<const int64_t*>(
+          pointer(exactly(args[6], "targets", at::kLong, shape, d.device)));
+      accepted = empty({shape[0]}, at::kInt, d.device);
+      path = empty(shape, at::kInt, d.device);
+      following = empty({shape[0]}, at::kLong, d.device);
+    }
+    void* stream = reinterpret_cast<void*>(integer(args[walk ? 7 : 5]));
+    if (shape[0] > 0 && shape[1] > 0) {
+      const int32_t* nodes = static_cast<const int32_t*>(pointer(first));
+      check(spx_paged_keep_path(caches.data(), small(count, "caches"), walk ? nodes : nullptr, drafts,
+                                targets, walk ? nullptr : nodes,
+                                walk ? static_cast<int32_t*>(pointer(accepted)) : nullptr,
+                                walk ? static_cast<int32_t*>(pointer(path)) : nullptr,
+                                walk ? static_cast<int64_t*>(pointer(following)) : nullptr, stream),
+            "spx_paged_keep_path");
+      for (const Pages& x : objects)
+        for (PyObject* page : x.held)
+          if (page != Py_None) written(tensor(page, "pages"));
+    } else if (walk && shape[0] > 0) {
+      refuse("trees without nodes");
+    }
+    if (!walk) Py_RETURN_NONE;
+    PyObject *a = wrap(accepted), *b = wrap(path), *c = wrap(following);
+    PyObject* out = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    Py_XDECREF(c);
+    return out;
+  });
+}
+
+// A ledger tensor: [B, Hkv, slots] for all slots that the page table reaches.
+const at::Tensor& ledger(const Description& d, PyObject* object, const char* name,
+                         at::ScalarType type) {
+  const at::Tensor& x = tensor(object, name);
+  const int64_t reach = (int64_t)d.c.table_width * d.c.page_size;
+  if (x.dim() != 3 || x.scalar_type() != type || x.size(0) != d.c.batch || x.size(1) != d.c.kv_heads ||
+      x.size(2) < reach || !x.is_contiguous())
+    refuse(name, " must be a contiguous ", type, " [", d.c.batch, ", ", d.c.kv_heads,
+           ", slots] tensor of at least ", reach, " slots, got ", x.sizes(), " ", x.scalar_type());
+  require_device(x, d.device);
+  require_no_gradient(x, name);
+  return x;
+}
+
+// pages x 4, page_table, starts, counts, weights, q, lse, scale, stream -> None
+PyObject* accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 12, [&]() -> PyObject* {
+    const at::Tensor& q_in = tensor(args[8], "q", true);
+    require_gpu(q_in);
+    Description d(q_in.device());
+    const at::Tensor q = rows(q_in, "q");
+    d.pages(args);
+    d.map(args + 4, q.size(0), q.size(1));
+    if (q.size(3) != d.c.head_dim || q.size(2) == 0 || d.c.kv_heads == 0 ||
+        q.size(2) % d.c.kv_heads != 0)
+      refuse("q ", q.sizes(), " does not fit a cache of ", d.c.kv_heads, " heads of ", d.c.head_dim);
+    const at::Tensor& weights = ledger(d, args[7], "weights", at::kFloat);
+    const at::Tensor& lse = exactly(args[9], "lse", at::kFloat, q.sizes().slice(0, 3), d.device);
+    const double scale = PyFloat_AsDouble(args[10]);
+    if (scale == -1.0 && PyErr_Occurred()) throw std::bad_exception();
+    void* stream = reinterpret_cast<void*>(integer(args[11]));
+    if (d.c.batch > 0 && d.c.tokens > 0) {
+      const int q_heads = small(q.size(2), "query heads");
+      const int64_t bytes = spx_paged_accumulate_weights_workspace_bytes(&d.c, q_heads);
+      at::Tensor workspace;
+      if (bytes > 0) workspace = empty({bytes}, at::kByte, d.device);
+      check(spx_paged_accumulate_weights(&d.c, pointer(q), q.strides().data(), q_heads,
+                                         static_cast<const float*>(pointer(lse)), (float)scale,
+                                         workspace.defined() ? pointer(workspace) : nullptr,
+                                         static_cast<float*>(pointer(weights)), weights.size(2), stream),
+            "spx_paged_accumulate_weights");
+      written(weights);
+    }
+    Py_RETURN_NONE;
+  });
+}
+
+// pages x 4, page_table, lengths, weights, positions or None, seen or None, budget, recent, sinks,
+// weights out or None, positions out or None, stream -> (lengths, weights, positions)
+PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded(n, 15, [&]() -> PyObject* {
+    const at::Tensor& lengths = tensor(args[5], "lengths");
+    require_gpu(lengths);
+    Description d(lengths.device());
+    d.pages(args);
+    PyObject* const map[3] = {args[4], args[5], Py_None};
+    d.map(map, lengths.dim() == 1 ? lengths.size(0) : 0, 1);
+    const at::Tensor& weights = ledger(d, args[6], "weights", at::kFloat);
+    const int32_t *positions = nullptr, *seen = nullptr;
+    if (args[7] != Py_None) {
+      const at::Tensor& x = ledger(d, args[7], "positions", at::kInt);
+      if (x.sizes() != weights.sizes())
+        refuse("positions ", x.sizes(), " and weights ", weights.sizes(), " differ");
+      positions = static_cast<const int32_t*>(pointer(x));
+    }
+    if (args[8] != Py_None) seen = d.lengths(args[8], "seen");
+    const int64_t budget = integer(args[9]), recent = integer(args[10]), sinks = integer(args[11]);
+    if (budget <= 0 || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent)
+      refuse("a budget of ", budget, " must be positive and hold the ", recent, " recent and ", sinks,
+             " first tokens");
+    if ((args[12] == Py_None) != (args[13] == Py_None)) refuse("out needs weights and positions");
+    at::Tensor weights_out, positions_out;
+    if (args[12] == Py_None) {
+      weights_out = empty(weights.sizes(), at::kFloat, d.device);
+      positions_out = empty(weights.sizes(), at::kInt, d.device);
+    } else {
+      weights_out = ledger(d, args[12], "out weights", at::kFloat);
+      positions_out = ledger(d, args[13], "out positions", at::kInt);
+      if (weights_out.sizes() != weights.sizes() || positions_out.sizes() != weights.sizes())
+        refuse("out ", weights_out.sizes(), " and ", positions_out.sizes(), " differ from weights ",
+               weights.sizes());
+    }
+    const at::Tensor left = empty(lengths.sizes(), at::kInt, d.device);
+    void* stream = reinterpret_cast<void*>(integer(args[14]));
+    if (d.c.batch > 0 && d.c.kv_heads > 0) {
+      const int limit = (int)std::min<int64_t>(budget, INT_MAX);
+      const int64_t bytes = spx_paged_evict_workspace_bytes(&d.c, limit);
+      const at::Tensor workspace = empty({std::max<int64_t>(bytes, 16)}, at::kByte, d.device);
+      check(spx_paged_evict(&d.c, static_cast<const float*>(pointer(weights)), positions,
+                            weights.size(2), seen, limit, (int)std::min<int64_t>(recent, INT_MAX),
+                            (int)std::min<int64_t>(sinks, INT_MAX), pointer(workspace),
+                            static_cast<float*>(pointer(weights_out)),
+                            static_cast<int32_t*>(pointer(positions_out)),
+                            static_cast<int32_t*>(pointer(left)), stream),
+            "spx_paged_evict");
+      for (int i = 0; i < 4; ++i)
+        if (args[i] != Py_None) written(tensor(args[i], "pages"));
+      if (args[12] != Py_None) {
+        written(weights_out);
+        written(positions_out);
+      }
+    }
+    PyObject *a = wrap(left), *b = wrap(weights_out), *c = wrap(positions_out);
+    PyObject* out = a && b && c ? PyTuple_Pack(3, a, b, c) : nullptr;
+    Py_XDECREF(a);
+    Py_XDECREF(b);
+    Py_XDECREF(c);
+    return out;
+  });
+}
+
 // pages x 4, page_table, starts, counts, batch, tokens -> (pages, page_size, Hkv, D, table width):
 // the checks alone, on any device
 PyObject* describe(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -386,6 +664,11 @@ PyMethodDef kMethods[] = {
     {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, nullptr},
     {"gather", (PyCFunction)(void (*)(void))gather, METH_FASTCALL, nullptr},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, nullptr},
+    {"draft_tree", (PyCFunction)(void (*)(void))draft_tree, METH_FASTCALL, nullptr},
+    {"tree_attention", (PyCFunction)(void (*)(void))tree_attention, METH_FASTCALL, nullptr},
+    {"keep_path", (PyCFunction)(void (*)(void))keep_path, METH_FASTCALL, nullptr},
+    {"accumulate", (PyCFunction)(void (*)(void))accumulate, METH_FASTCALL, nullptr},
+    {"evict", (PyCFunction)(void (*)(void))evict, METH_FASTCALL, nullptr},
     {"describe", (PyCFunction)(void (*)(void))describe, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

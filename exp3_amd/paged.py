@@ -102,7 +102,7 @@ def rope_table(positions: int, rotary_dim: int, theta: float = 1.0e6, device=Non
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _run(tensor: torch.Tensor, name: str, cache: PagedCache, *args):
+def _run(tensor: torch.Tensor, name: str, cache: PagedCache | None, *args, more=()):
     """A function of the host module on the tensor's device (the launch needs it to be the
     current one)."""
     if not isinstance(tensor, torch.Tensor):
@@ -112,16 +112,19 @@ def _run(tensor: torch.Tensor, name: str, cache: PagedCache, *args):
     device = tensor.get_device()
     if device != _current_device():
         with torch.cuda.device(device):
-            return _run(tensor, name, cache, *args)
-    return getattr(_lib.host_module(), name)(cache.key_pages, cache.value_pages, cache.key_scales,
-                                             cache.value_scales, *args, _lib.stream_of(device))
+            return _run(tensor, name, cache, *args, more=more)
+    call = getattr(_lib.host_module(), name)
+    if cache is None:
+        return call(*args, _lib.stream_of(device))
+    return call(cache.key_pages, cache.value_pages, cache.key_scales, cache.value_scales, *args,
+                _lib.stream_of(device), *more)
 
 
 def append_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Tensor,
                   k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None,
                   rope: tuple[torch.Tensor, torch.Tensor] | None = None,
                   counts: torch.Tensor | None = None, interleaved: bool = False,
-                  return_keys: bool = False):
+                  return_keys: bool = False, positions: torch.Tensor | None = None):
     """Rotate ``k`` (and ``q``), store ``k`` and ``v`` -> (rotated q or None, rotated k or None).
 
     k, v: bf16 ``[B, T, Hkv, D]``, q: bf16 ``[B, T, Hq, D]``, any strides (slices of one fused
@@ -135,10 +138,16 @@ def append_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Ten
     as NaN. Returned rows of tokens that are not live are 0.
 
     Two tokens of a call must not have the same place: pages that are appended to belong to one
-    sequence (full pages of a common prefix may be shared)."""
+    sequence (full pages of a common prefix may be shared).
+
+    ``positions``: int32 ``[B, T]``, the tokens' positions in the text for the rotation where they
+    are not their places in the cache: ``starts[:, None] + depths`` for the nodes of a drafted tree,
+    those of the text behind an eviction. ``rope`` then reaches as far as the text; dims that it
+    does not reach are stored and returned as NaN."""
     cos, sin = rope if rope is not None else (None, None)
+    more = () if positions is None else (positions,)
     return _run(k, "append", cache, page_table, starts, counts, k, v, q, cos, sin, interleaved,
-                return_keys)
+                return_keys, more=more)
 
 
 def gather_tokens(cache: PagedCache, page_table: torch.Tensor, starts: torch.Tensor, tokens: int,
@@ -163,3 +172,97 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor
     a few drafted tokens: each 16 of the T x Hq / Hkv rows of a KV head read K and V anew."""
     return _run(q, "attention", cache, page_table, starts, counts, q, scale,
                 0 if max_keys is None else max_keys, return_lse)
+
+
+# ------------------------------------------------------------- drafted trees
+
+def draft_tree(parents: torch.Tensor):
+    """The plan of trees of drafted tokens -> (depths int32 ``[B, T]``, masks int64
+    ``[B, T, ceil(T / 64)]``).
+
+    parents: int32 ``[B, T]``, T at most 256: the node that each one follows, one before it; any
+    other value (-1) for nodes that follow the cached tokens. ``masks``: bit ``j % 64`` of word
+    ``j // 64`` of row i is set where j is i or one of its ancestors; ``depths``: how many ancestors
+    a node has. Made once for a step, used by all layers."""
+    return _run(parents, "draft_tree", None, parents)
+
+
+def tree_attention(q: torch.Tensor, cache: PagedCache, page_table: torch.Tensor,
+                   starts: torch.Tensor, masks: torch.Tensor, scale: float,
+                   counts: torch.Tensor | None = None, max_keys: int | None = None,
+                   return_lse: bool = False):
+    """Attention of a tree of drafted tokens over the cache that already holds them: as
+    ``paged_attention``, but node i of sequence b (in place ``starts[b] + i``) sees the places below
+    ``starts[b]`` and the live nodes j whose bit is set in row i of ``masks``, e.g. from
+    ``draft_tree`` (any bits may be set). At most 256 nodes; K and V are read once for each 128 of
+    the T x Hq / Hkv rows of a KV head. ``max_keys``: an upper bound of ``starts[b] + T``, which only
+    chooses how the work is divided."""
+    return _run(q, "tree_attention", cache, page_table, starts, counts, q, masks, scale,
+                0 if max_keys is None else max_keys, return_lse)
+
+
+def _caches(caches):
+    return (caches,) if isinstance(caches, PagedCache) else tuple(caches)
+
+
+def accept_drafts(caches, page_table: torch.Tensor, starts: torch.Tensor, parents: torch.Tensor,
+                  drafts: torch.Tensor, targets: torch.Tensor, counts: torch.Tensor | None = None):
+    """The drafts that the model agrees with, moved into place in every cache -> (accepted int32
+    ``[B]``, path int32 ``[B, T]``, following int64 ``[B]``).
+
+    caches: a PagedCache or those of all layers, alike but for their pages. parents: as
+    ``draft_tree``; drafts, targets: int64 ``[B, T]``, a node's token and the token that the model
+    chose behind it. Node 0 (the last token that was decided) is accepted, then the first child whose
+    draft is the target of the node accepted last, as long as there is one. ``path``: the accepted
+    nodes, then -1; ``following``: the target of the last one, the next token. K and V of the
+    accepted nodes move to ``starts[b] .. starts[b] + accepted[b]``. No live node: 0 and -1."""
+    return _run(parents, "keep_path", None, _caches(caches), page_table, starts, counts, parents,
+                drafts, targets)
+
+
+def keep_path(caches, page_table: torch.Tensor, starts: torch.Tensor, path: torch.Tensor,
+              counts: torch.Tensor | None = None) -> None:
+    """K and V of a path that the caller accepted moved into place, in every cache: those of
+    ``starts[b] + path[b, j]`` to ``starts[b] + j``. path: int32 ``[B, T]``, T at most 256, live nodes
+    that ascend; it ends at the first one that is not one (-1)."""
+    _run(path, "keep_path", None, _caches(caches), page_table, starts, counts, path)
+
+
+# ------------------------------------------------------------------ eviction
+
+def accumulate_weights(weights: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, cache: PagedCache,
+                       page_table: torch.Tensor, starts: torch.Tensor, scale: float,
+                       counts: torch.Tensor | None = None) -> None:
+    """Add the attention weight that cached tokens receive from new ones, in place.
+
+    weights: fp32 ``[B, Hkv, slots]``, at least as many slots as the page table reaches, 0 where a
+    sequence begins; q and the other arguments as given to ``paged_attention``, lse: what it returned
+    with ``return_lse``. ``weights[b, kvh, p]`` grows by the sum over the rows (tokens, query heads of
+    the KV head) that see position p of their probability for it. Rows that see nothing add nothing.
+    A prompt's tokens are judged by its last ones: ``starts`` the prompt's length less T, q the
+    rotated queries of its last T tokens. Reads K once, whatever T."""
+    _run(q, "accumulate", cache, page_table, starts, counts, weights, q, lse, scale)
+
+
+def evict_tokens(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor,
+                 weights: torch.Tensor, budget: int, positions: torch.Tensor | None = None,
+                 seen: torch.Tensor | None = None, recent: int = 0, sinks: int = 0,
+                 out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """Drop the tokens of each KV head that gathered least, down to ``budget`` -> (lengths, weights,
+    positions).
+
+    lengths: int32 ``[B]``, tokens held (negative: a free slot). Kept are those whose position in the
+    text is below ``sinks`` or among the last ``recent`` (together at most ``budget``), then those of
+    the largest weight, the lower slot first among equals; NaN counts least. Heads keep different
+    tokens: the cache's slots are no positions any more. Tokens kept below slot ``budget`` stay, the
+    freed slots are filled in order with the ones kept behind it, so little moves and every later
+    append goes to the new end.
+
+    positions: int32, as weights, -1 for tokens appended since (all of them: None): those have
+    position ``seen[b] - lengths[b] + slot``; seen: int32 ``[B]``, tokens of the text so far (None:
+    the lengths, right for the first eviction). Returned are the new lengths and the new ``weights``
+    and ``positions`` (0 and -1 behind the end), in ``out`` if given, which may be the tensors
+    themselves. Sequences within the budget, or with a token that has no place, keep all. Later
+    tokens are appended with ``positions=``. Pages that are written to belong to one sequence."""
+    return _run(lengths, "evict", cache, page_table, lengths, weights, positions, seen, budget,
+                recent, sinks, *(out if out is not None else (None, None)))

@@ -38,7 +38,7 @@ extern "C" {
 #define SPX_EUNSUPPORTED (-2) /* valid in the reference, not built here       */
 #define SPX_ELAUNCH (-3)      /* HIP launch / runtime failure                 */
 
-#define SPX_ABI_VERSION 10
+#define SPX_ABI_VERSION 11
 
 /* int32 counters a work_queue argument of the attention entry points points to. */
 #define SPX_WORK_QUEUE_INTS 16
@@ -377,6 +377,15 @@ int spx_paged_append(const spx_paged_cache* cache, const void* q, const int64_t*
                      const float* rope_sin, int rope_positions, int rotary_dim, int interleaved,
                      void* q_out, void* k_out, void* stream);
 
+/* The same with the rotation's positions given, contiguous int32 [B, T]: those of new tokens whose
+ * place in the cache is not their position in the text (drafted trees, behind an eviction). The rope
+ * table has any length; where it does not reach a position, the rotated dims are NaN. */
+int spx_paged_append_at(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
+                        const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, int q_heads, const float* rope_cos,
+                        const float* rope_sin, int rope_positions, int rotary_dim, int interleaved,
+                        const int32_t* positions, void* q_out, void* k_out, void* stream);
+
 /* Read back: k_out, v_out contiguous bf16 [B, T, Hkv, D] of the tokens' positions; rows of
  * tokens that are not live or have no place are 0. 4-bit values are exact in bf16. */
 int spx_paged_gather(const spx_paged_cache* cache, void* k_out, void* v_out, void* stream);
@@ -398,6 +407,71 @@ int64_t spx_paged_attention_workspace_bytes(const spx_paged_cache* cache, int q_
 int spx_paged_attention(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
                         int q_heads, int max_keys, float scale, void* workspace, void* out,
                         float* lse, void* stream);
+
+/* ------------------------------------------ paged KV cache: drafted trees */
+
+/* Plan of trees of drafted tokens. parents: int32 [B, T], T at most 256; the parent of node i is a
+ * node before it, any other value (-1) is none. depths: int32 [B, T], how many ancestors a node has;
+ * masks: [B, T, ceil(T / 64)] words, bit j % 64 of word j / 64 of row i set where j is i or one of its
+ * ancestors. Both contiguous. */
+int spx_draft_tree(const int32_t* parents, int batch, int tokens, int32_t* depths, uint64_t* masks,
+                   void* stream);
+
+/* Attention of trees of drafted tokens over the cache that already holds them, node i in place
+ * starts[b] + i: it sees the places below starts[b] and those new live tokens j whose bit is set in
+ * row i of masks (as above; any bits). At most 256 tokens; everything else as spx_paged_attention, with
+ * spx_paged_tree_attention_workspace_bytes(...) bytes of workspace (never 0). K and V are read once for
+ * every 128 of the T Hq / Hkv rows of a KV head. */
+int64_t spx_paged_tree_attention_workspace_bytes(const spx_paged_cache* cache, int q_heads,
+                                                 int max_keys);
+int spx_paged_tree_attention(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
+                             int q_heads, const uint64_t* masks, int max_keys, float scale,
+                             void* workspace, void* out, float* lse, void* stream);
+
+/* Acceptance of drafted tokens: rows of K and V of an accepted path moved into place, from
+ * starts[b] + path[b][j] to starts[b] + j, in all caches (the layers of a model: descriptions that
+ * differ in their pages alone; read by the host before the call returns).
+ * Either with parents, drafts and targets, contiguous [B, T] (int32, int64, int64): node 0 is taken,
+ * then the first child whose drafts equals the targets of the node taken last, while there is one.
+ * accepted: int32 [B], how many were taken (0 without live tokens); path_out: int32 [B, T], their
+ * indexes, then -1; following: int64 [B], the targets of the last one, or -1.
+ * Or with path_in, int32 [B, T]: live indexes that ascend; it ends where one does not (the others
+ * NULL). Rows from or to a position without a place are not moved. T is at most 256. */
+int spx_paged_keep_path(const spx_paged_cache* caches, int cache_count, const int32_t* parents,
+                        const int64_t* drafts, const int64_t* targets, const int32_t* path_in,
+                        int32_t* accepted, int32_t* path_out, int64_t* following, void* stream);
+
+/* ---------------------------------------------- paged KV cache: eviction */
+
+/* weights[b][kvh][p] += the sum over the rows (token i, query head of kvh) that see position p of
+ * exp(scale q k_p - lse): tokens, positions and q as in spx_paged_attention, lse fp32 [B, T, Hq]
+ * contiguous as it gives it. weights: fp32, rows of row_stride (at least table_width * page_size)
+ * elements, [B, Hkv, row_stride] contiguous. Rows with an LSE of -inf and tokens that are not live add
+ * nothing; positions without a place are left as they are. Values of V are not read. workspace:
+ * spx_paged_accumulate_weights_workspace_bytes(...) bytes, 16-byte aligned (0: none, -1: unsupported
+ * shape). The order of the sums depends on the sizes and lengths only. */
+int64_t spx_paged_accumulate_weights_workspace_bytes(const spx_paged_cache* cache, int q_heads);
+int spx_paged_accumulate_weights(const spx_paged_cache* cache, const void* q, const int64_t* q_strides,
+                                 int q_heads, const float* lse, float scale, void* workspace,
+                                 float* weights, int64_t row_stride, void* stream);
+
+/* Each KV head of a sequence of more than `budget` tokens keeps that many: those whose position in the
+ * text is below `sinks` or at least seen[b] - recent, then those of the largest weight, the lower slot
+ * first among equals (NaN is the least of all). Tokens kept in slots below the budget stay there; the
+ * j-th of the other slots receives the j-th of the tokens kept behind it: K, V, weight and position.
+ * cache: starts holds the lengths (tokens held; negative: a free slot), tokens is 1, counts is not read.
+ * positions: int32, as weights, or NULL: -1 for all; slot s without one (negative) has position
+ * seen[b] - length + s. seen: int32 [B], tokens of the text so far, or NULL: the lengths. recent + sinks
+ * is at most the budget. weights_out, positions_out: the new values, 0 and -1 from the new length on
+ * (they may be the inputs); lengths_out: int32 [B]. Sequences within the budget, longer than the page
+ * table reaches, or with a token that has no place, keep all they have. Pages of the first `budget`
+ * slots are written: they belong to one sequence. workspace: spx_paged_evict_workspace_bytes(...)
+ * bytes, 8-byte aligned. */
+int64_t spx_paged_evict_workspace_bytes(const spx_paged_cache* cache, int budget);
+int spx_paged_evict(const spx_paged_cache* cache, const float* weights, const int32_t* positions,
+                    int64_t row_stride, const int32_t* seen, int budget, int recent, int sinks,
+                    void* workspace, float* weights_out, int32_t* positions_out, int32_t* lengths_out,
+                    void* stream);
 
 /* ----------------------------------------------------------- accounting */
 
