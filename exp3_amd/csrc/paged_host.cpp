@@ -188,6 +188,14 @@ at::Tensor rows(const at::Tensor& x, const char* name) {
   return (x.is_neg() ? x.resolve_neg() : x).contiguous().detach();
 }
 
+// A contiguous copy where the tensor is not contiguous or lazily negated.
+at::Tensor plain(const at::Tensor& x, const char* name) {
+  require_no_gradient(x, name);
+  if (!x.is_neg() && x.is_contiguous()) return x;
+  c10::AutoGradMode no_grad(false);
+  return (x.is_neg() ? x.resolve_neg() : x).contiguous().detach();
+}
+
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const c10::Device& device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
@@ -564,7 +572,12 @@ PyObject* accumulate(PyObject*, PyObject* const* args, Py_ssize_t n) {
         q.size(2) % d.c.kv_heads != 0)
       refuse("q ", q.sizes(), " does not fit a cache of ", d.c.kv_heads, " heads of ", d.c.head_dim);
     const at::Tensor& weights = ledger(d, args[7], "weights", at::kFloat);
-    const at::Tensor& lse = exactly(args[9], "lse", at::kFloat, q.sizes().slice(0, 3), d.device);
+    const at::Tensor& lse_in = tensor(args[9], "lse", true);
+    if (lse_in.scalar_type() != at::kFloat || lse_in.sizes() != q.sizes().slice(0, 3))
+      refuse("lse must be a float32 tensor of shape ", q.sizes().slice(0, 3), ", got ",
+             lse_in.sizes(), " ", lse_in.scalar_type());
+    require_device(lse_in, d.device);
+    const at::Tensor lse = plain(lse_in, "lse");
     const double scale = PyFloat_AsDouble(args[10]);
     if (scale == -1.0 && PyErr_Occurred()) throw std::bad_exception();
     void* stream = reinterpret_cast<void*>(integer(args[11]));

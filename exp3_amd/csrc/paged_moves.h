@@ -20,6 +20,13 @@ struct MoveArgs {
   PagePointers pages;
   const int32_t* counts;                 // [B, Hkv] moves of each list
   const u32x2* moves;                    // [B, Hkv, room] (to, from)
+  int64_t row;                           // elements of a row of weights and positions
+  const int32_t* lengths;                // [B]: new lengths (the map's starts are the old ones)
+  const int32_t* seen;                   // [B], or null: the old lengths
+  const float* weights;                  // [B, Hkv, row]
+  const int32_t* positions;              // the same, or null
+  float* weights_out;                    // these may be those
+  int32_t* positions_out;
 };
 
 int launch_moves(const MoveArgs& a, int head_dim, hipStream_t st);

@@ -159,7 +159,8 @@ __global__ __launch_bounds__(kPathThreads) void paged_path_kernel(PathArgs a, in
 
 // ---------------------------------------------------------------------- evictions
 
-// Rows `moves` of the lists of each (sequence, head): from the second place to the first.
+// The tokens of the list of each (sequence, head) moved, from the second slot to the first, and the
+// ledger cleared behind the old length.
 template <int D, bool kFour>
 __global__ __launch_bounds__(kMoveThreads) void paged_move_kernel(MoveArgs a) {
   using Part = RowPart<D, kFour>;
@@ -176,14 +177,25 @@ __global__ __launch_bounds__(kMoveThreads) void paged_move_kernel(MoveArgs a) {
     const int b = (int)(bh / a.map.kv_heads), head = (int)(bh % a.map.kv_heads);
     const int count = min(a.counts[bh], a.room);
     const u32x2* list = a.moves + bh * a.room;
+    const int length = a.map.starts[b], text = a.seen ? a.seen[b] : length;
+    for (int64_t i = max(length, 0) + blockIdx.x * kMoveThreads + threadIdx.x; i < a.row;
+         i += gridDim.x * kMoveThreads) {
+      a.weights_out[bh * a.row + i] = 0.0f;
+      a.positions_out[bh * a.row + i] = -1;
+    }
     for (int i0 = first; i0 < count; i0 += kAtOnce * step) {
       Part k[kAtOnce], v[kAtOnce];
       int64_t to[kAtOnce];
+      u32x2 move[kAtOnce];
+      float weight[kAtOnce];
+      int told[kAtOnce];
 #pragma unroll
       for (int n = 0; n < kAtOnce; ++n) {
-        const u32x2 move = list[min(i0 + n * step, count - 1)];
-        to[n] = a.map.row(max(a.map.page(b, (int)move[0]), 0), head, (int)move[0]);
-        const int64_t from = a.map.row(max(a.map.page(b, (int)move[1]), 0), head, (int)move[1]);
+        move[n] = list[min(i0 + n * step, count - 1)];
+        to[n] = a.map.row(max(a.map.page(b, (int)move[n][0]), 0), head, (int)move[n][0]);
+        const int64_t from = a.map.row(max(a.map.page(b, (int)move[n][1]), 0), head, (int)move[n][1]);
+        weight[n] = a.weights[bh * a.row + move[n][1]];
+        told[n] = a.positions ? a.positions[bh * a.row + move[n][1]] : -1;
         k[n].load(keys, key_scales, from, piece);
         v[n].load(values, value_scales, from, piece);
       }
@@ -192,6 +204,13 @@ __global__ __launch_bounds__(kMoveThreads) void paged_move_kernel(MoveArgs a) {
         if (i0 + n * step >= count) break;
         k[n].store(keys, key_scales, to[n], piece);
         v[n].store(values, value_scales, to[n], piece);
+        if (piece == 0) {
+          a.weights_out[bh * a.row + move[n][0]] = weight[n];
+          a.positions_out[bh * a.row + move[n][0]] =
+              told[n] >= 0 ? told[n] : text - length + (int)move[n][1];
+          a.weights_out[bh * a.row + move[n][1]] = 0.0f;
+          a.positions_out[bh * a.row + move[n][1]] = -1;
+        }
       }
     }
   }
@@ -202,7 +221,8 @@ int launch_moves(const MoveArgs& a, int head_dim, hipStream_t st) {
   const int64_t rows = (int64_t)a.batch * a.map.kv_heads;
   const int per_block = kMoveThreads / kWave * 4;
   const int64_t most = std::max<int64_t>(1, 4096 / rows);
-  const dim3 grid((unsigned)std::min<int64_t>(most, (a.room + per_block - 1) / per_block),
+  const int64_t clears = (a.row + 8 * kMoveThreads - 1) / (8 * kMoveThreads);
+  const dim3 grid((unsigned)std::min<int64_t>(most, std::max<int64_t>(clears, (a.room + per_block - 1) / per_block)),
                   (unsigned)std::min<int64_t>(rows, 65535));
   if (head_dim == 128) {
     if (four) paged_move_kernel<128, true><<<grid, kMoveThreads, 0, st>>>(a);

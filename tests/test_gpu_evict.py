@@ -165,10 +165,30 @@ def test_evict(gpu, budget, recent, sinks, bits, dim, page, in_place):
                  in_place=in_place)
 
 
-@pytest.mark.parametrize("keys,budget", ((1500, 700), (3000, 100), (5000, 4999), (2049, 1025)))
+@pytest.mark.parametrize("keys,budget", ((1500, 700), (3000, 100), (5000, 4999), (2049, 1025),
+                                         (4097, 2000), (32768, 9000), (33001, 20000), (50000, 300)))
 def test_evict_long(gpu, keys, budget):
+    """Rows of several digits' walks: ranks in LDS (up to 4096 and 32768 slots) and formed anew."""
     s = ref.make(72, 2, 1, 2, 1, 128, 64, -(-keys // 64), (0, 0))
     _check_evict(s, (keys, keys - 333), budget, budget // 10, 3)
+
+
+@pytest.mark.parametrize("keys", (700, 9000, 40000))
+@pytest.mark.parametrize("value", (0.0, 1.5, math.nan))
+def test_evict_ties(gpu, keys, value):
+    """All weights alike, or all but a few: the lowest slots stay."""
+    s = ref.make(78, 1, 1, 1, 1, 128, 128, -(-keys // 128), (0,))
+    cache, table, _, _ = ref.on_gpu(s)
+    weights = torch.full((1, 1, s.table.shape[1] * 128), value, device="cuda")
+    lengths = torch.tensor([keys], dtype=torch.int32, device="cuda")
+    budget = keys // 2
+    left, _, positions = paged.evict_tokens(cache, table, lengths, weights, budget, recent=10)
+    want = list(range(budget - 10)) + list(range(keys - 10, keys))
+    assert int(left[0]) == budget and positions[0, 0, :budget].tolist() == want
+    weights[0, 0, keys - 100:keys - 50:2] = math.inf
+    positions = paged.evict_tokens(cache, table, lengths, weights, budget)[2]
+    assert positions[0, 0, :budget].tolist() == \
+        list(range(budget - 25)) + list(range(keys - 100, keys - 50, 2))
 
 
 def test_evict_left_alone(gpu):
