@@ -54,7 +54,10 @@ HIPCC_FLAGS = [
 # the parked logits of up to 12 chunks (192 registers); the stored-chunk loop must
 # be unrolled in full (its register array indexed by constants), which a 12-chunk
 # body exceeds under the default unroll threshold (the array then went to scratch).
+# paged_tree.hip: as attn256.hip, O and Q at D = 256 (4 trees of 26 behind up to 12001 tokens, 4 bits,
+# 51.2 -> 44.5 us; D = 128 is as fast either way).
 EXTRA_FLAGS = {"attn256.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+               "paged_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "route.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                "selectors.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form",
                                  "-mllvm", "-pragma-unroll-threshold=1000000"]}
