@@ -40,6 +40,25 @@ __device__ __forceinline__ T global_load(GlobalBytes p, uint32_t offset) {
   return *(const __attribute__((address_space(1))) T*)(p + offset);
 }
 
+typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
+
+template <typename T>
+__device__ __forceinline__ T lds_load(LdsBytes p, int offset) {
+  return *(const __attribute__((address_space(3))) T*)(p + offset);
+}
+template <typename T>
+__device__ __forceinline__ void lds_store(LdsBytes p, int offset, const T& x) {
+  *(__attribute__((address_space(3))) T*)(p + offset) = x;
+}
+
+// All copies past the registers but the last kLeft are complete (any other loads under way make it
+// stricter).
+template <int kLeft>
+__device__ __forceinline__ void wait_copies() {
+  static_assert(kLeft < 64, "counted in six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+
 // The start of a tile, opaque: added to a lane's offset it is the scalar base of the load. Seen
 // through, the compiler held lane offset + head in two vector registers for each of the loads.
 __device__ __forceinline__ GlobalBytes tile_base(GlobalBytes p) {

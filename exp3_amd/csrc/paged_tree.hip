@@ -171,17 +171,6 @@ __device__ __forceinline__ int tree_swizzle(int row) {
   return (row & 3) << 2 | ((row ^ row >> 2) & 3);
 }
 
-typedef __attribute__((address_space(3))) uint8_t* LdsBytes;
-
-template <typename T>
-__device__ __forceinline__ T lds_load(LdsBytes p, int offset) {
-  return *(const __attribute__((address_space(3))) T*)(p + offset);
-}
-template <typename T>
-__device__ __forceinline__ void lds_store(LdsBytes p, int offset, const T& x) {
-  *(__attribute__((address_space(3))) T*)(p + offset) = x;
-}
-
 // Four times 16 bytes a lane from base + offset[i] to to + 1024 i + 16 lane, past the registers. From
 // assembly: the compiler would wait for its own form of it before any other read of LDS.
 __device__ __forceinline__ void copy_to_lds(GlobalBytes base, const uint32_t* offset, LdsBytes to) {
@@ -207,13 +196,6 @@ __device__ __forceinline__ void copy_to_lds(GlobalBytes base, const uint32_t* of
       : "s"(m0), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3]), "s"(base)
       : "memory", "scc");
 #endif
-}
-
-// All copies but the last kLeft are complete (any other loads under way make it stricter).
-template <int kLeft>
-__device__ __forceinline__ void wait_copies() {
-  static_assert(kLeft < 64, "counted in six bits");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
 }
 
 // 16 rows of K or V on their way into LDS.

@@ -2,15 +2,16 @@
 //
 //   weights[b, kvh, p] += sum over rows (i, h of the group) that see p of exp(scale q k_p - lse).
 //
-// Columns n = i group + h of a KV head, 16 to a matrix tile; a wave holds 32 keys and walks the
-// columns. v_mfma_f32_16x16x32_bf16 with Q as A and K as B operand: the scores of a key lie in one
-// lane's four registers, so the sum over columns is in the lane but for the lane groups at the end.
-// Q comes from LDS, 128 columns at a time, K straight from the pages into registers.
+// Columns n = i group + h of a KV head, 16 to a matrix tile. v_mfma_f32_16x16x32_bf16 with Q as A and
+// K as B operand: the scores of a key lie in one lane's four registers, so the sum over columns is
+// in the lane but for the four lane groups at the end. K comes straight from the pages into registers.
 //
-// Work: a stream is a (sequence, KV head, 128 or 256 keys), its units chunks of 128 columns. The units
-// of all streams are dealt in equal runs to one grid; where a stream has one unit (decode steps) every
-// workgroup adds to the weights itself, else streams that cross workgroups leave at most two partial
-// sums per workgroup, added in order by a second kernel.
+// With s and L the scale and the LSE in units of log 2, each rounded once (s', L'), a weight is
+//   2^(s x - L) = 2^(s' x - L') 2^e,   e = (s - s') x - (L - L') = (s / s' - 1) L' - (L - L') nearly,
+// as s' x is L' where the weight counts: the columns' factor 2^e makes up for both roundings.
+//
+// Two kernels: up to 16 columns (decode steps) a wave has Q in registers and walks the keys by itself,
+// bound by the pages' bytes; else 4 waves hold 256 keys and walk the columns through LDS, 64 at a time.
 #include <algorithm>
 #include <cmath>
 
@@ -18,9 +19,19 @@
 
 namespace spx {
 
-constexpr int kPwCols = 128;             // columns of a unit
+constexpr int kPwCols = 64;              // columns of a unit
+constexpr int kPwFewCols = 16;           // at most: a wave by itself
 constexpr int kPwCus = 256;
-constexpr int kPwTiles = 2;              // of 16 keys, a wave's
+constexpr int kPwWaves = 4;              // of a workgroup
+constexpr int kPwTiles = 4;              // of 16 keys, a wave's
+constexpr int kPwKeys = 16 * kPwTiles * kPwWaves;
+constexpr int kPwWhole = 8;              // chunks up to which a block of keys has one workgroup
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// Tiles of 16 keys that a wave has under way for few columns: as many as two sets of registers hold.
+template <int D, bool kFour>
+constexpr int kPwFewTiles = kFour || D == 128 ? 4 : 2;
 
 struct PagedWeightArgs {
   PagedMap map;
@@ -34,12 +45,13 @@ struct PagedWeightArgs {
   int batch, tokens, q_heads, kv_heads, group;
   int cols, chunks;                      // tokens x group, chunks of them at most
   int blocks;                            // blocks of keys that the table reaches
-  int grid;
+  int whole;                             // blocks are not shared by workgroups
+  int grid;                              // workgroups, or waves, that share the work
   double inv_grid, inv_group;
-  float scale, scale_low;                // scale log2(e) in two parts
+  float scale, scale_rest;               // scale log2(e), rounded; what of it is missing, relative
   float* weights;                        // [B, Hkv, row]
   int64_t row;
-  float* part;                           // [2 grid][keys of a block]
+  float* part;                           // [2 grid][kPwKeys]
   u32x2* parts;                          // [B, Hkv, blocks]
 };
 
@@ -60,7 +72,8 @@ struct WeightLengths {
   }
 };
 
-struct WeightScan {                      // the units of 64 sequences, one a lane
+// What is dealt to the workgroups: chunks of columns of the blocks of keys, or whole blocks.
+struct WeightScan {                      // of 64 sequences, one a lane
   int units, sum;
   __device__ __forceinline__ void load(const PagedWeightArgs& a, int block, int b) {
     WeightLengths x;
@@ -70,7 +83,7 @@ struct WeightScan {                      // the units of 64 sequences, one a lan
       if (a.map.counts) count = a.map.counts[b];
     }
     x.of(a, block, start, count);
-    units = x.blocks * x.chunks * a.kv_heads;
+    units = x.chunks == 0 ? 0 : x.blocks * (a.whole ? 1 : x.chunks) * a.kv_heads;
     sum = wave_prefix(units);
   }
   __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(sum, kWave - 1); }
@@ -95,8 +108,9 @@ struct WeightUnit {
     before += __builtin_amdgcn_readlane(scan.sum - scan.units, l);
     x.load(a, block, b);
     if (x.blocks <= 0 || x.chunks <= 0 || u < before) return false;
-    const int stream = (u - before) / x.chunks;
-    chunk = u - before - stream * x.chunks;
+    const int each = a.whole ? 1 : x.chunks;
+    const int stream = (u - before) / each;
+    chunk = u - before - stream * each;
     kvh = stream / x.blocks;
     at = stream - kvh * x.blocks;
     return kvh < a.kv_heads;
@@ -132,175 +146,381 @@ struct WeightRun {
   }
 };
 
-template <int D, bool kFour, int W>
-__global__ __launch_bounds__(64 * W) void paged_weight_kernel(PagedWeightArgs a) {
-  constexpr int kBlockKeys = 16 * kPwTiles * W, KK = D / 32, kRowChunks = D / 8;
-  __shared__ __align__(16) uint16_t qs[kPwCols * D];
-  __shared__ __align__(16) float lse_hi[kPwCols], lse_lo[kPwCols];
-  __shared__ __align__(16) int last_key[kPwCols];               // that a column sees; -1: none
-  const int tid = threadIdx.x, lane = tid & 63, w = first_lane(tid >> 6);
+// A column's LSE in units of log 2, rounded, the factor that makes up for the roundings, and the last
+// key that it sees (-1: none).
+struct WeightColumn {
+  float hi, factor;
+  int last;
+  __device__ __forceinline__ WeightColumn(const PagedWeightArgs& a, float lse, int last_key) {
+    hi = lse * kLog2e;
+    // log2(e) is kLog2e + 1.925963033500e-8
+    const float lo = __builtin_fmaf(lse, kLog2e, -hi) + lse * 1.925963033500e-8f;
+    // (finite whatever the LSE is: it multiplies zeros too)
+    const float e = __builtin_fmaf(hi, a.scale_rest, -lo);
+    factor = __builtin_fabsf(e) < 1.0f ? exp2_fast(e) : 1.0f;
+    last = lse == -INFINITY ? -1 : last_key;
+  }
+};
+
+// Sums over the four lane groups: tile g's in group g (of two tiles: g / 2's).
+__device__ __forceinline__ float weight_sums(const float (&x)[4]) {
+  float y[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[i]), __float_as_uint(x[i + 2]),
+                                                    false, false);
+    y[i] = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  }
+  const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(y[0]), __float_as_uint(y[1]), false,
+                                                  false);
+  return __uint_as_float(h[0]) + __uint_as_float(h[1]);
+}
+__device__ __forceinline__ float weight_sums(const float (&x)[2]) {
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x[0]), __float_as_uint(x[1]), false,
+                                                  false);
+  const float y = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+  return y + __shfl_xor(y, 16);
+}
+
+// ------------------------------------------------------------------ few columns
+
+template <int D, bool kFour>
+__global__ __launch_bounds__(64 * kPwWaves, kFour && D == 128 ? 4 : 2) void
+paged_weight_few_kernel(PagedWeightArgs a) {
+  constexpr int T = kPwFewTiles<D, kFour>, kKeys = 16 * T, KK = D / 32;
+  const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   WeightScan scan;
-  scan.load(a, kBlockKeys, lane);
+  scan.load(a, kKeys, lane);
   int total = scan.total();
   for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
     WeightScan more;
-    more.load(a, kBlockKeys, b0 + lane);
+    more.load(a, kKeys, b0 + lane);
+    total += more.total();
+  }
+  const WeightRun run(total, a.grid, a.inv_grid);
+  const int wave = blockIdx.x * kPwWaves + w;
+  int u = run.begin(wave);
+  const int end = run.begin(wave + 1);
+  WeightUnit s, next;                    // unit u and u + 1
+  if (u >= end || !s.find(a, kKeys, lane, scan, u)) return;
+  // lane t: page of tile t % T
+  const auto fetch_ids = [&](const WeightUnit& s) {
+    const int64_t p = (int64_t)s.at * kKeys + lane % T * 16;
+    return a.map.page(s.b, (int)min(p, (int64_t)s.x.keys - 1));
+  };
+  struct Keys {
+    KeyTile<D, kFour> tile[T];
+    float old;                           // the lane's key: its weight
+    float* at;                           // and where it stands, null: nowhere
+  };
+  const int mine = T == 4 ? g : g >> 1;  // the lane's tile at the end
+  const auto load = [&](Keys& k, const WeightUnit& s, int ids) {
+    const HeadPages<D, kFour> pages(a, s.kvh);
+    const int key0 = s.at * kKeys;
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      k.tile[t].load(pages, pages.row(max(__builtin_amdgcn_readlane(ids, t), 0), key0 + 16 * t), c, g);
+    const uint64_t lost = __ballot(ids < 0);
+    const int p = key0 + 16 * mine + c;
+    const bool stands = p < s.x.keys && !(lost >> mine & 1) && (T == 4 || g % 2 == 0);
+    k.at = stands ? a.weights + ((int64_t)s.b * a.kv_heads + s.kvh) * a.row + p : nullptr;
+    k.old = stands ? *k.at : 0.0f;
+  };
+  u32x4 q[KK];
+  float hi[4], factor[4];
+  int last[4];
+  int held_b = -1, held_kvh = 0;
+  int ids = fetch_ids(s);
+  const auto step = [&](Keys& now, Keys& coming) {
+    const WeightUnit at = s;
+    if (at.b != held_b || at.kvh != held_kvh) {
+      held_b = at.b;
+      held_kvh = at.kvh;
+      const int live = at.x.live * a.group;
+      const auto place = [&](int n, int& token, int& head) {
+        n = min(n, live - 1);
+        token = divide(n, a.group, a.inv_group);
+        head = at.kvh * a.group + n - token * a.group;
+      };
+      int token, head;
+      place(c, token, head);
+      const uint16_t* row = a.q + at.b * a.qs_b + token * a.qs_t + head * a.qs_h;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk)
+        q[kk] = *reinterpret_cast<const u32x4*>(row + KeyTile<D, kFour>::dim(kk, g));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        place(4 * g + r, token, head);
+        const WeightColumn x(a, a.lse[((int64_t)at.b * a.tokens + token) * a.q_heads + head],
+                             4 * g + r < live ? at.x.start + token : -1);
+        hi[r] = x.hi;
+        factor[r] = x.factor;
+        last[r] = x.last;
+      }
+    }
+    const bool more = ++u < end && next.next(a, kKeys);
+    if (more) {
+      load(coming, next, ids);
+      s = next;
+    }
+    if (more && u + 1 < end) {
+      WeightUnit after = next;
+      if (after.next(a, kKeys)) ids = fetch_ids(after);
+    }
+    const int key0 = at.at * kKeys + c;
+    float acc[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      f32x4 x{};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) x = mfma16(q[kk], now.tile[t].operand(kk, g), x);
+      acc[t] = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = exp2_fast(__builtin_fmaf(x[r], a.scale, -hi[r]));
+        acc[t] = __builtin_fmaf(key0 + 16 * t <= last[r] ? p : 0.0f, factor[r], acc[t]);
+      }
+    }
+    const float sum = weight_sums(acc);
+    if (now.at) *now.at = now.old + sum;
+    return more;
+  };
+  Keys one, two;
+  load(one, s, ids);
+  next = s;
+  if (u + 1 < end) {
+    WeightUnit after = next;
+    if (after.next(a, kKeys)) ids = fetch_ids(after);
+  }
+  while (step(one, two) && step(two, one)) {}
+}
+
+// ----------------------------------------------------------------- many columns
+
+// Four times 16 bytes a lane from from[i] to to + 1024 i + 16 lane, past the registers.
+__device__ __forceinline__ void copy_rows_to_lds(const uint64_t (&from)[4], LdsBytes to) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)to);
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %5, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(m0), "v"(from[0]), "v"(from[1]), "v"(from[2]), "v"(from[3])
+      : "memory", "scc");
+#endif
+}
+
+// A unit's columns in LDS: rows of Q, 16-byte chunks exchanged within a row by an XOR with row % 16.
+template <int D>
+struct WeightColumns {
+  static constexpr int kLanes = D / 8, kRows = kWave / kLanes, kCopies = 16 / kRows;
+  uint16_t q[kPwCols * D];
+  float hi[kPwCols], factor[kPwCols];
+  int last[kPwCols];
+  int least[4], most[4];                 // of last in 16 columns: every one sees it, one does
+};
+
+template <int D, bool kFour>
+__global__ __launch_bounds__(64 * kPwWaves, D == 128 ? 3 : 2) void
+paged_weight_kernel(PagedWeightArgs a) {
+  constexpr int T = kPwTiles, KK = D / 32;
+  using Columns = WeightColumns<D>;
+  __shared__ __align__(16) Columns columns[2];
+  const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  WeightScan scan;
+  scan.load(a, kPwKeys, lane);
+  int total = scan.total();
+  for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
+    WeightScan more;
+    more.load(a, kPwKeys, b0 + lane);
     total += more.total();
   }
   const WeightRun run(total, a.grid, a.inv_grid);
   const int begin = run.begin(blockIdx.x), end = run.begin(blockIdx.x + 1);
   WeightUnit s;
-  if (begin >= end || !s.find(a, kBlockKeys, lane, scan, begin)) return;
-  int held_b = -1, held_kvh = 0, held_chunk = 0;                // whose columns are in LDS
-  KeyTile<D, kFour> key[kPwTiles];
-  bool placed[kPwTiles];
-  const auto load_keys = [&](const WeightUnit& s) {
-    const HeadPages<D, kFour> pages(a, s.kvh);
-    const int key0 = s.block() * kBlockKeys + w * 16 * kPwTiles;
+  if (begin >= end || !s.find(a, kPwKeys, lane, scan, begin)) return;
+  // A wave brings 16 columns in; finish() after the copies are there.
+  float lse = 0.0f;
+  int last_key = 0;
+  const auto stage = [&](const WeightUnit& s, Columns& to) {
+    const int n = s.chunk * kPwCols + 16 * w + c, m = min(n, s.x.live * a.group - 1);
+    const int token = divide(m, a.group, a.inv_group), head = s.kvh * a.group + m - token * a.group;
+    const uint64_t row = (uint64_t)(a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h);
+    lse = a.lse[((int64_t)s.b * a.tokens + token) * a.q_heads + head];
+    last_key = n == m ? s.x.start + token : -1;
+    const LdsBytes place = (LdsBytes)to.q + 16 * w * 2 * D;
 #pragma unroll
-    for (int t = 0; t < kPwTiles; ++t) {
-      const int p = key0 + 16 * t;
-      const int id = a.map.uniform_page(s.b, min(p, s.x.keys - 1));
-      placed[t] = id >= 0;
-      key[t].load(pages, pages.row(max(id, 0), p), c, g);
+    for (int i = 0; i < Columns::kCopies; i += 4) {
+      uint64_t from[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = Columns::kRows * (i + j) + lane / Columns::kLanes;
+        from[j] = ((uint64_t)(uint32_t)__shfl((int)(row >> 32), r) << 32 |
+                   (uint32_t)__shfl((int)row, r)) +
+                  ((lane % Columns::kLanes) ^ r) * 16;
+      }
+      copy_rows_to_lds(from, place + 1024 * i);
     }
   };
+  const auto finish = [&](Columns& to) {
+    const WeightColumn x(a, lse, last_key);
+    int least = x.last, most = x.last;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      least = min(least, __shfl_xor(least, d));
+      most = max(most, __shfl_xor(most, d));
+    }
+    if (lane < 16) {
+      to.hi[16 * w + lane] = x.hi;
+      to.factor[16 * w + lane] = x.factor;
+      to.last[16 * w + lane] = x.last;
+    }
+    if (lane == 0) {
+      to.least[w] = least;
+      to.most[w] = most;
+    }
+    wait_copies<0>();
+  };
+  u32x4 key[T][KK];
+  bool placed = false;                   // the lane's key of tile g
+  const auto load_keys = [&](const WeightUnit& s) {
+    const HeadPages<D, kFour> pages(a, s.kvh);
+    const int key0 = s.block() * kPwKeys + w * 16 * T;
+    const int64_t p = (int64_t)key0 + lane % T * 16;
+    const int ids = a.map.page(s.b, (int)min(p, (int64_t)s.x.keys - 1));
+    KeyTile<D, kFour> tile[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+      tile[t].load(pages, pages.row(max(__builtin_amdgcn_readlane(ids, t), 0), key0 + 16 * t), c, g);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) key[t][kk] = tile[t].operand(kk, g);
+    placed = !(__ballot(ids < 0) >> g & 1);
+  };
+  float acc[T] = {};
+  const auto compute = [&](const Columns& q, int key0, int ct, bool masked) {
+    const LdsBytes row = (LdsBytes)q.q + (16 * ct + c) * 2 * D;
+    f32x4 x[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) x[t] = f32x4{};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int piece = KeyTile<D, kFour>::dim(kk, g) / 8;
+      const u32x4 qk = lds_load<u32x4>(row, (piece ^ c) << 4);
+#pragma unroll
+      for (int t = 0; t < T; ++t) x[t] = mfma16(qk, key[t][kk], x[t]);
+    }
+    const f32x4 hi = *reinterpret_cast<const f32x4*>(q.hi + 16 * ct + 4 * g);
+    const f32x4 factor = *reinterpret_cast<const f32x4*>(q.factor + 16 * ct + 4 * g);
+    i32x4 last{};
+    if (masked) last = *reinterpret_cast<const i32x4*>(q.last + 16 * ct + 4 * g);
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float p = exp2_fast(__builtin_fmaf(x[t][r], a.scale, -hi[r]));
+        if (masked) p = key0 + 16 * t + c <= last[r] ? p : 0.0f;
+        acc[t] = __builtin_fmaf(p, factor[r], acc[t]);
+      }
+  };
+  int buffer = 0;
+  stage(s, columns[0]);
   load_keys(s);
-  float acc[kPwTiles] = {};
-  bool fresh = true;                     // acc holds nothing of the stream
-  int first = s.chunk;                   // the first of its chunks here
+  finish(columns[0]);
+  block_sync();
+  bool fresh = true;                     // no partial sum left yet
+  int first = s.chunk;                   // the first of the block's chunks here
   for (int u = begin;;) {
-    const int block = s.block(), key0 = block * kBlockKeys + w * 16 * kPwTiles;
-    if (s.b != held_b || s.kvh != held_kvh || s.chunk != held_chunk) {
-      block_sync();                      // the last columns have been read
-      held_b = s.b;
-      held_kvh = s.kvh;
-      held_chunk = s.chunk;
-      const int n0 = s.chunk * kPwCols;
-      const int rows = min((s.x.live * a.group - n0 + 15) & ~15, kPwCols);
-      for (int i = tid; i < rows * kRowChunks; i += 64 * W) {
-        const int n = n0 + i / kRowChunks, piece = i % kRowChunks;
-        const int token = divide(n, a.group, a.inv_group);
-        const int head = s.kvh * a.group + n - token * a.group;
-        u32x4 x{};
-        if (token < s.x.live)
-          x = *reinterpret_cast<const u32x4*>(a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h +
-                                              8 * piece);
-        *reinterpret_cast<u32x4*>(qs + (n - n0) * D + ((piece ^ (n & 15)) << 3)) = x;
-      }
-      for (int i = tid; i < rows; i += 64 * W) {
-        const int n = n0 + i, token = divide(n, a.group, a.inv_group);
-        float lse = -INFINITY;
-        if (token < s.x.live)
-          lse = a.lse[((int64_t)s.b * a.tokens + token) * a.q_heads + s.kvh * a.group + n -
-                      token * a.group];
-        const float hi = lse * kLog2e;
-        // log2(e) is kLog2e + 1.925963033500e-8
-        const float lo = __builtin_fmaf(lse, kLog2e, -hi) + lse * 1.925963033500e-8f;
-        lse_hi[i] = hi;
-        lse_lo[i] = __builtin_isinf(hi) ? 0.0f : lo;
-        last_key[i] = lse == -INFINITY ? -1 : s.x.start + token;
-      }
-      block_sync();
-    }
-    const int n0 = s.chunk * kPwCols, columns = min(s.x.live * a.group - n0, kPwCols);
-    for (int ct = 0; ct < columns; ct += 16) {
-      const int last_token = divide(n0 + min(ct + 16, columns) - 1, a.group, a.inv_group);
-      if (key0 > s.x.start + last_token) continue;
-      f32x4 x[kPwTiles];
-#pragma unroll
-      for (int t = 0; t < kPwTiles; ++t) x[t] = f32x4{};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        const int piece = KeyTile<D, kFour>::dim(kk, g) / 8;
-        const u32x4 q = *reinterpret_cast<const u32x4*>(qs + (ct + c) * D + ((piece ^ c) << 3));
-#pragma unroll
-        for (int t = 0; t < kPwTiles; ++t) x[t] = mfma16(q, key[t].operand(kk, g), x[t]);
-      }
-      const f32x4 hi = *reinterpret_cast<const f32x4*>(lse_hi + ct + 4 * g);
-      const f32x4 lo = *reinterpret_cast<const f32x4*>(lse_lo + ct + 4 * g);
-      typedef int i32x4 __attribute__((ext_vector_type(4)));
-      const i32x4 see = *reinterpret_cast<const i32x4*>(last_key + ct + 4 * g);
-#pragma unroll
-      for (int t = 0; t < kPwTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = __builtin_fmaf(x[t][r], a.scale, -hi[r]) +
-                          __builtin_fmaf(x[t][r], a.scale_low, -lo[r]);
-          const float p = exp2_fast(y);
-          acc[t] += key0 + 16 * t + c <= see[r] ? p : 0.0f;
-        }
-    }
     const bool last = s.chunk == s.x.chunks - 1;
-    ++u;
-    if (last || u >= end) {
-      float sum[kPwTiles];
+    if (last || !a.whole) ++u;
+    WeightUnit next = s;
+    const bool more = u < end && next.next(a, kPwKeys);
+    const bool other = more && (next.chunk != s.chunk || next.kvh != s.kvh || next.b != s.b);
+    if (other) stage(next, columns[buffer ^ 1]);
+    const int block = s.block(), key0 = block * kPwKeys + w * 16 * T;
+    const Columns& q = columns[buffer];
+    const i32x4 least = *reinterpret_cast<const i32x4*>(q.least);
+    if (first_lane(min(min(least[0], least[1]), min(least[2], least[3]))) >= key0 + 16 * T - 1) {
 #pragma unroll
-      for (int t = 0; t < kPwTiles; ++t) {
-        sum[t] = acc[t] + __shfl_xor(acc[t], 16);
-        sum[t] += __shfl_xor(sum[t], 32);
-        acc[t] = 0.0f;
-      }
+      for (int ct = 0; ct < kPwCols / 16; ++ct) compute(q, key0, ct, false);
+    } else {
+      for (int ct = 0; ct < kPwCols / 16; ++ct)
+        if (first_lane(q.most[ct]) >= key0) compute(q, key0, ct, true);
+    }
+    if (last || !more) {
+      const float sum = weight_sums(acc);
+#pragma unroll
+      for (int t = 0; t < T; ++t) acc[t] = 0.0f;
       const bool whole = last && first == 0;
       const int slot = 2 * blockIdx.x + (fresh ? 0 : 1);
-      const int p = key0 + 16 * g + c;
-      const float mine = g == 0 ? sum[0] : sum[1];
-      if (g < kPwTiles) {
-        if (whole) {
-          if (p < s.x.keys && (g == 0 ? placed[0] : placed[1]))
-            a.weights[((int64_t)s.b * a.kv_heads + s.kvh) * a.row + p] += mine;
-        } else {
-          a.part[(int64_t)slot * kBlockKeys + w * 16 * kPwTiles + 16 * g + c] =
-              (g == 0 ? placed[0] : placed[1]) ? mine : 0.0f;
-        }
+      const int p = key0 + lane;
+      if (whole) {
+        if (p < s.x.keys && placed) a.weights[((int64_t)s.b * a.kv_heads + s.kvh) * a.row + p] += sum;
+      } else {
+        a.part[(int64_t)slot * kPwKeys + w * 16 * T + lane] = placed ? sum : 0.0f;
       }
-      if (!whole && first == 0 && tid == 0)
+      if (!a.whole && first == 0 && threadIdx.x == 0)
         a.parts[((int64_t)s.b * a.kv_heads + s.kvh) * a.blocks + block] =
-            u32x2{(uint32_t)slot, (uint32_t)(run.owner(u - 1 - s.chunk + s.x.chunks - 1) - blockIdx.x + 1)};
-      else if (whole && a.chunks > 1 && tid == 0)
-        a.parts[((int64_t)s.b * a.kv_heads + s.kvh) * a.blocks + block] = u32x2{0, 1};
+            whole ? u32x2{0, 1}
+                  : u32x2{(uint32_t)slot,
+                          (uint32_t)(run.owner(u - 1 - s.chunk + s.x.chunks - 1) - blockIdx.x + 1)};
       fresh = false;
       first = 0;
-      if (u >= end || !s.next(a, kBlockKeys)) return;
-      load_keys(s);
-    } else if (!s.next(a, kBlockKeys)) {
-      return;
+      if (!more) return;
+      load_keys(next);
     }
+    if (other) {
+      buffer ^= 1;
+      finish(columns[buffer]);
+      block_sync();
+    }
+    s = next;
   }
 }
 
 // The partial sums of the blocks of keys that several workgroups share, added in order.
-template <int W>
-__global__ __launch_bounds__(16 * kPwTiles * W) void paged_weight_merge_kernel(PagedWeightArgs a,
-                                                                              int64_t items) {
-  constexpr int kBlockKeys = 16 * kPwTiles * W;
+__global__ __launch_bounds__(kPwKeys) void paged_weight_merge_kernel(PagedWeightArgs a, int64_t items) {
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int block = (int)(item % a.blocks);
     const int64_t bh = item / a.blocks;
     const int b = (int)(bh / a.kv_heads);
     WeightLengths x;
-    x.of(a, kBlockKeys, a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
-    if (block >= x.blocks || x.chunks <= 1) continue;
+    x.of(a, kPwKeys, a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
+    if (block >= x.blocks || x.chunks < 1) continue;
     const u32x2 held = a.parts[item];
     const int slot0 = (int)min(held[0], 2u * a.grid - 1);       // in bounds whatever it holds
     const int parts = min((int)held[1], a.grid - slot0 / 2);
-    const int p = block * kBlockKeys + threadIdx.x;
+    const int p = block * kPwKeys + threadIdx.x;
     if (parts <= 1 || p >= x.keys) continue;
     float sum = 0.0f;
     for (int y = 0; y < parts; ++y)
-      sum += a.part[(int64_t)(y == 0 ? slot0 : (slot0 & ~1) + 2 * y) * kBlockKeys + threadIdx.x];
+      sum += a.part[(int64_t)(y == 0 ? slot0 : (slot0 & ~1) + 2 * y) * kPwKeys + threadIdx.x];
     a.weights[bh * a.row + p] += sum;
   }
 }
 
 // ------------------------------------------------------------------------- host
 
-constexpr int kPwFew = 4, kPwMany = 8;   // waves of a workgroup
-
 struct WeightSizes {
-  int64_t reach, chunks, blocks, units;
-  int waves, grid;
+  int64_t chunks, blocks, reach;
+  bool few, whole;
+  int grid;
 };
 
 static bool weight_sizes(const spx_paged_cache& z, int q_heads, WeightSizes& s) {
@@ -310,32 +530,35 @@ static bool weight_sizes(const spx_paged_cache& z, int q_heads, WeightSizes& s) 
   if ((double)z.batch * z.tokens * q_heads > 0x7fffffff) return false;
   s.reach = (int64_t)z.table_width * z.page_size;
   const int64_t cols = (int64_t)z.tokens * (q_heads / z.kv_heads);
+  const bool four = z.key_scales != nullptr;
+  s.few = cols <= kPwFewCols;
   s.chunks = (cols + kPwCols - 1) / kPwCols;
-  s.waves = s.chunks > 1 ? kPwMany : kPwFew;
-  const int64_t keys = 16 * kPwTiles * s.waves;
+  s.whole = s.chunks <= kPwWhole;
+  const int64_t keys = !s.few ? kPwKeys : 16 * (four || z.head_dim == 128 ? 3 : 2);
   s.blocks = (s.reach + keys - 1) / keys;
   // units are counted in 32 bits
   if (s.blocks > 0x7fffffff / s.chunks / ((int64_t)z.batch * z.kv_heads)) return false;
-  s.units = s.blocks * s.chunks * z.batch * z.kv_heads;
-  s.grid = (int)std::min<int64_t>(s.units, kPwCus * (s.waves == kPwFew ? 4 : 2));
+  const int64_t streams = s.blocks * z.batch * z.kv_heads;
+  const int resident = kPwCus * (s.few ? (four && z.head_dim == 128 ? 4 : 2) : z.head_dim == 128 ? 3 : 2);
+  s.grid = s.few ? (int)std::min<int64_t>((streams + kPwWaves - 1) / kPwWaves, resident)
+                 : (int)std::min<int64_t>(s.whole ? streams : streams * s.chunks, resident);
   return true;
 }
 
-template <int D, bool kFour, int W>
-static int launch_weights(const PagedWeightArgs& a, hipStream_t st) {
-  paged_weight_kernel<D, kFour, W><<<(unsigned)a.grid, 64 * W, 0, st>>>(a);
-  if (a.chunks > 1) {
+template <int D, bool kFour>
+static int launch_weights(PagedWeightArgs a, const WeightSizes& z, hipStream_t st) {
+  if (z.few) {
+    a.grid *= kPwWaves;
+    a.inv_grid = 1.0 / a.grid;
+    paged_weight_few_kernel<D, kFour><<<(unsigned)z.grid, 64 * kPwWaves, 0, st>>>(a);
+    return launch_status("paged_accumulate_weights");
+  }
+  paged_weight_kernel<D, kFour><<<(unsigned)a.grid, 64 * kPwWaves, 0, st>>>(a);
+  if (!a.whole) {
     const int64_t items = (int64_t)a.batch * a.kv_heads * a.blocks;
-    paged_weight_merge_kernel<W>
-        <<<(unsigned)std::min<int64_t>(items, 1 << 20), 16 * kPwTiles * W, 0, st>>>(a, items);
+    paged_weight_merge_kernel<<<(unsigned)std::min<int64_t>(items, 1 << 20), kPwKeys, 0, st>>>(a, items);
   }
   return launch_status("paged_accumulate_weights");
-}
-
-template <int D, bool kFour>
-static int launch_weights(const PagedWeightArgs& a, int waves, hipStream_t st) {
-  return waves == kPwFew ? launch_weights<D, kFour, kPwFew>(a, st)
-                         : launch_weights<D, kFour, kPwMany>(a, st);
 }
 
 }  // namespace spx
@@ -346,8 +569,8 @@ extern "C" int64_t spx_paged_accumulate_weights_workspace_bytes(const spx_paged_
                                                                 int q_heads) {
   WeightSizes z;
   if (cache == nullptr || !weight_sizes(*cache, q_heads, z)) return -1;
-  if (z.chunks == 1) return 0;
-  return ((int64_t)2 * z.grid * 16 * kPwTiles * z.waves) * 4 +
+  if (z.whole) return 0;
+  return (int64_t)2 * z.grid * kPwKeys * 4 +
          (int64_t)cache->batch * cache->kv_heads * z.blocks * 8;
 }
 
@@ -362,7 +585,7 @@ extern "C" int spx_paged_accumulate_weights(const spx_paged_cache* cache, const 
   SPX_REQUIRE(weight_sizes(*cache, q_heads, z), SPX_EINVAL,
               "bad shape: batch %d tokens %d q_heads %d kv_heads %d", cache->batch, cache->tokens,
               q_heads, cache->kv_heads);
-  SPX_REQUIRE(q && q_strides && lse && weights && (workspace || z.chunks == 1), SPX_EINVAL,
+  SPX_REQUIRE(q && q_strides && lse && weights && (workspace || z.whole), SPX_EINVAL,
               "null pointer");
   SPX_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15) == 0 && q_strides[3] == 1 &&
                   ((q_strides[0] | q_strides[1] | q_strides[2]) & 7) == 0,
@@ -384,19 +607,20 @@ extern "C" int spx_paged_accumulate_weights(const spx_paged_cache* cache, const 
   a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.group = q_heads / cache->kv_heads;
   a.cols = cache->tokens * a.group;
   a.chunks = (int)z.chunks;
+  a.whole = z.whole;
   a.blocks = (int)z.blocks;
   a.grid = z.grid;
   a.inv_grid = 1.0 / a.grid;
   a.inv_group = 1.0 / a.group;
   const double scale_log2 = (double)scale * 1.4426950408889634;
   a.scale = (float)scale_log2;
-  a.scale_low = (float)(scale_log2 - (double)a.scale);
+  a.scale_rest = a.scale == 0.0f ? 0.0f : (float)((scale_log2 - (double)a.scale) / (double)a.scale);
   a.weights = weights;
   a.row = row_stride;
   a.part = static_cast<float*>(workspace);
-  a.parts = reinterpret_cast<u32x2*>(a.part + (int64_t)2 * a.grid * 16 * kPwTiles * z.waves);
+  a.parts = reinterpret_cast<u32x2*>(a.part + (int64_t)2 * a.grid * kPwKeys);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 128)
-    return four ? launch_weights<128, true>(a, z.waves, st) : launch_weights<128, false>(a, z.waves, st);
-  return four ? launch_weights<256, true>(a, z.waves, st) : launch_weights<256, false>(a, z.waves, st);
+    return four ? launch_weights<128, true>(a, z, st) : launch_weights<128, false>(a, z, st);
+  return four ? launch_weights<256, true>(a, z, st) : launch_weights<256, false>(a, z, st);
 }
