@@ -10,8 +10,12 @@
 //   2^(s x - L) = 2^(s' x - L') 2^e,   e = (s - s') x - (L - L') = (s / s' - 1) L' - (L - L') nearly,
 // as s' x is L' where the weight counts: the columns' factor 2^e makes up for both roundings.
 //
-// Two kernels: up to 16 columns (decode steps) a wave has Q in registers and walks the keys by itself,
-// bound by the pages' bytes; else 4 waves hold 256 keys and walk the columns through LDS, 64 at a time.
+// Two kernels. Up to 16 columns (decode steps) a wave has Q in registers and walks the keys by itself, the
+// next 64 of them under way: bound by the pages' bytes (64 sequences of up to 8192 keys in 4 bits, 32/8
+// heads: 34 us, 4.7 TB/s). Else a wave holds 64 keys in registers and walks the columns, which the
+// workgroup copies into LDS a unit ahead: bound by the issue of three vector instructions a score beside
+// the products (2000 tokens over 16000 keys, 28/4 heads: 256 us, 0.84 PFLOP/s; scores of one tile spread
+// over the products of the next by hand: 265).
 #include <algorithm>
 #include <cmath>
 
@@ -19,13 +23,21 @@
 
 namespace spx {
 
-constexpr int kPwCols = 64;              // columns of a unit
-constexpr int kPwFewCols = 16;           // at most: a wave by itself
+// Up to kPwFewCols columns the first kernel: a batch of 16 x 8000 keys in 4 bits, 32/8 heads, 4 tokens
+// 18 us (30 with the second); 4 x 8000, D = 256, bf16 14.7 (16.8).
+constexpr int kPwFewCols = 16;
+// Up to kPwWholeCols columns a block of keys has one workgroup of 4 waves and no partial sums: 64 tokens
+// over 32640 keys, 28/4 heads 28 us (32 + 5 shared by workgroups of 8 waves), 8 x 16 over 4000, 32/8 heads
+// 16 (23 + 5). Beyond, runs of columns are shared: 301 tokens over 8000, 32/8 heads 36 + 5 us (53 by
+// whole blocks).
+constexpr int kPwWholeCols = 512;
 constexpr int kPwCus = 256;
-constexpr int kPwWaves = 4;              // of a workgroup
 constexpr int kPwTiles = 4;              // of 16 keys, a wave's
-constexpr int kPwKeys = 16 * kPwTiles * kPwWaves;
-constexpr int kPwWhole = 8;              // chunks up to which a block of keys has one workgroup
+
+// W waves of a workgroup: each has 64 keys and brings in 16 columns of a unit.
+constexpr int kPwWaves = 4, kPwManyWaves = 8;
+__host__ __device__ constexpr int weight_keys(int waves) { return 16 * kPwTiles * waves; }
+__host__ __device__ constexpr int weight_cols(int waves) { return 16 * waves; }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -51,23 +63,24 @@ struct PagedWeightArgs {
   float scale, scale_rest;               // scale log2(e), rounded; what of it is missing, relative
   float* weights;                        // [B, Hkv, row]
   int64_t row;
-  float* part;                           // [2 grid][kPwKeys]
+  float* part;                           // [2 grid][keys of a block]
   u32x2* parts;                          // [B, Hkv, blocks]
 };
 
 struct WeightLengths {
   int start, live, keys, blocks, chunks;
-  __device__ __forceinline__ void of(const PagedWeightArgs& a, int block, int start_, int count) {
+  __device__ __forceinline__ void of(const PagedWeightArgs& a, int block, int cols, int start_,
+                                     int count) {
     start = start_;
     const int64_t room = a.map.capacity() - start;
     live = start < 0 ? 0
                      : max(0, min(min(count, a.tokens), (int)min(room, (int64_t)a.tokens)));
     keys = live > 0 ? start + live : 0;
     blocks = (keys + block - 1) / block;
-    chunks = (live * a.group + kPwCols - 1) / kPwCols;
+    chunks = (live * a.group + cols - 1) / cols;
   }
-  __device__ __forceinline__ void load(const PagedWeightArgs& a, int block, int b) {
-    of(a, block, scalar_load(a.map.starts + b),
+  __device__ __forceinline__ void load(const PagedWeightArgs& a, int block, int cols, int b) {
+    of(a, block, cols, scalar_load(a.map.starts + b),
        a.map.counts ? scalar_load(a.map.counts + b) : a.tokens);
   }
 };
@@ -75,14 +88,14 @@ struct WeightLengths {
 // What is dealt to the workgroups: chunks of columns of the blocks of keys, or whole blocks.
 struct WeightScan {                      // of 64 sequences, one a lane
   int units, sum;
-  __device__ __forceinline__ void load(const PagedWeightArgs& a, int block, int b) {
+  __device__ __forceinline__ void load(const PagedWeightArgs& a, int block, int cols, int b) {
     WeightLengths x;
     int start = -1, count = a.tokens;
     if (b < a.batch) {
       start = a.map.starts[b];
       if (a.map.counts) count = a.map.counts[b];
     }
-    x.of(a, block, start, count);
+    x.of(a, block, cols, start, count);
     units = x.chunks == 0 ? 0 : x.blocks * (a.whole ? 1 : x.chunks) * a.kv_heads;
     sum = wave_prefix(units);
   }
@@ -93,20 +106,20 @@ struct WeightUnit {
   WeightLengths x;
   int b, kvh, at, chunk;                 // at: which of the blocks, in the order of the runs
 
-  __device__ __forceinline__ bool find(const PagedWeightArgs& a, int block, int lane, WeightScan scan,
-                                       int u) {
+  __device__ __forceinline__ bool find(const PagedWeightArgs& a, int block, int cols, int lane,
+                                       WeightScan scan, int u) {
     int before = 0, b0 = 0;
     uint64_t past;
     while (!(past = __ballot(before + scan.sum > u))) {
       before += scan.total();
       b0 += kWave;
       if (b0 >= a.batch) return false;
-      scan.load(a, block, b0 + lane);
+      scan.load(a, block, cols, b0 + lane);
     }
     const int l = __builtin_ctzll(past);
     b = b0 + l;
     before += __builtin_amdgcn_readlane(scan.sum - scan.units, l);
-    x.load(a, block, b);
+    x.load(a, block, cols, b);
     if (x.blocks <= 0 || x.chunks <= 0 || u < before) return false;
     const int each = a.whole ? 1 : x.chunks;
     const int stream = (u - before) / each;
@@ -115,7 +128,7 @@ struct WeightUnit {
     at = stream - kvh * x.blocks;
     return kvh < a.kv_heads;
   }
-  __device__ __forceinline__ bool next(const PagedWeightArgs& a, int block) {
+  __device__ __forceinline__ bool next(const PagedWeightArgs& a, int block, int cols) {
     if (++chunk < x.chunks) return true;
     chunk = 0;
     if (++at < x.blocks) return true;
@@ -124,7 +137,7 @@ struct WeightUnit {
     kvh = 0;
     do {
       if (++b >= a.batch) return false;
-      x.load(a, block, b);
+      x.load(a, block, cols, b);
     } while (x.blocks == 0 || x.chunks == 0);
     return true;
   }
@@ -191,11 +204,11 @@ paged_weight_few_kernel(PagedWeightArgs a) {
   const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   WeightScan scan;
-  scan.load(a, kKeys, lane);
+  scan.load(a, kKeys, kPwFewCols, lane);
   int total = scan.total();
   for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
     WeightScan more;
-    more.load(a, kKeys, b0 + lane);
+    more.load(a, kKeys, kPwFewCols, b0 + lane);
     total += more.total();
   }
   const WeightRun run(total, a.grid, a.inv_grid);
@@ -203,7 +216,7 @@ paged_weight_few_kernel(PagedWeightArgs a) {
   int u = run.begin(wave);
   const int end = run.begin(wave + 1);
   WeightUnit s, next;                    // unit u and u + 1
-  if (u >= end || !s.find(a, kKeys, lane, scan, u)) return;
+  if (u >= end || !s.find(a, kKeys, kPwFewCols, lane, scan, u)) return;
   // lane t: page of tile t % T
   const auto fetch_ids = [&](const WeightUnit& s) {
     const int64_t p = (int64_t)s.at * kKeys + lane % T * 16;
@@ -259,14 +272,14 @@ paged_weight_few_kernel(PagedWeightArgs a) {
         last[r] = x.last;
       }
     }
-    const bool more = ++u < end && next.next(a, kKeys);
+    const bool more = ++u < end && next.next(a, kKeys, kPwFewCols);
     if (more) {
       load(coming, next, ids);
       s = next;
     }
     if (more && u + 1 < end) {
       WeightUnit after = next;
-      if (after.next(a, kKeys)) ids = fetch_ids(after);
+      if (after.next(a, kKeys, kPwFewCols)) ids = fetch_ids(after);
     }
     const int key0 = at.at * kKeys + c;
     float acc[T];
@@ -291,7 +304,7 @@ paged_weight_few_kernel(PagedWeightArgs a) {
   next = s;
   if (u + 1 < end) {
     WeightUnit after = next;
-    if (after.next(a, kKeys)) ids = fetch_ids(after);
+    if (after.next(a, kKeys, kPwFewCols)) ids = fetch_ids(after);
   }
   while (step(one, two) && step(two, one)) {}
 }
@@ -325,44 +338,46 @@ __device__ __forceinline__ void copy_rows_to_lds(const uint64_t (&from)[4], LdsB
 }
 
 // A unit's columns in LDS: rows of Q, 16-byte chunks exchanged within a row by an XOR with row % 16.
-template <int D>
+template <int D, int W>
 struct WeightColumns {
   static constexpr int kLanes = D / 8, kRows = kWave / kLanes, kCopies = 16 / kRows;
-  uint16_t q[kPwCols * D];
-  float hi[kPwCols], factor[kPwCols];
-  int last[kPwCols];
-  int least[4], most[4];                 // of last in 16 columns: every one sees it, one does
+  static constexpr int kCols = weight_cols(W);
+  uint16_t q[kCols * D];
+  float hi[kCols], factor[kCols];
+  int last[kCols];
+  int least[W], most[W];                 // of 16 columns: keys up to it are seen by all, behind it by none
 };
 
-template <int D, bool kFour>
-__global__ __launch_bounds__(64 * kPwWaves, D == 128 ? 3 : 2) void
+template <int D, bool kFour, int W>
+__global__ __launch_bounds__(64 * W, D == 128 ? (W == kPwWaves ? 3 : 4) : 2) void
 paged_weight_kernel(PagedWeightArgs a) {
-  constexpr int T = kPwTiles, KK = D / 32;
-  using Columns = WeightColumns<D>;
+  constexpr int T = kPwTiles, KK = D / 32, kKeys = weight_keys(W), kCols = weight_cols(W);
+  using Columns = WeightColumns<D, W>;
   __shared__ __align__(16) Columns columns[2];
   const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   WeightScan scan;
-  scan.load(a, kPwKeys, lane);
+  scan.load(a, kKeys, kCols, lane);
   int total = scan.total();
   for (int b0 = kWave; b0 < a.batch; b0 += kWave) {
     WeightScan more;
-    more.load(a, kPwKeys, b0 + lane);
+    more.load(a, kKeys, kCols, b0 + lane);
     total += more.total();
   }
   const WeightRun run(total, a.grid, a.inv_grid);
   const int begin = run.begin(blockIdx.x), end = run.begin(blockIdx.x + 1);
   WeightUnit s;
-  if (begin >= end || !s.find(a, kPwKeys, lane, scan, begin)) return;
+  if (begin >= end || !s.find(a, kKeys, kCols, lane, scan, begin)) return;
   // A wave brings 16 columns in; finish() after the copies are there.
   float lse = 0.0f;
-  int last_key = 0;
+  int last_key = 0, latest = 0;
   const auto stage = [&](const WeightUnit& s, Columns& to) {
-    const int n = s.chunk * kPwCols + 16 * w + c, m = min(n, s.x.live * a.group - 1);
+    const int n = s.chunk * kCols + 16 * w + c, m = min(n, s.x.live * a.group - 1);
     const int token = divide(m, a.group, a.inv_group), head = s.kvh * a.group + m - token * a.group;
     const uint64_t row = (uint64_t)(a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h);
     lse = a.lse[((int64_t)s.b * a.tokens + token) * a.q_heads + head];
     last_key = n == m ? s.x.start + token : -1;
+    latest = s.x.start + __builtin_amdgcn_readlane(token, 15);
     const LdsBytes place = (LdsBytes)to.q + 16 * w * 2 * D;
 #pragma unroll
     for (int i = 0; i < Columns::kCopies; i += 4) {
@@ -379,20 +394,15 @@ paged_weight_kernel(PagedWeightArgs a) {
   };
   const auto finish = [&](Columns& to) {
     const WeightColumn x(a, lse, last_key);
-    int least = x.last, most = x.last;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-      least = min(least, __shfl_xor(least, d));
-      most = max(most, __shfl_xor(most, d));
-    }
+    const bool dead = __any(x.last < 0);
     if (lane < 16) {
       to.hi[16 * w + lane] = x.hi;
       to.factor[16 * w + lane] = x.factor;
       to.last[16 * w + lane] = x.last;
     }
     if (lane == 0) {
-      to.least[w] = least;
-      to.most[w] = most;
+      to.least[w] = dead ? -1 : last_key;
+      to.most[w] = latest;
     }
     wait_copies<0>();
   };
@@ -400,7 +410,7 @@ paged_weight_kernel(PagedWeightArgs a) {
   bool placed = false;                   // the lane's key of tile g
   const auto load_keys = [&](const WeightUnit& s) {
     const HeadPages<D, kFour> pages(a, s.kvh);
-    const int key0 = s.block() * kPwKeys + w * 16 * T;
+    const int key0 = s.block() * kKeys + w * 16 * T;
     const int64_t p = (int64_t)key0 + lane % T * 16;
     const int ids = a.map.page(s.b, (int)min(p, (int64_t)s.x.keys - 1));
     KeyTile<D, kFour> tile[T];
@@ -450,17 +460,19 @@ paged_weight_kernel(PagedWeightArgs a) {
     const bool last = s.chunk == s.x.chunks - 1;
     if (last || !a.whole) ++u;
     WeightUnit next = s;
-    const bool more = u < end && next.next(a, kPwKeys);
+    const bool more = u < end && next.next(a, kKeys, kCols);
     const bool other = more && (next.chunk != s.chunk || next.kvh != s.kvh || next.b != s.b);
     if (other) stage(next, columns[buffer ^ 1]);
-    const int block = s.block(), key0 = block * kPwKeys + w * 16 * T;
+    const int block = s.block(), key0 = block * kKeys + w * 16 * T;
     const Columns& q = columns[buffer];
-    const i32x4 least = *reinterpret_cast<const i32x4*>(q.least);
-    if (first_lane(min(min(least[0], least[1]), min(least[2], least[3]))) >= key0 + 16 * T - 1) {
+    int least = q.least[0];
 #pragma unroll
-      for (int ct = 0; ct < kPwCols / 16; ++ct) compute(q, key0, ct, false);
+    for (int i = 1; i < W; ++i) least = min(least, q.least[i]);
+    if (first_lane(least) >= key0 + 16 * T - 1) {
+#pragma unroll
+      for (int ct = 0; ct < kCols / 16; ++ct) compute(q, key0, ct, false);
     } else {
-      for (int ct = 0; ct < kPwCols / 16; ++ct)
+      for (int ct = 0; ct < kCols / 16; ++ct)
         if (first_lane(q.most[ct]) >= key0) compute(q, key0, ct, true);
     }
     if (last || !more) {
@@ -473,7 +485,7 @@ paged_weight_kernel(PagedWeightArgs a) {
       if (whole) {
         if (p < s.x.keys && placed) a.weights[((int64_t)s.b * a.kv_heads + s.kvh) * a.row + p] += sum;
       } else {
-        a.part[(int64_t)slot * kPwKeys + w * 16 * T + lane] = placed ? sum : 0.0f;
+        a.part[(int64_t)slot * kKeys + w * 16 * T + lane] = placed ? sum : 0.0f;
       }
       if (!a.whole && first == 0 && threadIdx.x == 0)
         a.parts[((int64_t)s.b * a.kv_heads + s.kvh) * a.blocks + block] =
@@ -495,22 +507,24 @@ paged_weight_kernel(PagedWeightArgs a) {
 }
 
 // The partial sums of the blocks of keys that several workgroups share, added in order.
-__global__ __launch_bounds__(kPwKeys) void paged_weight_merge_kernel(PagedWeightArgs a, int64_t items) {
+__global__ __launch_bounds__(weight_keys(kPwManyWaves)) void paged_weight_merge_kernel(PagedWeightArgs a,
+                                                                                     int64_t items) {
+  constexpr int kKeys = weight_keys(kPwManyWaves);
   for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int block = (int)(item % a.blocks);
     const int64_t bh = item / a.blocks;
     const int b = (int)(bh / a.kv_heads);
     WeightLengths x;
-    x.of(a, kPwKeys, a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
+    x.of(a, kKeys, weight_cols(kPwManyWaves), a.map.starts[b], a.map.counts ? a.map.counts[b] : a.tokens);
     if (block >= x.blocks || x.chunks < 1) continue;
     const u32x2 held = a.parts[item];
     const int slot0 = (int)min(held[0], 2u * a.grid - 1);       // in bounds whatever it holds
     const int parts = min((int)held[1], a.grid - slot0 / 2);
-    const int p = block * kPwKeys + threadIdx.x;
+    const int p = block * kKeys + threadIdx.x;
     if (parts <= 1 || p >= x.keys) continue;
     float sum = 0.0f;
     for (int y = 0; y < parts; ++y)
-      sum += a.part[(int64_t)(y == 0 ? slot0 : (slot0 & ~1) + 2 * y) * kPwKeys + threadIdx.x];
+      sum += a.part[(int64_t)(y == 0 ? slot0 : (slot0 & ~1) + 2 * y) * kKeys + threadIdx.x];
     a.weights[bh * a.row + p] += sum;
   }
 }
@@ -532,14 +546,17 @@ static bool weight_sizes(const spx_paged_cache& z, int q_heads, WeightSizes& s) 
   const int64_t cols = (int64_t)z.tokens * (q_heads / z.kv_heads);
   const bool four = z.key_scales != nullptr;
   s.few = cols <= kPwFewCols;
-  s.chunks = (cols + kPwCols - 1) / kPwCols;
-  s.whole = s.chunks <= kPwWhole;
-  const int64_t keys = !s.few ? kPwKeys : 16 * (four || z.head_dim == 128 ? 3 : 2);
+  s.whole = cols <= kPwWholeCols;
+  const int waves = s.whole ? kPwWaves : kPwManyWaves;
+  s.chunks = s.few ? 1 : (cols + weight_cols(waves) - 1) / weight_cols(waves);
+  const int64_t keys = !s.few ? weight_keys(waves) : 16 * (four || z.head_dim == 128 ? 4 : 2);
   s.blocks = (s.reach + keys - 1) / keys;
   // units are counted in 32 bits
   if (s.blocks > 0x7fffffff / s.chunks / ((int64_t)z.batch * z.kv_heads)) return false;
   const int64_t streams = s.blocks * z.batch * z.kv_heads;
-  const int resident = kPwCus * (s.few ? (four && z.head_dim == 128 ? 4 : 2) : z.head_dim == 128 ? 3 : 2);
+  const bool small = z.head_dim == 128;
+  const int resident =
+      kPwCus * (s.few ? (four && small ? 4 : 2) : s.whole ? (small ? 3 : 2) : small ? 2 : 1);
   s.grid = s.few ? (int)std::min<int64_t>((streams + kPwWaves - 1) / kPwWaves, resident)
                  : (int)std::min<int64_t>(s.whole ? streams : streams * s.chunks, resident);
   return true;
@@ -553,10 +570,13 @@ static int launch_weights(PagedWeightArgs a, const WeightSizes& z, hipStream_t s
     paged_weight_few_kernel<D, kFour><<<(unsigned)z.grid, 64 * kPwWaves, 0, st>>>(a);
     return launch_status("paged_accumulate_weights");
   }
-  paged_weight_kernel<D, kFour><<<(unsigned)a.grid, 64 * kPwWaves, 0, st>>>(a);
-  if (!a.whole) {
+  if (a.whole) {
+    paged_weight_kernel<D, kFour, kPwWaves><<<(unsigned)a.grid, 64 * kPwWaves, 0, st>>>(a);
+  } else {
+    paged_weight_kernel<D, kFour, kPwManyWaves><<<(unsigned)a.grid, 64 * kPwManyWaves, 0, st>>>(a);
     const int64_t items = (int64_t)a.batch * a.kv_heads * a.blocks;
-    paged_weight_merge_kernel<<<(unsigned)std::min<int64_t>(items, 1 << 20), kPwKeys, 0, st>>>(a, items);
+    paged_weight_merge_kernel<<<(unsigned)std::min<int64_t>(items, 1 << 20), weight_keys(kPwManyWaves),
+                                0, st>>>(a, items);
   }
   return launch_status("paged_accumulate_weights");
 }
@@ -570,7 +590,7 @@ extern "C" int64_t spx_paged_accumulate_weights_workspace_bytes(const spx_paged_
   WeightSizes z;
   if (cache == nullptr || !weight_sizes(*cache, q_heads, z)) return -1;
   if (z.whole) return 0;
-  return (int64_t)2 * z.grid * kPwKeys * 4 +
+  return (int64_t)2 * z.grid * weight_keys(kPwManyWaves) * 4 +
          (int64_t)cache->batch * cache->kv_heads * z.blocks * 8;
 }
 
@@ -618,7 +638,7 @@ extern "C" int spx_paged_accumulate_weights(const spx_paged_cache* cache, const 
   a.weights = weights;
   a.row = row_stride;
   a.part = static_cast<float*>(workspace);
-  a.parts = reinterpret_cast<u32x2*>(a.part + (int64_t)2 * a.grid * kPwKeys);
+  a.parts = reinterpret_cast<u32x2*>(a.part + (int64_t)2 * a.grid * weight_keys(kPwManyWaves));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (cache->head_dim == 128)
     return four ? launch_weights<128, true>(a, z, st) : launch_weights<128, false>(a, z, st);
