@@ -257,6 +257,10 @@ extern "C" int spx_paged_keep_path(const spx_paged_cache* caches, int cache_coun
                     z.tokens == first.tokens &&
                     (z.key_scales == nullptr) == (first.key_scales == nullptr),
                 SPX_EINVAL, "cache %d differs in more than its pages from the first", i);
+    // rows would move twice, the second time from places that the first has filled
+    for (int j = 0; j < i; ++j)
+      SPX_REQUIRE(z.key_pages != caches[j].key_pages && z.value_pages != caches[j].value_pages,
+                  SPX_EINVAL, "caches %d and %d are the same pages", j, i);
   }
   SPX_REQUIRE(first.tokens <= kPathTokens, SPX_EINVAL, "%d tokens are more than %d", first.tokens,
               kPathTokens);

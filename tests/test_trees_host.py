@@ -149,3 +149,8 @@ def test_wrappers_refuse():
 def test_description_size():
     """Several descriptions lie side by side as the C entry reads them."""
     assert len(_cache()) == 96 and ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_keep_path_of_the_same_pages_twice():
+    assert _keep(caches=_cache() + _cache(), count=2) == INVALID
+    assert b"same pages" in _lib.load().spx_last_error()
