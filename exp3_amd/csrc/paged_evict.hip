@@ -10,6 +10,11 @@
 // writes the list of moves, in the order of the slots, and clears the ledger of the tokens behind the
 // budget that it drops. The kept ones move in a launch of their own, row and ledger, so that both
 // may be in place.
+//
+// Bound by the walks' instructions: a row is one workgroup's, so few long rows leave most CUs idle (1
+// x 4 heads of 32640 tokens to 4096: 30.6 us, 16 waves, + 5.6 for the moves; 64 x 8 heads of 2112 to
+// 2048: 16.7 + 8.3, the bytes of both 8). A row shared by workgroups would need a launch per digit,
+// some 3 us each, for what a prompt does once.
 #include <algorithm>
 
 #include "paged_moves.h"
@@ -116,7 +121,7 @@ __global__ __launch_bounds__(64 * W) void paged_evict_kernel(EvictArgs a) {
   block_sync();
   // Ranks into LDS and their first digits counted; slots below the budget keep what they have for
   // now. Loads first, kAtOnce at a time: the stores between them may be to the same tensors.
-  constexpr int kAtOnce = 8;
+  constexpr int kAtOnce = W == 16 ? 16 : 8;
   for (int i0 = tid; i0 < W * part; i0 += kAtOnce * kThreads) {
     float x[kAtOnce];
     int told[kAtOnce];
@@ -291,6 +296,8 @@ __global__ __launch_bounds__(64 * W) void paged_evict_kernel(EvictArgs a) {
   }
   if (tid == 0) a.counts[bh] = moves;
   u32x2* list = a.moves + bh * a.room;
+  const bool wide =
+      ((reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(positions_out)) & 15) == 0;
   for (int i0 = begin; i0 < end; i0 += kChunk) {
     const int i = i0 + 4 * lane;
     uint32_t r[4];
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(64 * W) void paged_evict_kernel(EvictArgs a) {
       before = equals + up_to - mine;
       equals += __builtin_amdgcn_readlane(up_to, kWave - 1);
     }
-    bool hole[4], far[4];
+    bool hole[4], far[4], gone[4];
     int both = 0;                        // holes, and kept ones behind the budget << 16
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -313,10 +320,18 @@ __global__ __launch_bounds__(64 * W) void paged_evict_kernel(EvictArgs a) {
       hole[e] = !kept && low;
       far[e] = kept && !low;
       both += (int)hole[e] + ((int)far[e] << 16);
-      if (!kept && !low && i + e < length) {         // dropped; what is kept there, moves
-        weights_out[i + e] = 0.0f;
-        positions_out[i + e] = -1;
-      }
+      gone[e] = !kept && !low && i + e < length;     // dropped; what is kept there, moves
+    }
+    if (wide && gone[0] && gone[1] && gone[2] && gone[3]) {
+      *reinterpret_cast<u32x4*>(weights_out + i) = u32x4{};
+      *reinterpret_cast<u32x4*>(positions_out + i) = ~u32x4{};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (gone[e]) {
+          weights_out[i + e] = 0.0f;
+          positions_out[i + e] = -1;
+        }
     }
     if (!__any(both != 0)) continue;
     const int up_to = wave_prefix(both);

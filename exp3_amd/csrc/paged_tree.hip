@@ -7,7 +7,19 @@
 //
 // Columns n = i group + h of a KV head (token i of T, query head h of the group) share its K and V;
 // 64 or 128 of them are one tile. A stream is a (sequence, KV head, column tile), its work
-// ceil(keys / 64) units of 64 keys.
+// ceil(keys / 64) units of 64 keys, and the units of all streams are dealt in equal runs to one grid
+// (lengths are device data); a second kernel joins the partial results of the streams that
+// workgroups share.
+//
+// Between HBM and the matrix units: at 128 columns a unit's products take half as long as its bytes in
+// bf16, twice as long in 4 bits. So K and V are read once for 128 columns and are on their way a unit
+// and a half ahead, and a wave's softmax, or its widening of 4 bits, is issued between products. P goes
+// to the products in two bf16 parts, 2^-18 of it is lost; one part would save a third of the matrix
+// instructions and lose 2^-9, nearly as much as the output's own rounding.
+//
+// 8 ragged sequences of up to 16000 keys, trees of 32, 32/8 heads, bf16: 81 us (3.9 TB/s) + 11 to join;
+// 16 of up to 8192 in 4 bits, trees of 61, 28/4 heads: 99 (0.48 PFLOP/s, 0.72 with both parts of P) + 11;
+// 4 of up to 12001 in 4 bits at D = 256, trees of 26, 16/4 heads: 41 + 8, one wave per SIMD (LDS).
 #include <algorithm>
 #include <cmath>
 
@@ -626,8 +638,7 @@ __device__ __forceinline__ void tree_run(TreeState<D>& st, const TreeArgs& a, co
   } else if constexpr (!kFour) {
     // K of unit j + 2 comes in from the middle of unit j on, where K of unit j has been read, V of unit
     // j + 1 from the beginning of unit j on: each for one and a half units, 48 KB a workgroup at D =
-    // 128. (Both from the beginning of the unit before on: 8 ragged sequences of up to 16000 tokens,
-    // trees of 32, 32/8 heads, 83 us.)
+    // 128.
     constexpr int kCopies = TreeRows<D, false>::kCopies;
     const TreeRows<D, false> rows(lane);
     int64_t next_row = row_of(j);        // of the unit whose K went last

@@ -1,5 +1,6 @@
 """Paged KV cache on MI355X: append with the rotary embedding applied on the way, reading
-back, and attention of new tokens over the pages, in bf16 or in 4 bits.
+back, attention of new tokens over the pages, in bf16 or in 4 bits, drafted trees, and eviction of
+the tokens that gathered least attention.
 
 The serving side of the prefill backend: a prompt's projections go through
 ``append_tokens`` (which stores K and V and returns the rotated Q and K that
@@ -27,6 +28,11 @@ either mode: tensors that require a gradient are refused while gradients are rec
 those that carry a forward-mode tangent. The calls are refused while torch traces a graph
 (``torch.jit.trace``, ``make_fx``, ``torch.export``); ``torch.compile`` breaks its graph at
 them. q, k and v do not overlap the cache's memory, nor do its tensors each other's.
+
+A step of a drafted tree is ``draft_tree`` once, per layer ``append_tokens`` (with ``positions =
+starts[:, None] + depths``) and ``tree_attention``, and ``accept_drafts`` once for all layers. A cache
+held at a budget takes ``accumulate_weights`` behind the attention calls (with ``return_lse``) and now and
+then ``evict_tokens``.
 """
 
 from __future__ import annotations
