@@ -94,6 +94,36 @@ def test_weights_special_rows(gpu):
     assert nan == [[0, 1, 5]]
 
 
+@pytest.mark.parametrize("tokens", (30, 160))
+def test_weights_special_rows_of_many_tokens(gpu, tokens):
+    """The same where the columns are many; a row of NaN whose LSE is -inf."""
+    s = ref.make(68, 2, tokens, 8, 2, 128, 16, 50, (560, 20), counts=(tokens, tokens // 2))
+    lse = torch.full((2, tokens, 8), 1.0)
+    lse[0, 1], lse[0, 17, 3], lse[1, tokens // 2:] = -math.inf, -math.inf, math.nan
+    s.q[0, 1] = s.q[1, tokens // 2:] = math.nan
+    behind = 560 + tokens
+    for x in s.held:
+        x[int(s.table[0, behind // 16]), :, behind % 16:] = math.nan
+    _check_weights(s, 0.1, lse=lse.cuda())
+    s.held[0][int(s.table[0, 33]), 1, 5] = math.nan
+    cache, table, starts, counts = ref.on_gpu(s)
+    weights = torch.zeros(2, 2, 800, device="cuda")
+    paged.accumulate_weights(weights, s.q.cuda(), lse.cuda(), cache, table, starts, 0.1, counts)
+    assert torch.isnan(weights).nonzero().tolist() == [[0, 1, 533]]
+
+
+@pytest.mark.parametrize("bits", (16, 4))
+@pytest.mark.parametrize("tokens,layout", ((100, (16, 4, 256)), (140, (16, 4, 256)), (140, (28, 4, 128)),
+                                           (70, (28, 4, 128)), (3, (16, 4, 256)), (2, (28, 4, 128))))
+def test_weights_of_several_blocks(gpu, tokens, layout, bits):
+    """Blocks of keys that one workgroup has and that workgroups share; ragged, with padding."""
+    s = ref.make(69, 5, tokens, *layout, 64, 30, (1500, 511 - tokens, -1, 900, 0),
+                 counts=(tokens, tokens, tokens, tokens - 1, tokens), bits=bits)
+    first, before = _check_weights(s, 0.08, more=2)
+    again, _ = _check_weights(s, 0.08, more=2)
+    assert torch.equal(first, again)
+
+
 def test_weights_strided_queries_and_sums(gpu):
     """Queries read in place; a row's weights sum to its number of query heads and tokens."""
     s = ref.make(67, 2, 5, 12, 2, 128, 16, 20, (300, 100))

@@ -269,6 +269,35 @@ def test_evictions_on_two_streams(gpu):
         assert torch.equal(a.key_pages, b.key_pages) and torch.equal(a.value_pages, b.value_pages)
 
 
+@pytest.mark.parametrize("bits", (16, 4))
+def test_pages_past_32_bits(gpu, bits):
+    """The same step in the first pages of a cache and behind 2^32 elements of a larger one."""
+    s = ref.make(81, 2, 20, 28, 4, 128, 16, 24, (340, 90), bits=bits)
+    near, table, starts, _ = ref.on_gpu(s)
+    far = 2 ** 32 // (16 * 4 * 128) + 100
+    large = paged.empty_pages(far + s.pages, 16, 4, 128, "cuda", four_bit=bits == 4)
+    for x, y in zip(vars(large).values(), vars(near).values()):
+        if y is not None:
+            x[far:] = y
+    q, parents = s.q.cuda(), trees.random_parents(81, 2, 20).cuda()
+    _, masks = paged.draft_tree(parents)
+    drafts = torch.zeros(2, 20, dtype=torch.int64, device="cuda")
+    got = []
+    for cache, at in ((near, table), (large, table + far)):
+        weights = torch.zeros(2, 4, 384, device="cuda")
+        out, lse = paged.tree_attention(q, cache, at, starts, masks, 0.1, return_lse=True)
+        paged.accumulate_weights(weights, q, lse, cache, at, starts, 0.1)
+        paged.accumulate_weights(weights, q[:, :1], lse[:, :1], cache, at, starts, 0.1)
+        accepted, path, _ = paged.accept_drafts(cache, at, starts, parents, drafts, drafts)
+        got.append([out, lse, weights, accepted, path,
+                    *paged.evict_tokens(cache, at, starts + accepted, weights, 80, recent=5)])
+    assert accepted.min() > 1
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+    for x, y in zip(vars(large).values(), vars(near).values()):
+        assert y is None or torch.equal(x[far:], y)
+
+
 def _captured(seed):
     """A captured step on inputs of its own -> (graph, its outputs, the eager ones, what it reads)."""
     s = ref.make(seed, 2, 20, 28, 4, 128, 32, 40, (1100, 300))
