@@ -121,7 +121,7 @@ __global__ __launch_bounds__(64 * W) void paged_evict_kernel(EvictArgs a) {
   block_sync();
   // Ranks into LDS and their first digits counted; slots below the budget keep what they have for
   // now. Loads first, kAtOnce at a time: the stores between them may be to the same tensors.
-  constexpr int kAtOnce = W == 16 ? 16 : 8;
+  constexpr int kAtOnce = 16;
   for (int i0 = tid; i0 < W * part; i0 += kAtOnce * kThreads) {
     float x[kAtOnce];
     int told[kAtOnce];

@@ -430,7 +430,7 @@ int spx_paged_tree_attention(const spx_paged_cache* cache, const void* q, const 
 
 /* Acceptance of drafted tokens: rows of K and V of an accepted path moved into place, from
  * starts[b] + path[b][j] to starts[b] + j, in all caches (the layers of a model: descriptions that
- * differ in their pages alone; read by the host before the call returns).
+ * differ in their pages alone, no two with the same ones; read by the host before the call returns).
  * Either with parents, drafts and targets, contiguous [B, T] (int32, int64, int64): node 0 is taken,
  * then the first child whose drafts equals the targets of the node taken last, while there is one.
  * accepted: int32 [B], how many were taken (0 without live tokens); path_out: int32 [B, T], their
