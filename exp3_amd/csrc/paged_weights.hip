@@ -11,7 +11,7 @@
 // as s' x is L' where the weight counts: the columns' factor 2^e makes up for both roundings.
 //
 // Two kernels. Up to 16 columns (decode steps) a wave has Q in registers and walks the keys by itself, the
-// next 64 of them under way: bound by the pages' bytes (64 sequences of up to 8192 keys in 4 bits, 32/8
+// next 32 or 64 under way: bound by the pages' bytes (64 sequences of up to 8192 keys in 4 bits, 32/8
 // heads: 34 us, 4.7 TB/s). Else a wave holds 64 keys in registers and walks the columns, which the
 // workgroup copies into LDS a unit ahead: bound by the issue of three vector instructions a score beside
 // the products (2000 tokens over 16000 keys, 28/4 heads: 256 us, 0.84 PFLOP/s; scores of one tile spread
@@ -41,9 +41,12 @@ __host__ __device__ constexpr int weight_cols(int waves) { return 16 * waves; }
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Tiles of 16 keys that a wave has under way for few columns: as many as two sets of registers hold.
-template <int D, bool kFour>
-constexpr int kPwFewTiles = kFour || D == 128 ? 4 : 2;
+// Tiles of 16 keys that a wave has under way for few columns, and waves per SIMD. (bf16, D = 128 with 4
+// and 2 in place of 2 and 4: 100000 keys, 32/8 heads 44.4 us, not 42.8; 2000 keys 5.4, not 4.4.)
+template <bool kFour>
+constexpr int kPwFewTiles = kFour ? 4 : 2;
+template <int D>
+constexpr int kPwFewPerSimd = D == 128 ? 4 : 2;
 
 struct PagedWeightArgs {
   PagedMap map;
@@ -198,9 +201,9 @@ __device__ __forceinline__ float weight_sums(const float (&x)[2]) {
 // ------------------------------------------------------------------ few columns
 
 template <int D, bool kFour>
-__global__ __launch_bounds__(64 * kPwWaves, kFour && D == 128 ? 4 : 2) void
+__global__ __launch_bounds__(64 * kPwWaves, kPwFewPerSimd<D>) void
 paged_weight_few_kernel(PagedWeightArgs a) {
-  constexpr int T = kPwFewTiles<D, kFour>, kKeys = 16 * T, KK = D / 32;
+  constexpr int T = kPwFewTiles<kFour>, kKeys = 16 * T, KK = D / 32;
   const int lane = threadIdx.x & 63, w = first_lane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   WeightScan scan;
@@ -549,14 +552,17 @@ static bool weight_sizes(const spx_paged_cache& z, int q_heads, WeightSizes& s) 
   s.whole = cols <= kPwWholeCols;
   const int waves = s.whole ? kPwWaves : kPwManyWaves;
   s.chunks = s.few ? 1 : (cols + weight_cols(waves) - 1) / weight_cols(waves);
-  const int64_t keys = !s.few ? weight_keys(waves) : 16 * (four || z.head_dim == 128 ? 4 : 2);
+  const int64_t keys =
+      !s.few ? weight_keys(waves) : 16 * (four ? kPwFewTiles<true> : kPwFewTiles<false>);
   s.blocks = (s.reach + keys - 1) / keys;
   // units are counted in 32 bits
   if (s.blocks > 0x7fffffff / s.chunks / ((int64_t)z.batch * z.kv_heads)) return false;
   const int64_t streams = s.blocks * z.batch * z.kv_heads;
   const bool small = z.head_dim == 128;
-  const int resident =
-      kPwCus * (s.few ? (four && small ? 4 : 2) : s.whole ? (small ? 3 : 2) : small ? 2 : 1);
+  const int per_cu = s.few     ? (small ? kPwFewPerSimd<128> : kPwFewPerSimd<256>)
+                     : s.whole ? (small ? 3 : 2)
+                               : (small ? 2 : 1);
+  const int resident = kPwCus * per_cu;
   s.grid = s.few ? (int)std::min<int64_t>((streams + kPwWaves - 1) / kPwWaves, resident)
                  : (int)std::min<int64_t>(s.whole ? streams : streams * s.chunks, resident);
   return true;
