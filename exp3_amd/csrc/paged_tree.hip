@@ -756,11 +756,15 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
     const bool idle = s.tile * kColumns + 32 * wc >= a.cols;
     u32x4 q[D / 16];
     const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h + 8 * half;
+    // Queries of padding may hold anything: they count as 0, and what K and V make of them (columns
+    // that are not written) does not count as odd below.
+    const bool written = col < a.cols && token < s.x.live;
+    const uint32_t q_keep = written ? a.q_keep : 0;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       q[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[kk][e] = (q[kk][e] & a.q_keep) ^ a.q_flip;
+      for (int e = 0; e < 4; ++e) q[kk][e] = (q[kk][e] & q_keep) ^ a.q_flip;
     }
     TreeState<D> st;
     const LdsBytes lds = (LdsBytes)&tiles[0][0][0];
@@ -770,7 +774,7 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
     for (const auto& o : st.o)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(o[r], 0.0f, sum);
-    const bool odd = __any(sum != sum);
+    const bool odd = __any(sum != sum && written);
     if (lane == 0) wrong[w] = odd;
     block_sync();
     if (wrong[0] | wrong[1] | wrong[2] | wrong[3]) {
@@ -820,7 +824,7 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
       a.parts[((int64_t)s.b * a.kv_heads + s.kvh) * a.col_tiles + s.tile] =
           u32x2{(uint32_t)slot, (uint32_t)parts};
     }
-    if (wk == 0 && col < a.cols && token < s.x.live) {
+    if (wk == 0 && written) {
       if (whole) {
         const int64_t row = ((int64_t)s.b * a.tokens + token) * a.q_heads + head;
         const float inv = st.m == -INFINITY && st.l == 0.0f ? 0.0f : 1.0f / st.l;
