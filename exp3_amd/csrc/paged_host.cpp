@@ -196,6 +196,12 @@ at::Tensor plain(const at::Tensor& x, const char* name) {
   return (x.is_neg() ? x.resolve_neg() : x).contiguous().detach();
 }
 
+// Whether two contiguous tensors have bytes in common.
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  const auto a = reinterpret_cast<uintptr_t>(x.data_ptr()), b = reinterpret_cast<uintptr_t>(y.data_ptr());
+  return x.numel() > 0 && y.numel() > 0 && a < b + y.nbytes() && b < a + x.nbytes();
+}
+
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const c10::Device& device) {
   return at::empty(shape, at::TensorOptions().dtype(type).device(device));
 }
@@ -631,6 +637,19 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (weights_out.sizes() != weights.sizes() || positions_out.sizes() != weights.sizes())
         refuse("out ", weights_out.sizes(), " and ", positions_out.sizes(), " differ from weights ",
                weights.sizes());
+      // A row is written while others are read: only in its own place.
+      bool shared = overlap(weights_out, positions_out) || overlap(positions_out, weights);
+      shared = shared || (weights_out.data_ptr() != weights.data_ptr() && overlap(weights_out, weights));
+      if (args[7] != Py_None) {
+        const at::Tensor& x = tensor(args[7], "positions");
+        shared = shared || overlap(weights_out, x) ||
+                 (positions_out.data_ptr() != x.data_ptr() && overlap(positions_out, x));
+      }
+      for (PyObject* read : {args[5], args[8]})
+        if (read != Py_None)
+          shared = shared || overlap(weights_out, tensor(read, "lengths")) ||
+                   overlap(positions_out, tensor(read, "lengths"));
+      if (shared) refuse("out must be the weights and positions themselves or overlap no argument");
     }
     const at::Tensor left = empty(lengths.sizes(), at::kInt, d.device);
     void* stream = reinterpret_cast<void*>(integer(args[14]));

@@ -267,8 +267,8 @@ def evict_tokens(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Ten
     positions: int32, as weights, -1 for tokens appended since (all of them: None): those have
     position ``seen[b] - lengths[b] + slot``; seen: int32 ``[B]``, tokens of the text so far (None:
     the lengths, right for the first eviction). Returned are the new lengths and the new ``weights``
-    and ``positions`` (0 and -1 behind the end), in ``out`` if given, which may be the tensors
-    themselves. Sequences within the budget, or with a token that has no place, keep all. Later
+    and ``positions`` (0 and -1 behind the end), in ``out`` if given: the tensors themselves, or
+    others that share no memory with an argument. Sequences within the budget, or with a token that has no place, keep all. Later
     tokens are appended with ``positions=``. Pages that are written to belong to one sequence."""
     return _run(lengths, "evict", cache, page_table, lengths, weights, positions, seen, budget,
                 recent, sinks, *(out if out is not None else (None, None)))

@@ -462,10 +462,11 @@ int spx_paged_accumulate_weights(const spx_paged_cache* cache, const void* q, co
  * cache: starts holds the lengths (tokens held; negative: a free slot), tokens is 1, counts is not read.
  * positions: int32, as weights, or NULL: -1 for all; slot s without one (negative) has position
  * seen[b] - length + s. seen: int32 [B], tokens of the text so far, or NULL: the lengths. recent + sinks
- * is at most the budget. weights_out, positions_out: the new values, 0 and -1 from the new length on
- * (they may be the inputs); lengths_out: int32 [B]. Sequences within the budget, longer than the page
- * table reaches, or with a token that has no place, keep all they have. Pages of the first `budget`
- * slots are written: they belong to one sequence. workspace: spx_paged_evict_workspace_bytes(...)
+ * is at most the budget. weights_out, positions_out: the new values, 0 and -1 from the new length on:
+ * the inputs themselves, or memory that no input shares. lengths_out: int32 [B], in memory of its own.
+ * Sequences within the budget, longer than the page table reaches, or with a token that has no place,
+ * keep all they have. Pages of the first `budget` slots are written: they belong to one sequence.
+ * workspace: spx_paged_evict_workspace_bytes(...)
  * bytes, 8-byte aligned. */
 int64_t spx_paged_evict_workspace_bytes(const spx_paged_cache* cache, int budget);
 int spx_paged_evict(const spx_paged_cache* cache, const float* weights, const int32_t* positions,
