@@ -664,11 +664,13 @@ paged_attn_kernel(PagedAttnArgs args) {
       acc.load_ids(limits, j0, w, lane);
       u32x4 q[KK];
       const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h;
+      // queries of padding may hold anything: 0, so that they are no reason to run again
+      const uint32_t q_keep = token < s.live ? a.q_keep : 0;
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         q[kk] = *reinterpret_cast<const u32x4*>(qr + KeyTile<D, kFour>::dim(kk, g));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q[kk][e] = (q[kk][e] & a.q_keep) ^ a.q_flip;
+        for (int e = 0; e < 4; ++e) q[kk][e] = (q[kk][e] & q_keep) ^ a.q_flip;
       }
       const HeadPages<D, kFour> pages(a, s.kvh);
       acc.template run<false>(pages, limits, q, a.scale_log2, j0, j1, w, lane, c, g);
