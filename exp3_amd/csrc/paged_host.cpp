@@ -11,8 +11,10 @@
 #include <limits.h>
 #include <stdarg.h>
 
+#include <algorithm>
 #include <sstream>
 #include <stdexcept>
+#include <utility>
 #include <vector>
 
 #include <ATen/TracerMode.h>
@@ -515,6 +517,19 @@ PyObject* keep_path(PyObject*, PyObject* const* args, Py_ssize_t n) {
       if (objects[i].held[2] == Py_None) d.c.key_scales = d.c.value_scales = nullptr;
       caches[i] = d.c;
     }
+    // Rows would move twice, the second time from places that the first has filled.
+    std::vector<std::pair<uintptr_t, size_t>> ranges;
+    ranges.reserve(4 * count);
+    for (const Pages& x : objects)
+      for (PyObject* page : x.held)
+        if (page != Py_None) {
+          const at::Tensor& held = THPVariable_Unpack(page);
+          ranges.emplace_back(reinterpret_cast<uintptr_t>(held.data_ptr()), held.nbytes());
+        }
+    std::sort(ranges.begin(), ranges.end());
+    for (size_t i = 1; i < ranges.size(); ++i)
+      if (ranges[i].first < ranges[i - 1].first + ranges[i - 1].second)
+        refuse("the caches' pages overlap each other");
     at::Tensor accepted, path, following;
     const int64_t *drafts = nullptr, *targets = nullptr;
     if (walk) {

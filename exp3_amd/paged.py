@@ -216,8 +216,8 @@ def accept_drafts(caches, page_table: torch.Tensor, starts: torch.Tensor, parent
     """The drafts that the model agrees with, moved into place in every cache -> (accepted int32
     ``[B]``, path int32 ``[B, T]``, following int64 ``[B]``).
 
-    caches: a PagedCache or those of all layers, alike but for their pages, no two the same. parents: as
-    ``draft_tree``; drafts, targets: int64 ``[B, T]``, a node's token and the token that the model
+    caches: a PagedCache or those of all layers, alike but for their pages, which share no memory (those
+    of the drafts' rows belong to one sequence). parents: as ``draft_tree``; drafts, targets: int64 ``[B, T]``, a node's token and the token that the model
     chose behind it. Node 0 (the last token that was decided) is accepted, then the first child whose
     draft is the target of the node accepted last, as long as there is one. ``path``: the accepted
     nodes, then -1; ``following``: the target of the last one, the next token. K and V of the

@@ -430,13 +430,14 @@ int spx_paged_tree_attention(const spx_paged_cache* cache, const void* q, const 
 
 /* Acceptance of drafted tokens: rows of K and V of an accepted path moved into place, from
  * starts[b] + path[b][j] to starts[b] + j, in all caches (the layers of a model: descriptions that
- * differ in their pages alone, no two with the same ones; read by the host before the call returns).
+ * differ in their pages alone, which share no memory; read by the host before the call returns).
  * Either with parents, drafts and targets, contiguous [B, T] (int32, int64, int64): node 0 is taken,
  * then the first child whose drafts equals the targets of the node taken last, while there is one.
  * accepted: int32 [B], how many were taken (0 without live tokens); path_out: int32 [B, T], their
  * indexes, then -1; following: int64 [B], the targets of the last one, or -1.
  * Or with path_in, int32 [B, T]: live indexes that ascend; it ends where one does not (the others
- * NULL). Rows from or to a position without a place are not moved. T is at most 256. */
+ * NULL). Rows from or to a position without a place are not moved. The outputs share no memory with an
+ * input. T is at most 256. */
 int spx_paged_keep_path(const spx_paged_cache* caches, int cache_count, const int32_t* parents,
                         const int64_t* drafts, const int64_t* targets, const int32_t* path_in,
                         int32_t* accepted, int32_t* path_out, int64_t* following, void* stream);
