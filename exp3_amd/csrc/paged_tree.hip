@@ -756,10 +756,9 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
     const bool idle = s.tile * kColumns + 32 * wc >= a.cols;
     u32x4 q[D / 16];
     const uint16_t* qr = a.q + s.b * a.qs_b + token * a.qs_t + head * a.qs_h + 8 * half;
-    // Queries of padding may hold anything: they count as 0, and what K and V make of them (columns
-    // that are not written) does not count as odd below.
-    const bool written = col < a.cols && token < s.x.live;
-    const uint32_t q_keep = written ? a.q_keep : 0;
+    // Queries of padding may hold anything: 0, so that such columns are odd (below) only where others
+    // are, from K and V.
+    const uint32_t q_keep = token < s.x.live ? a.q_keep : 0;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       q[kk] = *reinterpret_cast<const u32x4*>(qr + 16 * kk);
@@ -774,7 +773,7 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
     for (const auto& o : st.o)
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum = __builtin_fmaf(o[r], 0.0f, sum);
-    const bool odd = __any(sum != sum && written);
+    const bool odd = __any(sum != sum);
     if (lane == 0) wrong[w] = odd;
     block_sync();
     if (wrong[0] | wrong[1] | wrong[2] | wrong[3]) {
@@ -824,7 +823,7 @@ __global__ __launch_bounds__(kTreeThreads, TreeShape<D>::kPerCu) void paged_tree
       a.parts[((int64_t)s.b * a.kv_heads + s.kvh) * a.col_tiles + s.tile] =
           u32x2{(uint32_t)slot, (uint32_t)parts};
     }
-    if (wk == 0 && written) {
+    if (wk == 0 && col < a.cols && token < s.x.live) {
       if (whole) {
         const int64_t row = ((int64_t)s.b * a.tokens + token) * a.q_heads + head;
         const float inv = st.m == -INFINITY && st.l == 0.0f ? 0.0f : 1.0f / st.l;
