@@ -668,7 +668,7 @@ PyObject* evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const at::Tensor left = empty(lengths.sizes(), at::kInt, d.device);
     void* stream = reinterpret_cast<void*>(integer(args[14]));
-    if (d.c.batch > 0 && d.c.kv_heads > 0) {
+    if (d.c.batch > 0) {
       const int limit = (int)std::min<int64_t>(budget, INT_MAX);
       const int64_t bytes = spx_paged_evict_workspace_bytes(&d.c, limit);
       const at::Tensor workspace = empty({std::max<int64_t>(bytes, 16)}, at::kByte, d.device);

@@ -54,3 +54,11 @@ def test_outputs_side_by_side(gpu):
         got.append([left, w.clone(), p.clone(), cache.key_pages, cache.value_pages])
     for other in got[1:]:
         assert all(torch.equal(x, y) for x, y in zip(got[0], other))
+
+
+def test_a_cache_without_heads_is_refused(gpu):
+    """No kernel would run, and nothing write the lengths that come back."""
+    cache, table, lengths, *_ = _call()
+    none = paged.PagedCache(cache.key_pages[:, :0], cache.value_pages[:, :0])
+    with pytest.raises(ValueError, match="kv_heads"):
+        paged.evict_tokens(none, table, lengths, torch.zeros(2, 0, 128, device="cuda"), 40)
