@@ -29,7 +29,7 @@
 //     the A operand wants them; a lane holds its dims of the eight rows it needs, and byte
 //     permutes pair the keys. P goes through in three bf16 parts, 24 bits as in fp32, and its sums
 //     are products of the same parts with ones: products and LSE are those of an fp32 P. (Two parts
-//     leave 2^-18: an LSE off by up to 2^-17, which no rounding of the output covers. The third
+//     lose up to 2^-17, and an LSE is off by as much, which no rounding of the output covers. The third
 //     costs 2 to 6 % with 4-bit pages, 64 sequences of 8192 keys 114 -> 121 us, 131072 keys 25.3 ->
 //     26.8, and nothing with bf16 pages.) Where that makes NaN (infinite values of bf16 pages meet a
 //     part of P that is 0) the wave runs again with P as it is, v_mfma_f32_16x16x4_f32.

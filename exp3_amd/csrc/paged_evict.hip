@@ -11,10 +11,11 @@
 // budget that it drops. The kept ones move in a launch of their own, row and ledger, so that both
 // may be in place.
 //
-// Bound by the walks' instructions: a row is one workgroup's, so few long rows leave most CUs idle (1
-// x 4 heads of 32640 tokens to 4096: 30.6 us, 16 waves, + 5.6 for the moves; 64 x 8 heads of 2112 to
-// 2048: 16.7 + 8.3, the bytes of both 8). A row shared by workgroups would need a launch per digit,
-// some 3 us each, for what a prompt does once.
+// Bound by the walks' instructions and serial steps: a row is one workgroup's, so few long rows leave
+// most CUs idle (1 x 4 heads of 32640 tokens to 4096: 30.4 us, 16 waves, + 5.6 for the moves; 64 x 8
+// heads of 2112 to 2048: 16.3 + 8.4, the bytes of both 8). Rows shared by workgroups (one histogram of
+// more bits over all of them, few candidates left) would take a launch or two more; not built, and not
+// measured.
 #include <algorithm>
 
 #include "paged_moves.h"
@@ -28,7 +29,7 @@ constexpr int kFew = 64;                 // tokens that one wave ranks
 struct EvictArgs {
   PagedMap map;
   int64_t row;                           // elements of a row of weights and positions
-  int batch, budget, recent, sinks, room;
+  int budget, recent, sinks, room;
   const float* weights;                  // [B, Hkv, row]
   const int32_t* positions;              // the same, or null
   const int32_t* seen;                   // [B], or null: the lengths
@@ -390,7 +391,6 @@ extern "C" int spx_paged_evict(const spx_paged_cache* cache, const float* weight
   SPX_REQUIRE(rows <= 1 << 21, SPX_EINVAL, "%lld sequences x heads are more than 2^21",
               (long long)rows);
   a.row = row_stride;
-  a.batch = cache->batch;
   a.budget = budget; a.recent = recent; a.sinks = sinks;
   a.room = (int)evict_room(*cache, budget);
   a.weights = weights; a.positions = positions; a.seen = seen;
@@ -407,13 +407,12 @@ extern "C" int spx_paged_evict(const spx_paged_cache* cache, const float* weight
   if (launched != SPX_OK) return launched;
   MoveArgs m{};
   m.map = a.map;
-  m.batch = a.batch;
+  m.batch = cache->batch;
   m.room = a.room;
   m.pages = PagePointers{cache->key_pages, cache->value_pages, cache->key_scales, cache->value_scales};
   m.counts = a.counts;
   m.moves = a.moves;
   m.row = a.row;
-  m.lengths = lengths_out;
   m.seen = seen;
   m.weights = weights;
   m.positions = positions;

@@ -21,8 +21,7 @@ struct MoveArgs {
   const int32_t* counts;                 // [B, Hkv] moves of each list
   const u32x2* moves;                    // [B, Hkv, room] (to, from)
   int64_t row;                           // elements of a row of weights and positions
-  const int32_t* lengths;                // [B]: new lengths (the map's starts are the old ones)
-  const int32_t* seen;                   // [B], or null: the old lengths
+  const int32_t* seen;                   // [B], or null: the old lengths, which the map's starts are
   const float* weights;                  // [B, Hkv, row]
   const int32_t* positions;              // the same, or null
   float* weights_out;                    // these may be those

@@ -14,12 +14,14 @@
 // Between HBM and the matrix units: at 128 columns a unit's products take half as long as its bytes in
 // bf16, twice as long in 4 bits. So K and V are read once for 128 columns and are on their way a unit
 // and a half ahead, and a wave's softmax, or its widening of 4 bits, is issued between products. P goes
-// to the products in two bf16 parts, 2^-18 of it is lost; one part would save a third of the matrix
-// instructions and lose 2^-9, nearly as much as the output's own rounding.
+// to the products in two bf16 parts, which lose up to 2^-17 of it: an output is off by up to 2^-17 of
+// the sum of p |v|, and 0.12 % of the outputs round otherwise than with P in fp32. One part would save a
+// third of the matrix instructions and lose up to 2^-8, as much as the output's own rounding.
 //
-// 8 ragged sequences of up to 16000 keys, trees of 32, 32/8 heads, bf16: 81 us (3.9 TB/s) + 11 to join;
-// 16 of up to 8192 in 4 bits, trees of 61, 28/4 heads: 99 (0.48 PFLOP/s, 0.72 with both parts of P) + 11;
-// 4 of up to 12001 in 4 bits at D = 256, trees of 26, 16/4 heads: 41 + 8, one wave per SIMD (LDS).
+// 8 ragged sequences of up to 16000 keys, trees of 32, 32/8 heads, bf16: 79 us (4.0 TB/s) + 11 to join;
+// 16 of up to 8192 in 4 bits, trees of 61, 28/4 heads: 101 (0.47 PFLOP/s, 0.71 with both parts of P) + 11;
+// 4 of up to 12001 at D = 256, trees of 26, 16/4 heads: 40 + 9 in 4 bits and in bf16, one wave per SIMD
+// (LDS). The plan of a tree (below): 16 nodes 1.8 us, 64 trees of 61 3.2.
 #include <algorithm>
 #include <cmath>
 
@@ -347,8 +349,9 @@ __device__ __forceinline__ void tree_rescale(TreeState<D>& st, float corr) {
 #endif
 }
 
-// P of 32 keys in two bf16 parts, operands of two products over 16 keys each: 2^-18 of it is lost, an
-// output moves by at most 2^-9 of its own rounding. The sums take P as it is.
+// P of 32 keys in two bf16 parts, operands of two products over 16 keys each. Of a P in [2^e, 2^(e + 1))
+// the first part leaves up to 2^(e - 8), half a step, and the second, whose half steps are 2^-9 of that
+// or finer, up to 2^(e - 17). The sums take P as it is.
 struct TreeProbs {
   u32x4 hi[2], lo[2];
 };

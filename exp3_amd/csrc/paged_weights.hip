@@ -12,10 +12,11 @@
 //
 // Two kernels. Up to 16 columns (decode steps) a wave has Q in registers and walks the keys by itself, the
 // next 32 or 64 under way: bound by the pages' bytes (64 sequences of up to 8192 keys in 4 bits, 32/8
-// heads: 34 us, 4.7 TB/s). Else a wave holds 64 keys in registers and walks the columns, which the
-// workgroup copies into LDS a unit ahead: bound by the issue of three vector instructions a score beside
-// the products (2000 tokens over 16000 keys, 28/4 heads: 256 us, 0.84 PFLOP/s; scores of one tile spread
-// over the products of the next by hand: 265).
+// heads: 34 us, 5.0 TB/s). Else a wave holds 64 keys in registers and walks the columns, which the
+// workgroup copies into LDS a unit ahead: bound by three vector instructions a score and the products,
+// which overlap little (2000 tokens over 16000 keys, 28/4 heads: 243 us a call with the join, 0.88
+// PFLOP/s, matrix units busy 38 % of the time; scores of one tile spread over the products of the next
+// by hand: 265 for 256). At D = 128 that kernel spills 10 (bf16) or 11 registers (4 bits).
 #include <algorithm>
 #include <cmath>
 
@@ -58,7 +59,6 @@ struct PagedWeightArgs {
   const uint8_t* key_scales;
   const uint8_t* value_scales;
   int batch, tokens, q_heads, kv_heads, group;
-  int cols, chunks;                      // tokens x group, chunks of them at most
   int blocks;                            // blocks of keys that the table reaches
   int whole;                             // blocks are not shared by workgroups
   int grid;                              // workgroups, or waves, that share the work
@@ -631,8 +631,6 @@ extern "C" int spx_paged_accumulate_weights(const spx_paged_cache* cache, const 
   a.value_scales = static_cast<const uint8_t*>(cache->value_scales);
   a.batch = cache->batch; a.tokens = cache->tokens;
   a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.group = q_heads / cache->kv_heads;
-  a.cols = cache->tokens * a.group;
-  a.chunks = (int)z.chunks;
   a.whole = z.whole;
   a.blocks = (int)z.blocks;
   a.grid = z.grid;
