@@ -15,7 +15,7 @@
 // heads: 34 us, 5.0 TB/s). Else a wave holds 64 keys in registers and walks the columns, which the
 // workgroup copies into LDS a unit ahead: bound by three vector instructions a score and the products,
 // which overlap little (2000 tokens over 16000 keys, 28/4 heads: 243 us a call with the join, 0.88
-// PFLOP/s, matrix units busy 38 % of the time; scores of one tile spread over the products of the next
+// PFLOP/s, matrix units busy 46 % of the cycles; scores of one tile spread over the products of the next
 // by hand: 265 for 256). At D = 128 that kernel spills 10 (bf16) or 11 registers (4 bits).
 #include <algorithm>
 #include <cmath>
