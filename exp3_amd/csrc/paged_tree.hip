@@ -15,8 +15,10 @@
 // bf16, twice as long in 4 bits. So K and V are read once for 128 columns and are on their way a unit
 // and a half ahead, and a wave's softmax, or its widening of 4 bits, is issued between products. P goes
 // to the products in two bf16 parts, which lose up to 2^-17 of it: an output is off by up to 2^-17 of
-// the sum of p |v|, and 0.12 % of the outputs round otherwise than with P in fp32. One part would save a
-// third of the matrix instructions and lose up to 2^-8, as much as the output's own rounding.
+// the sum of p |v|, and 0.12 % of the outputs round otherwise than the plain fp32 form's. With a third
+// part it is 0.03 to 0.08 %, the order of the sums, for 5 to 17 % more time (in a graph 87.9 -> 103, 4
+// bits 113 -> 132, D = 256 50.2 -> 54.0 us). One part would save a third of the matrix instructions and
+// lose up to 2^-8, as much as the output's own rounding.
 //
 // 8 ragged sequences of up to 16000 keys, trees of 32, 32/8 heads, bf16: 79 us (4.0 TB/s) + 11 to join;
 // 16 of up to 8192 in 4 bits, trees of 61, 28/4 heads: 101 (0.47 PFLOP/s, 0.71 with both parts of P) + 11;
