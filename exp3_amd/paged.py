@@ -18,7 +18,7 @@ Common arguments:
   starts      int32 [B]: the position of each sequence's first new token, i.e. the tokens
               held before; negative for a free slot of the batch
   counts      int32 [B] or None: how many of the T new tokens of each sequence are tokens;
-              the rest is padding
+              the rest is padding, whose rows may hold anything
 
 A new token is live if its sequence is not a free slot, it is no padding, and the table
 reaches its position. Positions whose page id is outside the cache have no place: nothing is
